@@ -315,6 +315,133 @@ int inferc_dev_decode_attention(const float* q, const float* k_cache,
                                 int64_t heads, int64_t head_dim,
                                 int64_t max_len, int64_t L, void* stream);
 
+/* ------------------------------------------------- paged cache, many requests */
+
+/* The cache that a server's requests share: keys and values live in pages of
+ * page_size positions, [num_pages, kv_heads, page_size, head_dim] with free
+ * strides (in elements; the last is 1), so both head-major and token-major
+ * pages fit. Position p of sequence b is slot p % page_size of page
+ * page_table[b * table_stride + p / page_size]; only the entries that lens[b]
+ * positions need are read. No counterpart in the reference, whose decode
+ * grows one dense cache per request by Concat (src/kernels/movement.cc:142-189).
+ *
+ * dtype is an ONNX TensorProto code: 1 float, 10 float16, 16 bfloat16; it is
+ * the type of the caches and of every query, key, value and output row that
+ * meets them. head_dim: a multiple of 8, 8..256. Caches and rows are 16-byte
+ * aligned with strides that are multiples of 16 bytes. page_size * max_pages
+ * < 2^31. Sums, norms and softmax statistics are fp32; results are rounded to
+ * dtype once.
+ *
+ * A length, page id, token range or rotary position that points outside its
+ * buffer is never followed: the positions concerned are left out (attention; a
+ * negative length counts as 0, one past the table as its capacity, in evict
+ * too), or the row is not written (norm, append, evict), and the next
+ * inferc_dev_stream_synchronize on that device returns INFERC_ERR_RANGE. */
+typedef struct InfercPagedKv {
+  void* k;                   /* DEVICE */
+  void* v;                   /* DEVICE */
+  const int32_t* page_table; /* DEVICE [batch, max_pages] */
+  const int32_t* lens;       /* DEVICE [batch]: positions held, this step's tokens included */
+  int64_t k_page_stride, k_head_stride, k_token_stride;
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+  int64_t num_pages, kv_heads, page_size;
+  int64_t batch, max_pages, table_stride;
+  int32_t head_dim, dtype;
+} InfercPagedKv;
+
+/* What happens to every query and key head before it is used:
+ * y = x * gamma / sqrt(mean(x^2) + eps) over the head's head_dim values (a NULL
+ * gamma leaves that side as it is), then for each pair (a, b) of the first
+ * rotary_dim columns, with (c, s) = row `position` of the tables,
+ * (a c - b s, b c + a s). Pairs are columns (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) when interleaved. rotary_dim 0 rotates nothing. cos and sin
+ * are fp32 tables [table_len, rotary_dim / 2] with row stride table_stride,
+ * made once by the caller (far positions need 64-bit angles). positions may be
+ * NULL: the token's row index (qk_norm_rotary) or its slot in the cache
+ * (append). */
+typedef struct InfercHeadRotary {
+  const float* q_gamma;     /* DEVICE [head_dim] or NULL */
+  const float* k_gamma;     /* DEVICE [head_dim] or NULL */
+  const float* cos;         /* DEVICE */
+  const float* sin;         /* DEVICE */
+  const int32_t* positions; /* DEVICE [tokens] or NULL */
+  int64_t table_len, table_stride;
+  float eps;
+  int32_t rotary_dim, interleaved;
+} InfercHeadRotary;
+
+/* Norm and rotation of all query and key heads of `tokens` rows in one pass:
+ * row t's head h starts at q + t * q_token_stride + h * q_head_stride (so q
+ * and k may be column blocks of one projection), results likewise; q_out may
+ * be q and k_out may be k. q_heads or kv_heads may be 0. */
+int inferc_dev_qk_norm_rotary(const InfercHeadRotary* rot, int dtype, const void* q,
+                              int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                              int64_t k_token_stride, int64_t k_head_stride, void* q_out,
+                              int64_t q_out_token_stride, int64_t q_out_head_stride, void* k_out,
+                              int64_t k_out_token_stride, int64_t k_out_head_stride,
+                              int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                              int64_t head_dim, void* stream);
+
+/* The paged form of inferc_dev_kv_append: writes `tokens` new key and value
+ * rows into the cache. Sequence b's new tokens are rows cu_tokens[b] ..
+ * cu_tokens[b+1] - 1 (cu_tokens: DEVICE [batch + 1], not decreasing, from 0;
+ * NULL: one token per sequence, tokens == batch) and become its last
+ * positions, lens[b] counting them already. Rows behind the last sequence are
+ * left alone, q's among them. rot may be NULL (plain append); with it keys are
+ * normed and rotated on the way, and so are the queries of the same rows when
+ * q_heads > 0 (q -> q_out, in place allowed). Values are copied as they are.
+ * Two sequences that share a page may read it, but not append into it. */
+int inferc_dev_paged_kv_append(const InfercPagedKv* kv, const InfercHeadRotary* rot,
+                               const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                               const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                               void* q_out, int64_t q_out_token_stride,
+                               int64_t q_out_head_stride, int64_t q_heads,
+                               const int32_t* cu_tokens, int64_t tokens, void* stream);
+
+/* The paged, batched form of inferc_dev_decode_attention: one new token per
+ * sequence, out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j over the
+ * sequence's lens[b] positions; q_heads is a multiple of kv_heads, query head h
+ * reads key head h / (q_heads / kv_heads). A sequence of length 0 gives zeros.
+ * weights may be NULL; otherwise fp32 [batch, kv_heads, >= max_pages *
+ * page_size] in the order of positions, to which each position's softmax
+ * weight is added, summed over the query heads of its key head (in a fixed
+ * order: equal calls give equal bits). workspace: DEVICE scratch of at least
+ * inferc_dev_paged_decode_attention_workspace() bytes, 16-byte aligned, which
+ * no other call in flight may use; calls (or captured graphs) that may overlap
+ * need one each. That size depends on the sizes in kv, q_heads and on whether
+ * weights are kept, not on lens; it is -1 for sizes the call would refuse. */
+int64_t inferc_dev_paged_decode_attention_workspace(const InfercPagedKv* kv, int64_t q_heads,
+                                                    int with_weights);
+int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,
+                                      int64_t q_batch_stride, int64_t q_head_stride,
+                                      int64_t q_heads, float scale, void* out,
+                                      int64_t out_batch_stride, int64_t out_head_stride,
+                                      float* weights, int64_t weights_batch_stride,
+                                      int64_t weights_head_stride, void* workspace,
+                                      int64_t workspace_bytes, void* stream);
+
+/* Trims every sequence longer than `keep` to `keep` positions per key head: the
+ * last `recent` stay, and of the others the keep - recent with the largest
+ * weight (weights as inferc_dev_paged_decode_attention keeps them; equal
+ * weights: the lower position stays; a NaN counts as the largest). What stays
+ * moves to positions 0 .. keep - 1 in its order, in keys, values and weights.
+ * Other sequences stay whole. keep >= 1, 0 <= recent <= keep.
+ * dst_table: page table of the result [batch, dst_max_pages], dst_max_pages *
+ * page_size >= min(keep, max_pages * page_size). NULL: in place, in the
+ * sequence's own pages. Otherwise the pages it names are not in page_table
+ * (needed when sequences share pages). weights_out: like weights, or NULL for
+ * in place; of row (b, h), positions 0 .. lens[b] - 1 are written, those from
+ * keep on with 0. lens_out [batch] receives min(lens[b], keep) and may not be
+ * lens itself. kept [batch, kv_heads, keep] receives the old positions, -1
+ * behind the last. */
+int inferc_dev_paged_kv_evict(const InfercPagedKv* kv, const int32_t* dst_table,
+                              int64_t dst_max_pages, int64_t dst_table_stride, float* weights,
+                              int64_t weights_batch_stride, int64_t weights_head_stride,
+                              float* weights_out, int64_t weights_out_batch_stride,
+                              int64_t weights_out_head_stride, int64_t keep, int64_t recent,
+                              int32_t* lens_out, int32_t* kept, void* stream);
+
 /* ------------------------------------------------------- graph executor */
 
 /* A device executor for an optimized inferc plan: the ONNX model `inferc

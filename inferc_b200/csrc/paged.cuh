@@ -1,0 +1,125 @@
+// The paged cache's device view: element types, row access, page lookup and
+// the flag for indexes that point outside their buffers. Shared by
+// paged_kv.cu (norm, rotation, append, evict) and paged_attention.cu.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace inferc_dev {
+namespace paged {
+
+enum DType : int { F32 = 1, F16 = 10, BF16 = 16 };  // ONNX TensorProto codes
+
+// Unsigned division by a constant of the launch: q = (n * m) >> 32 >> s with
+// m = ceil(2^(32+s) / d), s = ceil(log2 d) is exact for n < 2^31 when formed
+// in 64 bits with m < 2^33; m is kept as 2^32 + mul.
+struct FastDiv {
+  uint32_t d = 1, mul = 0, shift = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t d_) : d(d_) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __host__ __device__ uint32_t div(uint32_t n) const {
+#ifdef __CUDA_ARCH__
+    const uint32_t hi = __umulhi(n, mul);
+#else
+    const uint32_t hi = (uint32_t)(((uint64_t)n * mul) >> 32);
+#endif
+    return (uint32_t)(((uint64_t)hi + n) >> shift);
+  }
+  __host__ __device__ uint32_t mod(uint32_t n) const { return n - div(n) * d; }
+};
+
+// Eight consecutive values of a row (one 16-byte load of a 16-bit type, two
+// of fp32), widened to fp32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (std::is_same_v<T, float>) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0];
+    const float4 b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 f;
+      if constexpr (std::is_same_v<T, __half>)
+        f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      else
+        f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* x) {
+  if constexpr (std::is_same_v<T, float>) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Device arguments of every paged kernel: the caller's descriptor, the
+// division by the page size, and the flag raised by an index that points
+// outside its buffer.
+struct Args {
+  InfercPagedKv kv;
+  FastDiv page;
+  int* flag;
+};
+
+// Positions of sequence b, clamped into what its page table can name.
+__device__ __forceinline__ int seq_len(const Args& a, int64_t b) {
+  const int n = a.kv.lens[b];
+  const int cap = (int)(a.kv.max_pages * a.kv.page_size);
+  if (n >= 0 && n <= cap) return n;
+  *a.flag = 1;
+  return n < 0 ? 0 : cap;
+}
+
+// Page of position p of a sequence whose table row is `row`; -1 (and the
+// flag) when the id is no page.
+__device__ __forceinline__ int page_of(const Args& a, const int32_t* row, uint32_t index) {
+  const int id = row[index];
+  if (id >= 0 && id < a.kv.num_pages) return id;
+  *a.flag = 1;
+  return -1;
+}
+
+// Address of the flag on the current device; read_and_clear_paged_range()
+// (inferc_dev_stream_synchronize) reports it.
+int* range_flag_ptr();
+// Throws INFERC_ERR_INVALID when the descriptor is not one the kernels take.
+void check_kv(const InfercPagedKv* kv, const char* op);
+void check_rows(const char* op, const char* what, const void* p, int64_t stride_a,
+                int64_t stride_b, int dtype);
+int elem_bytes(int dtype);
+
+}  // namespace paged
+
+int read_and_clear_paged_range();
+
+}  // namespace inferc_dev

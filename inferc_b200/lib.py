@@ -25,6 +25,24 @@ class Int4Gemv(ctypes.Structure):
     _fields_ = [("w", _p), ("scales", _p), ("x", _p), ("y", _p), ("n", _i64), ("k", _i64)]
 
 
+class PagedKv(ctypes.Structure):
+    """Mirror of InfercPagedKv."""
+
+    _fields_ = [(n, _p) for n in ("k", "v", "page_table", "lens")] + [
+        (n, _i64) for n in ("k_page_stride", "k_head_stride", "k_token_stride", "v_page_stride",
+                            "v_head_stride", "v_token_stride", "num_pages", "kv_heads",
+                            "page_size", "batch", "max_pages", "table_stride")] + [
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class HeadRotary(ctypes.Structure):
+    """Mirror of InfercHeadRotary."""
+
+    _fields_ = [(n, _p) for n in ("q_gamma", "k_gamma", "cos", "sin", "positions")] + [
+        ("table_len", _i64), ("table_stride", _i64), ("eps", _f),
+        ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
 # name -> (argtypes, restype); restype None means void.
 SIGNATURES: dict[str, tuple[list, object]] = {
     "inferc_dev_last_error_string": ([], ctypes.c_char_p),
@@ -71,6 +89,13 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "inferc_dev_argmax": ([_p, _i64, _p, _p], _i),
     "inferc_dev_kv_append": ([_p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p], _i),
     "inferc_dev_decode_attention": ([_p, _p, _p, _p, _i64, _i64, _i64, _i64, _p], _i),
+    "inferc_dev_qk_norm_rotary": ([_p, _i] + [_p, _i64, _i64] * 4 + [_i64] * 4 + [_p], _i),
+    "inferc_dev_paged_kv_append": ([_p, _p] + [_p, _i64, _i64] * 4 + [_i64, _p, _i64, _p], _i),
+    "inferc_dev_paged_decode_attention_workspace": ([_p, _i64, _i], _i64),
+    "inferc_dev_paged_decode_attention": ([_p, _p, _i64, _i64, _i64, _f, _p, _i64, _i64, _p, _i64,
+                                           _i64, _p, _i64, _p], _i),
+    "inferc_dev_paged_kv_evict": ([_p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64,
+                                   _p, _p, _p], _i),
     "inferc_dev_graph_describe": ([_p, _sz, _p, _sz, ctypes.POINTER(_sz)], _i),
     "inferc_dev_graph_load": ([_p, _sz, ctypes.POINTER(_p)], _i),
     "inferc_dev_graph_set_input": ([_p, ctypes.c_char_p, _i, _p, _i, _p, _i, _p], _i),

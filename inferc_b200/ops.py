@@ -14,6 +14,10 @@ Reference signatures (src/kernels/*.h):
   Gemm(a, b, c, alpha, beta, trans_a, trans_b)  matmul.h:19
   MatMul(a, b)                                  matmul.h:17
   Gelu / GeluTanh / Softmax(x, axis)            activation.h:14-24
+
+The operators of a cache that many requests share (PagedKV, PagedKVAppend,
+QKNormRotary, QKNormRotaryAppend, PagedDecodeAttention, PagedKVEvict) have no
+reference counterpart; they are defined in inferc_b200/paged.py.
 """
 from __future__ import annotations
 
@@ -23,10 +27,14 @@ import torch
 
 from . import lib as _lib
 from .lib import InfercError, Int4Gemv
+from .paged import (PagedDecodeAttention, PagedKV, PagedKVAppend, PagedKVEvict, QKNormRotary,
+                    QKNormRotaryAppend, RotaryTable)
 
 __all__ = ["FusedMatMulAddGELU", "FusedQKVProjection", "FusedAttention", "LayerNorm", "Gemm",
            "MatMul", "Gelu", "GeluTanh", "Softmax", "Gemv", "Int4GemvRowScale",
-           "Int4GemvBatched", "Argmax", "InfercError"]
+           "Int4GemvBatched", "Argmax", "PagedKV", "PagedKVAppend", "QKNormRotary",
+           "QKNormRotaryAppend", "PagedDecodeAttention", "PagedKVEvict", "RotaryTable",
+           "InfercError"]
 
 
 def _stream() -> int:
