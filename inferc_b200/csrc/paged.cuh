@@ -9,32 +9,12 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "paged_plan.h"
 
 namespace inferc_dev {
 namespace paged {
 
 enum DType : int { F32 = 1, F16 = 10, BF16 = 16 };  // ONNX TensorProto codes
-
-// Unsigned division by a constant of the launch: q = (n * m) >> 32 >> s with
-// m = ceil(2^(32+s) / d), s = ceil(log2 d) is exact for n < 2^31 when formed
-// in 64 bits with m < 2^33; m is kept as 2^32 + mul.
-struct FastDiv {
-  uint32_t d = 1, mul = 0, shift = 0;
-  FastDiv() = default;
-  explicit FastDiv(uint32_t d_) : d(d_) {
-    while ((1ull << shift) < d) ++shift;
-    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __host__ __device__ uint32_t div(uint32_t n) const {
-#ifdef __CUDA_ARCH__
-    const uint32_t hi = __umulhi(n, mul);
-#else
-    const uint32_t hi = (uint32_t)(((uint64_t)n * mul) >> 32);
-#endif
-    return (uint32_t)(((uint64_t)hi + n) >> shift);
-  }
-  __host__ __device__ uint32_t mod(uint32_t n) const { return n - div(n) * d; }
-};
 
 // Eight consecutive values of a row (one 16-byte load of a 16-bit type, two
 // of fp32), widened to fp32.

@@ -1,145 +1,270 @@
-// Attention of one new token per sequence over the paged cache
-// (inferc_dev_paged_decode_attention).
+// Attention of one new token per sequence over the paged cache: entry points,
+// the join of sequences that several warps read, and the running sums of
+// attention weights. paged_attention.cuh reads the cache.
 #include <algorithm>
 #include <string>
 
-#include "paged.cuh"
+#include "paged_attention.cuh"
 
 namespace inferc_dev {
 namespace paged {
 namespace {
 
-struct AttendArgs {
-  Args a;
-  const void* q;
-  int64_t q_batch, q_head;
-  void* out;
-  int64_t o_batch, o_head;
-  float scale;  // times log2(e)
-  int group;    // query heads per key head
-  float* scores;  // [batch, q_heads, capacity] scaled scores in the log2 domain, or nullptr
-  float* stats;   // [batch, q_heads, 2] maximum and 1 / sum
-  int64_t capacity;
-  float* w;
-  int64_t w_batch, w_head;
+constexpr int kSMs = 148;  // B200; elsewhere the grid runs in waves
+constexpr int kLeast = 4;
+constexpr int kJoinThreads = 256;
+
+// The parts of one (sequence, head block): warp `first`'s second slot, then
+// the first slots of the warps behind it.
+struct Parts {
+  int64_t first;
+  int count;
+  __device__ __forceinline__ int64_t slot(int i) const {
+    return i == 0 ? 2 * first + 1 : 2 * (first + i);
+  }
 };
 
-constexpr int kThreads = 256;
-
-// One block per (query head, sequence); G lanes share a key.
-template <typename T, int G>
-__global__ void attend_kernel(const __grid_constant__ AttendArgs g) {
-  constexpr int kSubs = kThreads / G;
-  __shared__ float sm_m[kSubs], sm_l[kSubs];
-  extern __shared__ float sm_o[];  // [kSubs][d]
-  const InfercPagedKv& kv = g.a.kv;
-  const int h = blockIdx.x, d = kv.head_dim, tid = threadIdx.x;
-  const int64_t b = blockIdx.y;
-  const int c = tid % G, sub = tid / G, hk = h / g.group;
-  const int n = seq_len(g.a, b);
-  const bool live = c * 8 < d;
-  T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + h * g.o_head;
-  float q[8] = {}, o[8] = {}, m = -INFINITY, l = 0.f;
-  if (live) load8(reinterpret_cast<const T*>(g.q) + b * g.q_batch + h * g.q_head + c * 8, q);
-  const int32_t* row = kv.page_table + b * kv.table_stride;
-  const T* kc = reinterpret_cast<const T*>(kv.k) + hk * kv.k_head_stride + c * 8;
-  const T* vc = reinterpret_cast<const T*>(kv.v) + hk * kv.v_head_stride + c * 8;
-  float* scores = g.scores ? g.scores + (b * gridDim.x + h) * g.capacity : nullptr;
-  for (int j0 = 0; j0 < n; j0 += kSubs) {
-    const int j = j0 + sub;
-    int page = -1;
-    uint32_t slot = 0;
-    if (j < n) {
-      const uint32_t index = g.a.page.div(j);
-      slot = j - index * g.a.page.d;
-      page = page_of(g.a, row, index);
-    }
-    float x[8] = {}, s = 0.f;
-    if (page >= 0 && live) load8(kc + page * kv.k_page_stride + slot * kv.k_token_stride, x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += q[i] * x[i];
-#pragma unroll
-    for (int off = G / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= g.scale;
-    if (j >= n) continue;
-    if (page < 0) s = -INFINITY;
-    if (scores && c == 0) scores[j] = s;
-    if (page < 0) continue;
-    const float m2 = fmaxf(m, s);
-    const float base = m2 == -INFINITY ? 0.f : m2;
-    const float keep = exp2f(m - base), p = exp2f(s - base);
-    m = m2;
-    l = l * keep + p;
-    if (live) load8(vc + page * kv.v_page_stride + slot * kv.v_token_stride, x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = o[i] * keep + p * x[i];
-  }
-  if (c == 0) sm_m[sub] = m, sm_l[sub] = l;
-  if (live)
-    for (int i = 0; i < 8; ++i) sm_o[sub * d + c * 8 + i] = o[i];
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < kSubs; ++s) top = fmaxf(top, sm_m[s]);
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int s = 0; s < kSubs; ++s) sum += sm_l[s] * exp2f(sm_m[s] - base);
-  const float inv = n == 0 ? 0.f : 1.0f / sum;
-  if (tid == 0 && g.stats) {
-    g.stats[2 * (b * gridDim.x + h)] = base;
-    g.stats[2 * (b * gridDim.x + h) + 1] = inv;
-  }
-  if (tid < d / 8) {
-    float r[8] = {};
-    for (int s = 0; s < kSubs; ++s) {
-      const float f = exp2f(sm_m[s] - base);
-      for (int i = 0; i < 8; ++i) r[i] += f * sm_o[s * d + tid * 8 + i];
-    }
-    for (int i = 0; i < 8; ++i) r[i] = n == 0 ? 0.f : r[i] * inv;
-    store8(out + tid * 8, r);
-  }
-}
-
-// Adds each position's softmax weight, summed over the group's query heads.
-__global__ void weights_kernel(const __grid_constant__ AttendArgs g) {
-  const InfercPagedKv& kv = g.a.kv;
-  const int64_t b = blockIdx.y / kv.kv_heads;
-  const int h = blockIdx.y % kv.kv_heads;
-  const int64_t q_heads = kv.kv_heads * g.group;
-  const int n = seq_len(g.a, b);
-  float* w = g.w + b * g.w_batch + h * g.w_head;
-  for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < n; j += gridDim.x * blockDim.x) {
-    float sum = 0.f;
-    for (int i = 0; i < g.group; ++i) {
-      const int64_t r = b * q_heads + h * g.group + i;
-      sum += exp2f(g.scores[r * g.capacity + j] - g.stats[2 * r]) * g.stats[2 * r + 1];
-    }
-    w[j] += sum;
-  }
-}
-
+// Joins what several warps left of a (sequence, head block):
+//   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+// One block per cut head block (or per share of its heads, grid.y). Its jobs
+// are found by (sequence, head block) where those are fewer than the warps,
+// else by the warp that left the first part. A few hundred floats per part:
+// bound by latency, so a part's values are spread over the threads first and
+// the parts over what threads are left.
 template <typename T>
-void launch(const AttendArgs& g, cudaStream_t st) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttendArgs g,
+                                                            bool by_warp) {
+  __shared__ float s_max[16], s_inv[16];
+  __shared__ float4 s_sum[kJoinThreads];
   const InfercPagedKv& kv = g.a.kv;
-  const int d = kv.head_dim;
-  const dim3 grid((unsigned)(kv.kv_heads * g.group), (unsigned)kv.batch);
-  if (d <= 64) attend_kernel<T, 8><<<grid, kThreads, kThreads / 8 * d * 4, st>>>(g);
-  else if (d <= 128) attend_kernel<T, 16><<<grid, kThreads, kThreads / 16 * d * 4, st>>>(g);
-  else attend_kernel<T, 32><<<grid, kThreads, kThreads / 32 * d * 4, st>>>(g);
-  IDEV_LAUNCHED();
-  if (g.w) {
-    weights_kernel<<<dim3(32, (unsigned)(kv.batch * kv.kv_heads)), 256, 0, st>>>(g);
-    IDEV_LAUNCHED();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int heads = (int)kv.kv_heads * g.blocks, d = kv.head_dim;
+  pdl_wait();
+  const int64_t total = g.before[kv.batch];
+  if (total == 0) return;
+  const int64_t used = warps_used(total, g.warps, g.least);
+  int64_t b, head;
+  if (by_warp) {
+    b = g.jobs[2 * (int64_t)blockIdx.x];
+    head = g.jobs[2 * (int64_t)blockIdx.x + 1];
+    if (b < 0) return;
+  } else {
+    b = blockIdx.x / heads;
+    head = blockIdx.x % heads;
+  }
+  const int64_t tiles = (g.before[b + 1] - g.before[b]) / heads;
+  if (tiles == 0) return;
+  const int64_t t0 = g.before[b] + head * tiles;
+  Parts parts;
+  parts.first = owner_of(t0, total, used);
+  parts.count = (int)(owner_of(t0 + tiles - 1, total, used) - parts.first) + 1;
+  if (parts.count == 1) return;
+
+  const int hk = (int)(head / g.blocks), q0 = hk * g.group + (int)(head % g.blocks) * g.block;
+  const int cols = min(g.block, hk * g.group + g.group - q0);
+  const int h0 = cols * (int)blockIdx.y / (int)gridDim.y;
+  const int h1 = cols * ((int)blockIdx.y + 1) / (int)gridDim.y;
+  if (h0 == h1) return;
+  for (int h = h0 + warp; h < h1; h += kJoinThreads / 32) {
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < parts.count; i += 32)
+      m = fmaxf(m, g.part_ml[(parts.slot(i) * g.block + h) * 2]);
+    m = warp_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int i = lane; i < parts.count; i += 32) {
+      const float2 x =
+          reinterpret_cast<const float2*>(g.part_ml)[parts.slot(i) * g.block + h];
+      l += ex2(x.x - base) * x.y;
+    }
+    l = warp_sum(l);
+    if (lane == 0) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      s_max[h] = base;
+      s_inv[h] = inv;
+      if (g.stats) {
+        const int64_t r = b * (int64_t)(kv.kv_heads * g.group) + q0 + h;
+        g.stats[2 * r] = base;
+        g.stats[2 * r + 1] = inv;
+      }
+    }
+  }
+  __syncthreads();
+
+  const int quads = d / 4, items = (h1 - h0) * quads;  // float4s of the result
+  const int shares = max(1, min(kJoinThreads / max(items, 1), parts.count));
+  const int share = tid / items, item0 = tid % items;
+  T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + q0 * g.o_head;
+  for (int item = shares > 1 ? item0 : tid; item < items; item += kJoinThreads) {
+    const int h = h0 + item / quads, quad = item % quads;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (shares == 1 || share < shares) {
+#pragma unroll 4
+      for (int i = shares > 1 ? share : 0; i < parts.count; i += shares) {
+        const int64_t row = parts.slot(i) * g.block + h;
+        const float f = ex2(g.part_ml[row * 2] - s_max[h]);
+        const float4 x = reinterpret_cast<const float4*>(g.part_o + row * d)[quad];
+        sum.x += f * x.x;
+        sum.y += f * x.y;
+        sum.z += f * x.z;
+        sum.w += f * x.w;
+      }
+    }
+    if (shares > 1) {  // every thread passes here at most once, all of them together
+      s_sum[tid] = sum;
+      __syncthreads();
+      if (share == 0)
+        for (int s = 1; s < shares; ++s) {
+          const float4 x = s_sum[s * items + item];
+          sum.x += x.x;
+          sum.y += x.y;
+          sum.z += x.z;
+          sum.w += x.w;
+        }
+    }
+    if (shares == 1 || share == 0) {
+      const float inv = s_inv[h];
+      T* to = out + h * g.o_head + quad * 4;
+      to[0] = T(sum.x * inv);
+      to[1] = T(sum.y * inv);
+      to[2] = T(sum.z * inv);
+      to[3] = T(sum.w * inv);
+    }
   }
 }
 
-int64_t workspace_bytes(const InfercPagedKv& kv, int64_t q_heads, bool weights) {
-  const int64_t rows = kv.batch * q_heads;
-  return weights ? rows * (kv.max_pages * kv.page_size + 2) * 4 : 0;
+// Adds each position's softmax weight, 2^(s - M) / L summed over the query
+// heads of its key head in their order, to the running sum. The positions are
+// cut among the warps like the tiles.
+constexpr int kSumThreads = 256;
+
+__global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant__ AttendArgs g,
+                                                           int64_t warps) {
+  const InfercPagedKv& kv = g.a.kv;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * (kSumThreads / 32) + (threadIdx.x >> 5);
+  const int hk_n = (int)kv.kv_heads;
+  const int64_t q_heads = kv.kv_heads * g.group;
+  pdl_wait();
+  // tiles of one head per key head, not per block of query heads
+  const int64_t total = g.before[kv.batch] / g.blocks;
+  if (total == 0) return;
+  const int64_t used = warps_used(total, warps, 2);
+  if (w >= used) return;
+  const int64_t t0 = first_tile(w, total, used), t1 = first_tile(w + 1, total, used);
+  // the sequence that holds t0: 32 probes a step
+  int64_t b = 0, size = kv.batch;
+  while (size > 1) {
+    const int64_t step = (size + 31) / 32;
+    const bool below = lane * step < size && g.before[b + lane * step] / g.blocks <= t0;
+    const int n = __popc(__ballot_sync(0xffffffffu, below));
+    b += (n - 1) * step;
+    size = min(step, size - (n - 1) * step);
+  }
+  int64_t t = t0;
+  while (t < t1) {
+    const int64_t first = g.before[b] / g.blocks, after = g.before[b + 1] / g.blocks;
+    if (first == after) {
+      ++b;
+      continue;
+    }
+    const int64_t tiles = (after - first) / hk_n;
+    const int h = (int)((t - first) / tiles);
+    const int64_t from = (t - first) - h * tiles;  // tiles of this head: [from, upto)
+    const int64_t upto = min(tiles, from + (t1 - t));
+    const int n = min((int64_t)seq_len(g.a, b), upto * kTile);
+    const int64_t r = b * q_heads + (int64_t)h * g.group;
+    const float* s = g.scores + r * g.capacity;
+    float* sum = g.w + b * g.w_batch + h * g.w_head;
+    for (int j = (int)from * kTile + lane; j < n; j += 32) {
+      float p = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < g.group; ++i) {
+        const float2 st = reinterpret_cast<const float2*>(g.stats)[r + i];
+        p += ex2(s[i * g.capacity + j] - st.x) * st.y;
+      }
+      sum[j] += p;
+    }
+    t += upto - from;
+    if (upto == tiles && h + 1 == hk_n) ++b;
+  }
+}
+
+int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+
+int block_of(int64_t group) {
+  const int64_t blocks = (group + 15) / 16;
+  return (int)((group + blocks - 1) / blocks);
+}
+
+// Sizes of the work and of its scratch; those parts of AttendArgs that the
+// sizes decide.
+struct Plan {
+  AttendArgs g{};
+  bool cut;  // a sequence may be read by several warps
+  int64_t bytes = 0;
+};
+
+Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
+  Plan p;
+  AttendArgs& g = p.g;
+  g.group = (int)(q_heads / kv.kv_heads);
+  g.block = block_of(g.group);
+  g.blocks = (g.group + g.block - 1) / g.block;
+  g.capacity = kv.max_pages * kv.page_size;
+  g.least = kLeast;
+  const int64_t tiles = (g.capacity + kTile - 1) / kTile;
+  const int per_sm = kv.dtype == F32    ? blocks_per_sm<float>(kv.head_dim)
+                     : kv.dtype == F16 ? blocks_per_sm<__half>(kv.head_dim)
+                                       : blocks_per_sm<__nv_bfloat16>(kv.head_dim);
+  const int64_t most = kv.batch * kv.kv_heads * g.blocks * tiles;
+  g.warps = std::max<int64_t>(1, std::min<int64_t>((int64_t)kSMs * per_sm * kWarps, most));
+  // With at most kLeast tiles each, no (sequence, head block) is worth cutting, but the
+  // shares still end inside one unless it is a single tile.
+  p.cut = tiles > 1;
+  auto take = [&](int64_t bytes) {
+    char* at = ws + p.bytes;
+    p.bytes += align16(bytes);
+    return at;
+  };
+  if (p.cut || weights) g.before = reinterpret_cast<int64_t*>(take((kv.batch + 1) * 8));
+  if (p.cut) {
+    g.jobs = reinterpret_cast<int32_t*>(take(g.warps * 8));
+    g.part_ml = reinterpret_cast<float*>(take(2 * g.warps * g.block * 8));
+    g.part_o = reinterpret_cast<float*>(take(2 * g.warps * g.block * kv.head_dim * 4));
+  }
+  if (weights) {
+    g.stats = reinterpret_cast<float*>(take(kv.batch * q_heads * 8));
+    g.scores = reinterpret_cast<float*>(take(kv.batch * q_heads * g.capacity * 4));
+  }
+  return p;
 }
 
 void check(const InfercPagedKv* kv, int64_t q_heads) {
   check_kv(kv, "PagedDecodeAttention");
   IDEV_CHECK_ARG(q_heads >= 1 && q_heads <= 65535 && q_heads % kv->kv_heads == 0,
                  "PagedDecodeAttention: q_heads must be a multiple of kv_heads");
+  IDEV_CHECK_ARG(kv->batch * q_heads <= INT32_MAX, "PagedDecodeAttention: too many heads in one call");
+}
+
+template <typename T>
+void run(const Plan& p, cudaStream_t st) {
+  const AttendArgs& g = p.g;
+  const InfercPagedKv& kv = g.a.kv;
+  launch_attend<T>(g, st);
+  if (p.cut) {
+    const int64_t pairs = kv.batch * kv.kv_heads * g.blocks;
+    const bool by_warp = pairs > g.warps;
+    const int64_t jobs = by_warp ? g.warps : pairs;
+    // few jobs: their heads go to blocks of their own
+    const int split = (int)std::min<int64_t>(g.block, std::max<int64_t>(1, 4 * kSMs / jobs));
+    launch_pdl(join_kernel<T>, dim3((unsigned)jobs, (unsigned)split), dim3(kJoinThreads), 0, st, g,
+               by_warp);
+  }
+  if (g.w) {
+    const int64_t warps = (int64_t)kSMs * 64;
+    launch_pdl(sums_kernel, dim3((unsigned)(warps * 32 / kSumThreads)), dim3(kSumThreads), 0, st, g,
+               warps);
+  }
 }
 
 }  // namespace
@@ -156,7 +281,7 @@ int64_t inferc_dev_paged_decode_attention_workspace(const InfercPagedKv* kv, int
   int64_t bytes = -1;
   guard([&] {
     check(kv, q_heads);
-    bytes = workspace_bytes(*kv, q_heads, with_weights != 0);
+    bytes = plan_of(*kv, q_heads, with_weights != 0, nullptr).bytes;
   });
   return bytes;
 }
@@ -167,17 +292,17 @@ int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,
                                       int64_t out_batch_stride, int64_t out_head_stride,
                                       float* weights, int64_t weights_batch_stride,
                                       int64_t weights_head_stride, void* workspace,
-                                      int64_t workspace_bytes_given, void* stream) {
+                                      int64_t workspace_bytes, void* stream) {
   return guard([&] {
     const char* op = "PagedDecodeAttention";
     check(kv, q_heads);
     if (kv->batch == 0) return;
     check_rows(op, "query", q, q_batch_stride, q_head_stride, kv->dtype);
     check_rows(op, "output", out, out_batch_stride, out_head_stride, kv->dtype);
-    const int64_t need = workspace_bytes(*kv, q_heads, weights != nullptr);
-    IDEV_CHECK_ARG(workspace_bytes_given >= need && (need == 0 || (workspace && aligned16(workspace))),
+    Plan p = plan_of(*kv, q_heads, weights != nullptr, static_cast<char*>(workspace));
+    IDEV_CHECK_ARG(workspace_bytes >= p.bytes && (p.bytes == 0 || (workspace && aligned16(workspace))),
                    "PagedDecodeAttention: the workspace is too small or not 16-byte aligned");
-    AttendArgs g{};
+    AttendArgs& g = p.g;
     g.a.kv = *kv;
     g.a.page = FastDiv((uint32_t)kv->page_size);
     g.a.flag = range_flag_ptr();
@@ -188,19 +313,13 @@ int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,
     g.o_batch = out_batch_stride;
     g.o_head = out_head_stride;
     g.scale = scale * 1.4426950408889634f;
-    g.group = (int)(q_heads / kv->kv_heads);
-    g.capacity = kv->max_pages * kv->page_size;
-    if (weights) {
-      g.scores = static_cast<float*>(workspace);
-      g.stats = g.scores + kv->batch * q_heads * g.capacity;
-      g.w = weights;
-      g.w_batch = weights_batch_stride;
-      g.w_head = weights_head_stride;
-    }
+    g.w = weights;
+    g.w_batch = weights_batch_stride;
+    g.w_head = weights_head_stride;
     cudaStream_t st = as_stream(stream);
-    if (kv->dtype == F32) launch<float>(g, st);
-    else if (kv->dtype == F16) launch<__half>(g, st);
-    else launch<__nv_bfloat16>(g, st);
+    if (kv->dtype == F32) run<float>(p, st);
+    else if (kv->dtype == F16) run<__half>(p, st);
+    else run<__nv_bfloat16>(p, st);
   });
 }
 

@@ -1,0 +1,61 @@
+// How the paged attention's work is cut among warps: plain integer
+// arithmetic, the same on host and device (the CPU tests build it alone).
+//
+// A tile is 16 consecutive positions of one sequence for one block of query
+// heads that share a key head. Tiles are numbered sequence by sequence, head
+// block by head block, along the positions; warp w of n takes the tiles
+// [w * total / n, (w + 1) * total / n). So every warp reads the same amount
+// whatever the lengths are, and a (sequence, head block) is cut only where two
+// warps' shares meet.
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__CUDACC__)
+#define PAGED_HD __host__ __device__ __forceinline__
+#else
+#define PAGED_HD inline
+#endif
+
+namespace inferc_dev {
+namespace paged {
+
+constexpr int kTile = 16;
+
+// Unsigned division by a constant of the launch, exact for every 32-bit n:
+// q = (((n * mul) >> 32) + n) >> shift with shift = ceil(log2 d) and
+// mul = floor(2^32 (2^shift - d) / d) + 1, the sum formed in 64 bits.
+struct FastDiv {
+  uint32_t d = 1, mul = 1, shift = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t d_) : d(d_) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  PAGED_HD uint32_t div(uint32_t n) const {
+    const uint64_t hi = ((uint64_t)n * mul) >> 32;
+    return (uint32_t)((hi + n) >> shift);
+  }
+  PAGED_HD uint32_t mod(uint32_t n) const { return n - div(n) * d; }
+};
+
+// Warps that get work: no more than there are tiles, and none gets fewer than
+// `least` tiles while others would have to be joined to it.
+PAGED_HD int64_t warps_used(int64_t total, int64_t warps, int64_t least) {
+  int64_t n = total / least;
+  if (n < 1) n = 1;
+  if (n > warps) n = warps;
+  return n < total ? n : total;
+}
+
+PAGED_HD int64_t first_tile(int64_t w, int64_t total, int64_t warps) {
+  return w * total / warps;
+}
+
+// The warp whose share holds tile t (warps <= total).
+PAGED_HD int64_t owner_of(int64_t t, int64_t total, int64_t warps) {
+  return ((t + 1) * warps - 1) / total;
+}
+
+}  // namespace paged
+}  // namespace inferc_dev
