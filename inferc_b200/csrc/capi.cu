@@ -19,7 +19,7 @@ thread_local std::string g_last_error;
 void set_last_error(const std::string& msg) { g_last_error = msg; }
 
 int read_and_clear_tc_error();
-int read_and_clear_paged_range();
+int read_and_clear_paged();
 void launch_split_tf32(const float* x, float* big, float* small, int64_t n, cudaStream_t st);
 bool gemm_use_tc(int64_t M, int64_t N, int64_t K);
 bool gemm_tc_supported(const float* A, int64_t lda, const float* Bb, const float* Bs,
@@ -113,7 +113,10 @@ int inferc_dev_stream_synchronize(void* stream) {
     if (read_and_clear_f16_range())
       throw Error(INFERC_ERR_RANGE,
                   "split-fp16 GEMM: an activation does not fit fp16 (results invalid)");
-    if (read_and_clear_paged_range())
+    const int paged = read_and_clear_paged();
+    if (paged & 2)
+      throw Error(INFERC_ERR_TIMEOUT, "a paged attention wait timed out (results invalid)");
+    if (paged & 1)
       throw Error(INFERC_ERR_RANGE,
                   "paged cache: a length, page, token range or position is out of range (skipped)");
   });

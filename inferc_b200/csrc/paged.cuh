@@ -63,8 +63,8 @@ __device__ __forceinline__ void store8(T* p, const float* x) {
 }
 
 // Device arguments of every paged kernel: the caller's descriptor, the
-// division by the page size, and the flag raised by an index that points
-// outside its buffer.
+// division by the page size, and two flags: flag[0] is raised by an index that
+// points outside its buffer, flag[1] by a wait that gave up.
 struct Args {
   InfercPagedKv kv;
   FastDiv page;
@@ -89,8 +89,8 @@ __device__ __forceinline__ int page_of(const Args& a, const int32_t* row, uint32
   return -1;
 }
 
-// Address of the flag on the current device; read_and_clear_paged_range()
-// (inferc_dev_stream_synchronize) reports it.
+// Address of the flags on the current device; inferc_dev_stream_synchronize
+// reports them.
 int* range_flag_ptr();
 // Throws INFERC_ERR_INVALID when the descriptor is not one the kernels take.
 void check_kv(const InfercPagedKv* kv, const char* op);
@@ -100,6 +100,7 @@ int elem_bytes(int dtype);
 
 }  // namespace paged
 
-int read_and_clear_paged_range();
+// Bit 0: an index was out of range; bit 1: a wait gave up.
+int read_and_clear_paged();
 
 }  // namespace inferc_dev

@@ -11,8 +11,7 @@ namespace paged {
 namespace {
 
 constexpr int kSMs = 148;  // B200; elsewhere the grid runs in waves
-constexpr int kLeast = 4;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinMost = 512;  // threads of a join block: this many, or a quarter where there are jobs for every SM
 
 // The parts of one (sequence, head block): warp `first`'s second slot, then
 // the first slots of the warps behind it.
@@ -28,107 +27,117 @@ struct Parts {
 //   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
 // One block per cut head block (or per share of its heads, grid.y). Its jobs
 // are found by (sequence, head block) where those are fewer than the warps,
-// else by the warp that left the first part. A few hundred floats per part:
-// bound by latency, so a part's values are spread over the threads first and
-// the parts over what threads are left.
+// else by the warp that left the first part. Bound by latency: each thread
+// takes four columns of a head and every `shares`-th part, fetches four parts'
+// columns, maxima and sums at once, and the shares meet in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttendArgs g,
+__global__ void __launch_bounds__(kJoinMost, 2) join_kernel(const __grid_constant__ AttendArgs g,
                                                             bool by_warp) {
-  __shared__ float s_max[16], s_inv[16];
-  __shared__ float4 s_sum[kJoinThreads];
+  __shared__ float4 s_o[kJoinMost];
+  __shared__ float2 s_ml[kJoinMost];
+  constexpr int kAtOnce = 4;
   const InfercPagedKv& kv = g.a.kv;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, threads = blockDim.x;
   const int heads = (int)kv.kv_heads * g.blocks, d = kv.head_dim;
+  pdl_launch_dependents();
   pdl_wait();
   const int64_t total = g.before[kv.batch];
   if (total == 0) return;
-  const int64_t used = warps_used(total, g.warps, g.least);
-  int64_t b, head;
+  int64_t b = blockIdx.x / heads;
+  int head = blockIdx.x % heads;
   if (by_warp) {
     b = g.jobs[2 * (int64_t)blockIdx.x];
     head = g.jobs[2 * (int64_t)blockIdx.x + 1];
     if (b < 0) return;
-  } else {
-    b = blockIdx.x / heads;
-    head = blockIdx.x % heads;
   }
-  const int64_t tiles = (g.before[b + 1] - g.before[b]) / heads;
+  const int64_t begin = g.before[b], tiles = (g.before[b + 1] - begin) / heads;
   if (tiles == 0) return;
-  const int64_t t0 = g.before[b] + head * tiles;
+  const int64_t used = warps_used(total, g.warps);
+  const int64_t t0 = begin + head * tiles;
   Parts parts;
   parts.first = owner_of(t0, total, used);
   parts.count = (int)(owner_of(t0 + tiles - 1, total, used) - parts.first) + 1;
   if (parts.count == 1) return;
 
-  const int hk = (int)(head / g.blocks), q0 = hk * g.group + (int)(head % g.blocks) * g.block;
+  const int hk = head / g.blocks, q0 = hk * g.group + (head % g.blocks) * g.block;
   const int cols = min(g.block, hk * g.group + g.group - q0);
   const int h0 = cols * (int)blockIdx.y / (int)gridDim.y;
   const int h1 = cols * ((int)blockIdx.y + 1) / (int)gridDim.y;
-  if (h0 == h1) return;
-  for (int h = h0 + warp; h < h1; h += kJoinThreads / 32) {
+  const int quads = d / 4, items = (h1 - h0) * quads;  // float4s of the result
+  for (int base = 0; base < items; base += threads) {
+    const int n = min(items - base, threads);
+    const int shares = min(threads / n, parts.count);
+    const int share = tid / n, item = base + tid % n;
+    const int h = h0 + item / quads, quad = item % quads;
     float m = -INFINITY, l = 0.f;
-    for (int i = lane; i < parts.count; i += 32)
-      m = fmaxf(m, g.part_ml[(parts.slot(i) * g.block + h) * 2]);
-    m = warp_max(m);
-    const float base = m == -INFINITY ? 0.f : m;
-    for (int i = lane; i < parts.count; i += 32) {
-      const float2 x =
-          reinterpret_cast<const float2*>(g.part_ml)[parts.slot(i) * g.block + h];
-      l += ex2(x.x - base) * x.y;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (share < shares) {
+      for (int i0 = share; i0 < parts.count; i0 += kAtOnce * shares) {
+        float2 ml[kAtOnce];
+        float4 x[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int i = i0 + u * shares;
+          ml[u] = make_float2(-INFINITY, 0.f);
+          x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i < parts.count) {
+            const int64_t row = parts.slot(i) * g.block + h;
+            ml[u] = reinterpret_cast<const float2*>(g.part_ml)[row];
+            x[u] = reinterpret_cast<const float4*>(g.part_o + row * d)[quad];
+          }
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) top = fmaxf(top, ml[u].x);
+        const float to = top == -INFINITY ? 0.f : top;
+        const float keep = ex2(m - to);
+        m = top;
+        l *= keep;
+        o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const float f = ex2(ml[u].x - to);
+          l += f * ml[u].y;
+          o.x += f * x[u].x;
+          o.y += f * x[u].y;
+          o.z += f * x[u].z;
+          o.w += f * x[u].w;
+        }
+      }
     }
-    l = warp_sum(l);
-    if (lane == 0) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      s_max[h] = base;
-      s_inv[h] = inv;
-      if (g.stats) {
+    s_ml[tid] = make_float2(m, l);
+    s_o[tid] = o;
+    __syncthreads();
+    if (share == 0) {
+      float top = m;
+      for (int s = 1; s < shares; ++s) top = fmaxf(top, s_ml[s * n + tid].x);
+      const float to = top == -INFINITY ? 0.f : top;
+      const float keep = ex2(m - to);
+      l *= keep;
+      o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+      for (int s = 1; s < shares; ++s) {
+        const float2 ml = s_ml[s * n + tid];
+        const float4 x = s_o[s * n + tid];
+        const float f = ex2(ml.x - to);
+        l += f * ml.y;
+        o.x += f * x.x;
+        o.y += f * x.y;
+        o.z += f * x.z;
+        o.w += f * x.w;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: every page was bad
+      T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + (q0 + h) * g.o_head + quad * 4;
+      out[0] = T(o.x * inv);
+      out[1] = T(o.y * inv);
+      out[2] = T(o.z * inv);
+      out[3] = T(o.w * inv);
+      if (g.stats && quad == 0) {
         const int64_t r = b * (int64_t)(kv.kv_heads * g.group) + q0 + h;
-        g.stats[2 * r] = base;
+        g.stats[2 * r] = to;
         g.stats[2 * r + 1] = inv;
       }
     }
-  }
-  __syncthreads();
-
-  const int quads = d / 4, items = (h1 - h0) * quads;  // float4s of the result
-  const int shares = max(1, min(kJoinThreads / max(items, 1), parts.count));
-  const int share = tid / items, item0 = tid % items;
-  T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + q0 * g.o_head;
-  for (int item = shares > 1 ? item0 : tid; item < items; item += kJoinThreads) {
-    const int h = h0 + item / quads, quad = item % quads;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (shares == 1 || share < shares) {
-#pragma unroll 4
-      for (int i = shares > 1 ? share : 0; i < parts.count; i += shares) {
-        const int64_t row = parts.slot(i) * g.block + h;
-        const float f = ex2(g.part_ml[row * 2] - s_max[h]);
-        const float4 x = reinterpret_cast<const float4*>(g.part_o + row * d)[quad];
-        sum.x += f * x.x;
-        sum.y += f * x.y;
-        sum.z += f * x.z;
-        sum.w += f * x.w;
-      }
-    }
-    if (shares > 1) {  // every thread passes here at most once, all of them together
-      s_sum[tid] = sum;
-      __syncthreads();
-      if (share == 0)
-        for (int s = 1; s < shares; ++s) {
-          const float4 x = s_sum[s * items + item];
-          sum.x += x.x;
-          sum.y += x.y;
-          sum.z += x.z;
-          sum.w += x.w;
-        }
-    }
-    if (shares == 1 || share == 0) {
-      const float inv = s_inv[h];
-      T* to = out + h * g.o_head + quad * 4;
-      to[0] = T(sum.x * inv);
-      to[1] = T(sum.y * inv);
-      to[2] = T(sum.z * inv);
-      to[3] = T(sum.w * inv);
-    }
+    __syncthreads();
   }
 }
 
@@ -148,7 +157,7 @@ __global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant
   // tiles of one head per key head, not per block of query heads
   const int64_t total = g.before[kv.batch] / g.blocks;
   if (total == 0) return;
-  const int64_t used = warps_used(total, warps, 2);
+  const int64_t used = warps_used(total, warps);
   if (w >= used) return;
   const int64_t t0 = first_tile(w, total, used), t1 = first_tile(w + 1, total, used);
   // the sequence that holds t0: 32 probes a step
@@ -171,18 +180,26 @@ __global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant
     const int h = (int)((t - first) / tiles);
     const int64_t from = (t - first) - h * tiles;  // tiles of this head: [from, upto)
     const int64_t upto = min(tiles, from + (t1 - t));
-    const int n = min((int64_t)seq_len(g.a, b), upto * kTile);
+    const int n = min((int64_t)seq_len(g.a, b), upto * g.tile);
     const int64_t r = b * q_heads + (int64_t)h * g.group;
     const float* s = g.scores + r * g.capacity;
     float* sum = g.w + b * g.w_batch + h * g.w_head;
-    for (int j = (int)from * kTile + lane; j < n; j += 32) {
-      float p = 0.f;
+    // four positions a lane; g.capacity and the tiles are multiples of 4
+    for (int j = (int)from * g.tile + lane * 4; j < n; j += 128) {
+      float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int i = 0; i < g.group; ++i) {
         const float2 st = reinterpret_cast<const float2*>(g.stats)[r + i];
-        p += ex2(s[i * g.capacity + j] - st.x) * st.y;
+        const float4 x = *reinterpret_cast<const float4*>(s + i * g.capacity + j);
+        p.x += ex2(x.x - st.x) * st.y;
+        p.y += ex2(x.y - st.x) * st.y;
+        p.z += ex2(x.z - st.x) * st.y;
+        p.w += ex2(x.w - st.x) * st.y;
       }
-      sum[j] += p;
+      sum[j] += p.x;
+      if (j + 1 < n) sum[j + 1] += p.y;
+      if (j + 2 < n) sum[j + 2] += p.z;
+      if (j + 3 < n) sum[j + 3] += p.w;
     }
     t += upto - from;
     if (upto == tiles && h + 1 == hk_n) ++b;
@@ -210,16 +227,14 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
   g.group = (int)(q_heads / kv.kv_heads);
   g.block = block_of(g.group);
   g.blocks = (g.group + g.block - 1) / g.block;
-  g.capacity = kv.max_pages * kv.page_size;
-  g.least = kLeast;
-  const int64_t tiles = (g.capacity + kTile - 1) / kTile;
-  const int per_sm = kv.dtype == F32    ? blocks_per_sm<float>(kv.head_dim)
-                     : kv.dtype == F16 ? blocks_per_sm<__half>(kv.head_dim)
-                                       : blocks_per_sm<__nv_bfloat16>(kv.head_dim);
+  g.capacity = (kv.max_pages * kv.page_size + 3) / 4 * 4;
+  const Shape shape = kv.dtype == F32   ? shape_of<float>(kv.head_dim)
+                      : kv.dtype == F16 ? shape_of<__half>(kv.head_dim)
+                                        : shape_of<__nv_bfloat16>(kv.head_dim);
+  g.tile = shape.tile;
+  const int64_t tiles = (g.capacity + g.tile - 1) / g.tile;
   const int64_t most = kv.batch * kv.kv_heads * g.blocks * tiles;
-  g.warps = std::max<int64_t>(1, std::min<int64_t>((int64_t)kSMs * per_sm * kWarps, most));
-  // With at most kLeast tiles each, no (sequence, head block) is worth cutting, but the
-  // shares still end inside one unless it is a single tile.
+  g.warps = std::max<int64_t>(1, std::min<int64_t>((int64_t)kSMs * shape.blocks * kWarps, most));
   p.cut = tiles > 1;
   auto take = [&](int64_t bytes) {
     char* at = ws + p.bytes;
@@ -257,7 +272,8 @@ void run(const Plan& p, cudaStream_t st) {
     const int64_t jobs = by_warp ? g.warps : pairs;
     // few jobs: their heads go to blocks of their own
     const int split = (int)std::min<int64_t>(g.block, std::max<int64_t>(1, 4 * kSMs / jobs));
-    launch_pdl(join_kernel<T>, dim3((unsigned)jobs, (unsigned)split), dim3(kJoinThreads), 0, st, g,
+    launch_pdl(join_kernel<T>, dim3((unsigned)jobs, (unsigned)split),
+               dim3(jobs * split > kSMs ? kJoinMost / 4 : kJoinMost), 0, st, g,
                by_warp);
   }
   if (g.w) {

@@ -18,23 +18,34 @@
 // full bandwidth); tcgen05 tiles would need 64 rows and a trip through tensor
 // memory for each 16 positions.
 //
-// Layout. Each warp owns a ring of kSlots shared-memory slots, each 16 rows of
-// K or V, filled by 16-byte cp.async some tiles ahead across the boundaries
-// of heads and sequences, so that warps never wait for each other and the
-// loads never drain. Rows are padded to an odd number of 16-byte pieces (fp32:
-// by 16 words), which keeps ldmatrix (fp32: 16-byte loads) free of bank
-// conflicts. Rows past a sequence's end, or on a page that does not exist,
-// are filled with zeros and their scores set to -inf, so what the page holds
-// there is never used.
+// Layout. Each warp owns a ring of kSlots shared-memory slots, each a tile of K
+// or of V in 128-byte columns with the 128-byte swizzle (free of bank conflicts
+// for ldmatrix and for fp32's 16-byte loads). One lane fills them by TMA, boxes
+// of 16 rows of 128 bytes, some tiles ahead and across the boundaries of heads
+// and sequences, so that warps never wait for each other and the loads never
+// drain. A box never leaves its page when the page size is a multiple of 16;
+// for other page sizes, or strides a tensor map cannot carry, the slots are
+// filled by 16-byte cp.async, row by row. Rows past a sequence's end, or on a
+// page that does not exist, are scored -inf and their values cleared before
+// they are used, whatever the page holds there.
+//
+// A tile is 32 positions where a row has up to 256 bytes and 16 above: the
+// cost of a tile that does not depend on its rows (maximum over the warp,
+// bookkeeping, waits) was a third of all instructions at 16.
 //
 // Numbers. 16-bit products are exact in fp32. P goes into the second product
 // as two 16-bit pieces, P = hi + lo, so that rounding it adds less than the
 // result's own rounding; fp16 P carries a factor 2^10 (in m), which keeps
 // weights down to 2^-34 of the largest. fp32 operands are taken as two tf32
-// pieces each, three products (big big, big small, small big): 2^-22 relative.
+// pieces each, three products (big big, big small, small big), so that at most
+// 2^-20 of a product is lost (cut operands lose 3 * 2^-23, rounded ones 2^-22,
+// small * small is below 2^-21).
 #pragma once
 
+#include <atomic>
+
 #include "paged.cuh"
+#include "tc_ptx.cuh"
 
 namespace inferc_dev {
 namespace paged {
@@ -49,8 +60,8 @@ struct AttendArgs {
   int group;        // query heads per key head
   int block;        // query heads per block (at most 16)
   int blocks;       // blocks per key head
+  int tile;         // positions per tile
   int64_t warps;    // in the grid
-  int least;        // tiles per warp, see warps_used
   int64_t* before;  // [batch + 1] tiles before each sequence
   int32_t* jobs;    // [warps, 2] (sequence, head block) whose first part this warp left; -1
   float* part_ml;   // [2 warps, block, 2] maximum and sum of a part
@@ -64,20 +75,25 @@ struct AttendArgs {
 
 constexpr int kWarps = 4;  // per block
 
+constexpr int kBox = 16;  // rows that TMA fetches at once, and of one matrix instruction
+
+// Shared memory of a warp: kSlots slots of kColumns columns of kTile rows of
+// 128 bytes, then a barrier and a row mask for each slot.
 template <typename T, int kDim>
 struct Layout {
   static constexpr bool kWide = sizeof(T) == 4;
-  // row stride in bytes; both operands of fp32 share the larger one's slot
-  static constexpr int kRowK = kWide ? (kDim + 16) * 4 : kDim * 2 + 16;
-  static constexpr int kRowV = kWide ? (kDim + 8) * 4 : kDim * 2 + 16;
-  static constexpr int kSlot = kTile * kRowK;
+  static constexpr int kTile = kDim * (int)sizeof(T) <= 256 ? 32 : 16;  // positions
+  static constexpr int kElems = 128 / sizeof(T);                       // per column
+  static constexpr int kColumns = (kDim + kElems - 1) / kElems;
+  static constexpr int kColumn = kTile * 128;
+  static constexpr int kSlot = kColumns * kColumn;
   // Two blocks (8 warps) per SM with as many slots as their shares of the
   // 227 KB allow, one block where that would leave fewer than three.
-  static constexpr int kTwo = 112 * 1024 / (kWarps * kSlot + 64);
+  static constexpr int kTwo = 110 * 1024 / (kWarps * (kSlot + 16));
   static constexpr int kBlocks = kTwo >= 3 ? 2 : 1;
-  static constexpr int kFit = kBlocks == 2 ? kTwo : 220 * 1024 / (kWarps * kSlot + 64);
-  static constexpr int kSlots = kFit > 8 ? 8 : kFit;
-  static constexpr int kSmem = kWarps * kSlots * (kSlot + 16);
+  static constexpr int kFit = kBlocks == 2 ? kTwo : 220 * 1024 / (kWarps * (kSlot + 16));
+  static constexpr int kSlots = kFit > 6 ? 6 : kFit;
+  static constexpr int kSmem = kWarps * kSlots * (kSlot + 16) + 1024;  // + alignment slack
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -149,6 +165,13 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& big, uint32_t& sma
   small = __float_as_uint(x - __uint_as_float(big)) + 0x1000u;
 }
 
+// The same by cutting instead of rounding, in half the instructions: big keeps
+// 11 bits, small the other 13, of which the instruction uses at least 11.
+__device__ __forceinline__ void cut_tf32(uint32_t x, uint32_t& big, uint32_t& small) {
+  big = x & 0xffffe000u;
+  small = __float_as_uint(__uint_as_float(x) - __uint_as_float(big));
+}
+
 // P in [0, 1] (fp16: [0, 2^10]) as two 16-bit pieces, two values packed.
 template <typename T>
 __device__ __forceinline__ void split_pair16(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -168,34 +191,41 @@ __device__ __forceinline__ void split_pair16(float x, float y, uint32_t& hi, uin
 }
 
 // A place in the numbering of tiles.
+template <int kTile>
 struct Cursor {
-  int b, head, tile, tiles, len;  // head: key head x head block
+  int b, hk, block, tile, tiles, len;
 
-  // Goes to sequence b or the first one after it that holds something.
+  // Goes to sequence `first` or the first one after it that holds something.
   __device__ __forceinline__ void open(const AttendArgs& g, int first) {
     b = first;
-    head = tile = tiles = 0;
+    hk = block = tile = tiles = 0;
     for (; b < (int)g.a.kv.batch; ++b) {
       len = seq_len(g.a, b);
       tiles = (len + kTile - 1) / kTile;
       if (tiles) return;
     }
   }
-  __device__ __forceinline__ void next(const AttendArgs& g, int heads) {
+  __device__ __forceinline__ void next(const AttendArgs& g) {
     if (++tile < tiles) return;
     tile = 0;
-    if (++head < heads) return;
+    if (++block < g.blocks) return;
+    block = 0;
+    if (++hk < (int)g.a.kv.kv_heads) return;
     open(g, b + 1);
   }
 };
 
-template <typename T, int kDim, int kCols>
+template <typename T, int kDim, int kCols, bool kTma>
 __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
-    attend_kernel(const __grid_constant__ AttendArgs g) {
+    attend_kernel(const __grid_constant__ AttendArgs g, const __grid_constant__ CUtensorMap k_map,
+                  const __grid_constant__ CUtensorMap v_map) {
   using L = Layout<T, kDim>;
   constexpr bool kWide = L::kWide;
-  constexpr int kElem = sizeof(T), kThreads = kWarps * 32;
-  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int kElem = sizeof(T), kThreads = kWarps * 32, kTile = L::kTile;
+  constexpr int kSubs = kTile / kBox;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int64_t s_before[kThreads + 1];
   __shared__ int64_t s_warp[kWarps];
   const InfercPagedKv& kv = g.a.kv;
@@ -205,6 +235,11 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
   const int batch = (int)kv.batch;
   const int d = kv.head_dim;
   pdl_launch_dependents();
+  if constexpr (kTma)
+    if (tid == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)));
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)));
+    }
 
   // Tiles before each thread's run of sequences, and in all.
   const int run = (batch + kThreads - 1) / kThreads;
@@ -251,20 +286,18 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
 
   const int64_t w = (int64_t)blockIdx.x * kWarps + warp;
   if (g.jobs && lane == 0 && w < g.warps) g.jobs[2 * w] = -1;
-  const int64_t used = warps_used(total, g.warps, g.least);
+  const int64_t used = warps_used(total, g.warps);
   if (w >= used) return;
   const int64_t t0 = first_tile(w, total, used);
   const int count = (int)(first_tile(w + 1, total, used) - t0);
 
   // The tile t0: the thread whose run holds it, then the sequence, then the head.
-  Cursor load;
+  Cursor<kTile> load;
   {
-    int lo = 0, hi = kThreads;  // s_before[lo] <= t0 < s_before[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (s_before[mid] <= t0) lo = mid;
-      else hi = mid;
-    }
+    int lo = -1;  // runs that begin at t0 or before it, less one
+#pragma unroll
+    for (int i = 0; i < kThreads; i += 32)
+      lo += __popc(__ballot_sync(0xffffffffu, s_before[i + lane] <= t0));
     int64_t left = t0 - s_before[lo];
     load.open(g, min(lo * run, batch));
     while (load.b < batch && left >= (int64_t)load.tiles * heads) {
@@ -272,98 +305,227 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       load.open(g, load.b + 1);
     }
     if (load.b >= batch) return;  // only if the lengths change under the kernel
-    load.head = (int)(left / load.tiles);
-    load.tile = (int)(left % load.tiles);
+    const int head = (int)divide(left, load.tiles);
+    load.hk = head / g.blocks;
+    load.block = head - load.hk * g.blocks;
+    load.tile = (int)(left - (int64_t)head * load.tiles);
   }
-  Cursor use = load;
+  Cursor<kTile> use = load;
 
-  unsigned char* ring = smem + warp * L::kSlots * (L::kSlot + 16);
-  uint32_t* masks = reinterpret_cast<uint32_t*>(ring + L::kSlots * L::kSlot);
+  unsigned char* ring = smem + warp * L::kSlots * L::kSlot;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * L::kSlots * L::kSlot) +
+                   warp * L::kSlots;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + kWarps * L::kSlots * (L::kSlot + 8)) +
+                    warp * L::kSlots;
   const uint32_t ring_addr = smem_addr(ring);
-  if (d < kDim)  // columns that no copy fills
+  if constexpr (kTma) {
+    if (lane == 0) {
+      for (int i = 0; i < L::kSlots; ++i) tc::mbar_init(&full[i], 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      tc::fence_proxy_async();
+    }
+  } else if (d < kDim) {  // what no copy fills
     for (int i = lane * 16; i < L::kSlots * L::kSlot; i += 32 * 16)
       *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
+  }
   __syncwarp();
 
-  // ---- loads: one slot at a time, the keys of a tile, then its values
-  constexpr int kPieces = kDim * kElem / 16;  // 16-byte pieces of a full row
-  constexpr int kLanes = kPieces <= 8 ? 8 : kPieces <= 16 ? 16 : 32;
-  constexpr int kRowsAt = 32 / kLanes, kSteps = kTile / kRowsAt;
-  constexpr int kTurns = (kPieces + 31) / 32;
-  const int pieces = d * kElem / 16, piece = lane % kLanes;
-  int loaded = 0, slot_in = 0;
-  bool values = false;
+  // ---- loads: one slot at a time, the keys of a tile, then its values.
+  // Kept from a tile's keys to its values:
+  int tiles_in = 0, slot_in = 0;  // tiles whose values are on their way; next slot
+  bool fetched = false;           // the keys of one more are
+  uint32_t mask_in = 0;           // rows that exist
+  // kTma: pages of the tile's boxes (those of the next tile are read one ahead) and the
+  // first row's place in its page
+  int page_next[kSubs], page[kSubs];
+  uint32_t at[kSubs];
+  // else: this lane's row of the tile, in V
   int64_t off_v = 0;
   bool row_ok = false;
-  const char* k_base = reinterpret_cast<const char*>(kv.k) + piece * 16;
-  const char* v_base = reinterpret_cast<const char*>(kv.v) + piece * 16;
-  auto fill = [&]() {
-    if (loaded < count && load.b < batch) {
-      int64_t off;
-      if (!values) {
-        const int j = load.tile * kTile + (lane & 15);
+
+  auto look_up = [&]() {
+    if constexpr (kTma) {
+      const int32_t* row = kv.page_table + load.b * kv.table_stride;
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) {
+        const int j = load.tile * kTile + i * kBox;
+        page_next[i] = -1;
+        if (load.b < batch && j < load.len) page_next[i] = row[g.a.page.div(j)];
+      }
+    }
+  };
+  auto boxes = [&](const CUtensorMap* map) {
+    const uint32_t bar = tc::smem_u32(&full[slot_in]);
+    const uint32_t dst = ring_addr + slot_in * L::kSlot;
+#pragma unroll
+    for (int s = 0; s < kSubs; ++s)
+      if (mask_in >> (s * kBox) & 1) {
+#pragma unroll
+        for (int i = 0; i < L::kColumns; ++i)
+          asm volatile(
+              "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+              " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + i * L::kColumn + s * kBox * 128),
+              "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(i * L::kElems), "r"(at[s]),
+              "r"(load.hk), "r"(page[s])
+              : "memory");
+      }
+  };
+  auto expect = [&]() {
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int s = 0; s < kSubs; ++s)
+      if (mask_in >> (s * kBox) & 1) bytes += L::kColumns * kBox * 128;
+    if (bytes) tc::mbar_expect_tx(&full[slot_in], bytes);
+    else tc::mbar_arrive(&full[slot_in]);
+  };
+  // kLanes lanes share a row, 16 bytes each.
+  auto copy_rows = [&](const void* cache, int64_t off) {
+    constexpr int kPieces = kDim * kElem / 16;
+    constexpr int kLanes = kPieces <= 8 ? 8 : kPieces <= 16 ? 16 : 32;
+    constexpr int kRowsAt = 32 / kLanes, kTurns = (kPieces + 31) / 32;
+    const int pieces = d * kElem / 16, piece0 = lane % kLanes;
+    const uint32_t dst = ring_addr + slot_in * L::kSlot;
+#pragma unroll
+    for (int i = 0; i < kTile / kRowsAt; ++i) {
+      const int row = i * kRowsAt + lane / kLanes;
+      const int64_t from = __shfl_sync(0xffffffffu, off, row);
+      const bool ok = __shfl_sync(0xffffffffu, (int)row_ok, row);
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int piece = piece0 + 32 * t;
+        if (piece < pieces)
+          copy16(dst + (piece >> 3) * L::kColumn + row * 128 + (((piece & 7) ^ (row & 7)) << 4),
+                 static_cast<const char*>(cache) + from + piece * 16, ok);
+      }
+    }
+  };
+  auto filled = [&]() {
+    if constexpr (!kTma) asm volatile("cp.async.commit_group;" ::: "memory");
+    slot_in = slot_in + 1 == L::kSlots ? 0 : slot_in + 1;
+  };
+  auto fill_k = [&]() {
+    if (tiles_in < count && load.b < batch) {
+      fetched = true;
+      if constexpr (kTma) {
+        mask_in = 0;
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s) {
+          const int j = load.tile * kTile + s * kBox;
+          page[s] = page_next[s];
+          at[s] = g.a.page.mod(j);
+          const int rows = min(load.len - j, kBox);
+          if (rows > 0) {
+            if (page[s] >= 0 && page[s] < kv.num_pages) mask_in |= ((1u << rows) - 1) << (s * kBox);
+            else *g.a.flag = 1;
+          }
+        }
+        if (lane == 0) {
+          masks[slot_in] = mask_in;
+          expect();
+          boxes(&k_map);
+        }
+      } else {
+        const int j = load.tile * kTile + (lane & (kTile - 1));
         row_ok = j < load.len;
-        int page = 0;
+        int id = 0;
         uint32_t slot = 0;
         if (row_ok) {
           const uint32_t index = g.a.page.div(j);
           slot = j - index * g.a.page.d;
-          page = page_of(g.a, kv.page_table + load.b * kv.table_stride, index);
-          row_ok = page >= 0;
+          id = page_of(g.a, kv.page_table + load.b * kv.table_stride, index);
+          row_ok = id >= 0;
         }
-        const int hk = load.head / g.blocks;
-        off = row_ok ? (page * kv.k_page_stride + slot * kv.k_token_stride +
-                        hk * kv.k_head_stride) * kElem
-                     : 0;
-        off_v = row_ok ? (page * kv.v_page_stride + slot * kv.v_token_stride +
-                          hk * kv.v_head_stride) * kElem
+        const int64_t off_k = row_ok ? (id * kv.k_page_stride + slot * kv.k_token_stride +
+                                        load.hk * kv.k_head_stride) * kElem
+                                     : 0;
+        off_v = row_ok ? (id * kv.v_page_stride + slot * kv.v_token_stride +
+                          load.hk * kv.v_head_stride) * kElem
                        : 0;
         const uint32_t mask = __ballot_sync(0xffffffffu, row_ok);
         if (lane == 0) masks[slot_in] = mask;
-      } else {
-        off = off_v;
+        copy_rows(kv.k, off_k);
       }
-      const char* base = values ? v_base : k_base;
-      const uint32_t dst = ring_addr + slot_in * L::kSlot + piece * 16;
-      const int stride = values ? L::kRowV : L::kRowK;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int row = i * kRowsAt + lane / kLanes;
-        const int64_t from = __shfl_sync(0xffffffffu, off, row);
-        const bool ok = __shfl_sync(0xffffffffu, (int)row_ok, row);
-#pragma unroll
-        for (int t = 0; t < kTurns; ++t)
-          if (piece + 32 * t < pieces)
-            copy16(dst + row * stride + 512 * t, base + from + 512 * t, ok);
-      }
-      if (values) {
-        ++loaded;
-        load.next(g, heads);
-      }
-      values = !values;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    slot_in = slot_in + 1 == L::kSlots ? 0 : slot_in + 1;
+    filled();
   };
-#pragma unroll 1
-  for (int i = 0; i < L::kSlots; ++i) fill();
+  auto fill_v = [&]() {
+    if (fetched) {
+      fetched = false;
+      ++tiles_in;
+      if constexpr (kTma) {
+        if (lane == 0) {
+          expect();
+          boxes(&v_map);
+        }
+      } else {
+        copy_rows(kv.v, off_v);
+      }
+      load.next(g);
+      look_up();
+    }
+    filled();
+  };
+  look_up();
+#pragma unroll
+  for (int i = 0; i < L::kSlots; ++i) {
+    if (i & 1) fill_v();
+    else fill_k();
+  }
+
+  int slot_out = 0;
+  uint32_t phase = 0;
+  // Waits for the slot's rows; false after the time limit.
+  auto wait = [&]() {
+    bool done = true;
+    if constexpr (kTma) {
+      done = tc::mbar_try(&full[slot_out], phase) || tc::mbar_wait(&full[slot_out], phase);
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(L::kSlots - 1) : "memory");
+      __syncwarp();
+    }
+    return done;
+  };
+  auto released = [&]() {
+    if (++slot_out == L::kSlots) {
+      slot_out = 0;
+      phase ^= 1;
+    }
+  };
+  // Gives up: no copy into this block's memory may be in flight when it leaves.
+  auto give_up = [&]() {
+    if (lane == 0) atomicExch(g.a.flag + 1, 1);
+    const int fills = min(2 * tiles_in + (fetched ? 1 : 0), (int)L::kSlots);
+    for (int i = 0; i < fills; ++i) {
+      tc::mbar_wait(&full[slot_out], phase);
+      released();
+    }
+  };
 
   // ---- the state of one (sequence, head block)
   constexpr int kKSteps = kWide ? kDim / 8 : kDim / 16;  // steps along head_dim
   constexpr int kMTiles = kDim / 16;                     // blocks of 16 columns of V
   constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
-  uint32_t qf[kCols][kKSteps][2];
+  // fp32 queries are split once where their pieces fit the registers
+  constexpr bool kSplitOnce = kWide && kDim * kCols <= 128;
+  uint32_t qf[kCols][kKSteps][kSplitOnce ? 4 : 2];
   float o[kCols][kMTiles][4];
   float m[kCols][2], l[kCols][2];
   bool begins = false;
-  int slot_out = 0;
+  int q0 = 0, cols = 0;
+  // ldmatrix places: row and 16-byte piece of this lane, swizzled; the step's
+  // bits of the piece are xored in
+  const uint32_t k_place = ((lane & 7) + ((lane >> 3) & 1) * 8) * 128 +
+                           (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_place = ((lane & 7) + (lane >> 4) * 8) * 128 +
+                           ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 
+  int t = 0;
 #pragma unroll 1
-  for (int t = 0; t < count && use.b < batch; ++t) {
-    const int hk = use.head / g.blocks, q0 = hk * g.group + (use.head % g.blocks) * g.block;
-    const int cols = min(g.block, hk * g.group + g.group - q0);
+  for (; t < count && use.b < batch; ++t) {
     if (t == 0 || use.tile == 0) {
       begins = use.tile == 0;
+      q0 = use.hk * g.group + use.block * g.block;
+      cols = min(g.block, (use.hk + 1) * g.group - q0);
       const T* q = reinterpret_cast<const T*>(g.q) + use.b * g.q_batch + q0 * g.q_head;
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
@@ -371,17 +533,14 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
         const T* row = q + (int64_t)h * g.q_head;
 #pragma unroll
         for (int s = 0; s < kKSteps; ++s) {
-          if constexpr (kWide) {
-            // columns are taken in the order the 16-byte loads of K give them
-            const int at = (s >> 1) * 16 + tig * 4 + (s & 1) * 2;
-            const bool in = h < cols && at < d;
-            qf[c][s][0] = in ? __float_as_uint(row[at]) : 0u;
-            qf[c][s][1] = in ? __float_as_uint(row[at + 1]) : 0u;
-          } else {
-            const int at = s * 16 + tig * 2;
-            qf[c][s][0] = h < cols && at < d ? *reinterpret_cast<const uint32_t*>(row + at) : 0u;
-            qf[c][s][1] =
-                h < cols && at + 8 < d ? *reinterpret_cast<const uint32_t*>(row + at + 8) : 0u;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int col = kWide ? s * 8 + tig + 4 * i : s * 16 + tig * 2 + 8 * i;
+            const bool in = h < cols && col < d;
+            uint32_t x = 0;
+            if (in) x = *reinterpret_cast<const uint32_t*>(row + col);
+            if constexpr (kSplitOnce) split_tf32(__uint_as_float(x), qf[c][s][i], qf[c][s][2 + i]);
+            else qf[c][s][i] = x;
           }
         }
         m[c][0] = m[c][1] = -INFINITY;
@@ -392,99 +551,108 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     }
 
     // ---- scores
-    asm volatile("cp.async.wait_group %0;" ::"n"(L::kSlots - 1) : "memory");
-    __syncwarp();
-    const uint32_t k_addr = ring_addr + slot_out * L::kSlot;
-    const unsigned char* k_ptr = ring + slot_out * L::kSlot;
+    if (!wait()) {
+      give_up();
+      return;
+    }
     const uint32_t mask = masks[slot_out];
-    float sc[kCols][4];
-    if constexpr (!kWide) {
-      float acc[kCols][2][4] = {};
-      const uint32_t addr =
-          k_addr + ((lane & 7) + ((lane >> 3) & 1) * 8) * L::kRowK + (lane >> 4) * 16;
+    float sc[kSubs][kCols][4];
+    {
+      const uint32_t k_addr = ring_addr + slot_out * L::kSlot + k_place;
+      // two chains of products, so that one need not wait for the one before
+      float acc[kSubs][kCols][2][4] = {};
 #pragma unroll
       for (int s = 0; s < kKSteps; ++s) {
-        uint32_t a[4];
-        ldmatrix4(addr + s * 32, a);
+        uint32_t qs[kCols][4];
+        if constexpr (kWide) {
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) mma16<T>(acc[c][s & 1], a, qf[c][s][0], qf[c][s][1]);
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if constexpr (kSplitOnce) {
+                qs[c][i] = qf[c][s][i];
+                qs[c][2 + i] = qf[c][s][2 + i];
+              } else {
+                split_tf32(__uint_as_float(qf[c][s][i]), qs[c][i], qs[c][2 + i]);
+              }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) {
+          uint32_t a[4];
+          ldmatrix4((k_addr ^ ((s & 3) << 5)) + (s >> 2) * L::kColumn + u * kBox * 128, a);
+          if constexpr (!kWide) {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+              mma16<T>(acc[u][c][s & 1], a, qf[c][s][0], qf[c][s][1]);
+          } else {
+            uint32_t big[4], small[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cut_tf32(a[i], big[i], small[i]);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              mma_tf32(acc[u][c][1], small, qs[c][0], qs[c][1]);
+              mma_tf32(acc[u][c][0], big, qs[c][0], qs[c][1]);
+              mma_tf32(acc[u][c][1], big, qs[c][2], qs[c][3]);
+            }
+          }
+        }
       }
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[c][i] = acc[c][0][i] + acc[c][1][i];
-    } else {
-      // two chains, so that a product need not wait for the one before
-      float acc[kCols][2][4] = {};
-      const unsigned char* r0 = k_ptr + gid * L::kRowK + tig * 16;
-      const unsigned char* r1 = r0 + 8 * L::kRowK;
-#pragma unroll
-      for (int s = 0; s < kKSteps; s += 2) {
-        const float4 x = *reinterpret_cast<const float4*>(r0 + s * 32);
-        const float4 y = *reinterpret_cast<const float4*>(r1 + s * 32);
-        uint32_t big[2][4], small[2][4];
-        split_tf32(x.x, big[0][0], small[0][0]);
-        split_tf32(y.x, big[0][1], small[0][1]);
-        split_tf32(x.y, big[0][2], small[0][2]);
-        split_tf32(y.y, big[0][3], small[0][3]);
-        split_tf32(x.z, big[1][0], small[1][0]);
-        split_tf32(y.z, big[1][1], small[1][1]);
-        split_tf32(x.w, big[1][2], small[1][2]);
-        split_tf32(y.w, big[1][3], small[1][3]);
+      for (int u = 0; u < kSubs; ++u)
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t b0, b1, s0, s1;
-            split_tf32(__uint_as_float(qf[c][s + u][0]), b0, s0);
-            split_tf32(__uint_as_float(qf[c][s + u][1]), b1, s1);
-            mma_tf32(acc[c][1], small[u], b0, b1);
-            mma_tf32(acc[c][1], big[u], s0, s1);
-            mma_tf32(acc[c][0], big[u], b0, b1);
-          }
-      }
+          for (int i = 0; i < 4; ++i)
+            sc[u][c][i] = (acc[u][c][0][i] + acc[u][c][1][i]) * g.scale;
+    }
+    __syncwarp();
+    if constexpr (L::kSlots % 2 == 0) fill_k();
+    else fill_v();
+    released();
+
+    // ---- softmax: of 16 positions gid and gid + 8, of 8 heads 2 tig and 2 tig + 1
+    if (mask != (kTile == 32 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(mask >> (u * kBox + gid + (i >> 1) * 8) & 1))
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) sc[u][c][i] = -INFINITY;
+    }
+    if (g.scores) {
+      const int left = use.len - use.tile * kTile - gid;  // positions from this lane's on
+      float* to0 = g.scores + (use.b * (int64_t)(kv.kv_heads * g.group) + q0 + tig * 2) *
+                                  g.capacity + use.tile * kTile + gid;
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[c][i] = acc[c][0][i] + acc[c][1][i];
+        for (int i = 0; i < 2; ++i) {
+          if (c * 8 + tig * 2 + i >= cols) continue;
+          float* to = to0 + (c * 8 + i) * g.capacity;
+#pragma unroll
+          for (int u = 0; u < kSubs; ++u) {
+            if (left > u * kBox) to[u * kBox] = sc[u][c][i];
+            if (left > u * kBox + 8) to[u * kBox + 8] = sc[u][c][i + 2];
+          }
+        }
     }
-    __syncwarp();
-    fill();
-
-    // ---- softmax: positions gid and gid + 8, heads 2 tig and 2 tig + 1 of each column block
-    const bool ok0 = mask >> gid & 1, ok1 = mask >> (gid + 8) & 1;
     float top[kCols][2];
     bool grew = false;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      sc[c][0] = ok0 ? sc[c][0] * g.scale : -INFINITY;
-      sc[c][1] = ok0 ? sc[c][1] * g.scale : -INFINITY;
-      sc[c][2] = ok1 ? sc[c][2] * g.scale : -INFINITY;
-      sc[c][3] = ok1 ? sc[c][3] * g.scale : -INFINITY;
-      if (g.scores) {
-        float* to = g.scores + (use.b * (int64_t)(kv.kv_heads * g.group) + q0 + c * 8 + tig * 2) *
-                                   g.capacity + use.tile * kTile + gid;
-        const int left = use.len - use.tile * kTile - gid;  // positions from this lane's on
-        const int h = c * 8 + tig * 2;
-        if (h < cols) {
-          if (left > 0) to[0] = sc[c][0];
-          if (left > 8) to[8] = sc[c][2];
-        }
-        if (h + 1 < cols) {
-          if (left > 0) to[g.capacity] = sc[c][1];
-          if (left > 8) to[g.capacity + 8] = sc[c][3];
-        }
-      }
+    for (int c = 0; c < kCols; ++c)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float x = fmaxf(sc[c][i], sc[c][i + 2]);
+        float x = fmaxf(sc[0][c][i], sc[0][c][i + 2]);
+#pragma unroll
+        for (int u = 1; u < kSubs; ++u) x = fmaxf(x, fmaxf(sc[u][c][i], sc[u][c][i + 2]));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
         top[c][i] = x - kLift;
         grew |= top[c][i] > m[c][i];
       }
-    }
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
@@ -510,83 +678,102 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float base = m[c][i] == -INFINITY ? 0.f : m[c][i];
-        sc[c][i] = ex2(sc[c][i] - base);
-        sc[c][i + 2] = ex2(sc[c][i + 2] - base);
-        l[c][i] += sc[c][i] + sc[c][i + 2];
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) {
+          sc[u][c][i] = ex2(sc[u][c][i] - base);
+          sc[u][c][i + 2] = ex2(sc[u][c][i + 2] - base);
+          l[c][i] += sc[u][c][i] + sc[u][c][i + 2];
+        }
       }
 
     // ---- values
-    slot_out = slot_out + 1 == L::kSlots ? 0 : slot_out + 1;
-    asm volatile("cp.async.wait_group %0;" ::"n"(L::kSlots - 1) : "memory");
-    __syncwarp();
-    const uint32_t v_addr = ring_addr + slot_out * L::kSlot;
-    const unsigned char* v_ptr = ring + slot_out * L::kSlot;
-    if constexpr (!kWide) {
-      uint32_t hi[kCols][2], lo[kCols][2];
+    if (!wait()) {
+      give_up();
+      return;
+    }
+    unsigned char* v_ptr = ring + slot_out * L::kSlot;
+    if (kTma && mask != (kTile == 32 ? 0xffffffffu : 0xffffu)) {  // rows that do not exist
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          split_pair16<T>(sc[c][2 * i], sc[c][2 * i + 1], hi[c][i], lo[c][i]);
-          hi[c][i] = transpose8x8(hi[c][i]);
-          lo[c][i] = transpose8x8(lo[c][i]);
-        }
-      const uint32_t addr =
-          v_addr + ((lane & 7) + (lane >> 4) * 8) * L::kRowV + ((lane >> 3) & 1) * 16;
-#pragma unroll
-      for (int i = 0; i < kMTiles; ++i) {
-        uint32_t a[4];
-        ldmatrix4_trans(addr + i * 32, a);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, lo[c][0], lo[c][1]);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, hi[c][0], hi[c][1]);
+      for (int i = 0; i < L::kSlot / 512; ++i) {
+        const int to = i * 512 + lane * 16;
+        if (!(mask >> ((to % L::kColumn) >> 7) & 1))
+          *reinterpret_cast<uint4*>(v_ptr + to) = make_uint4(0, 0, 0, 0);
       }
-    } else {
-      // P of positions (tig, tig + 4) of each half, head gid: from the lanes that hold them
-      uint32_t b_big[kCols][2][2], b_small[kCols][2][2];
+      tc::fence_proxy_async();  // before TMA writes here again
+      __syncwarp();
+    }
+    if constexpr (!kWide) {
+      const uint32_t v_addr = ring_addr + slot_out * L::kSlot + v_place;
+      uint32_t hi[kSubs][kCols][2], lo[kSubs][kCols][2];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
+      for (int u = 0; u < kSubs; ++u)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int c = 0; c < kCols; ++c)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int src = (tig + 4 * i) * 4 + (gid >> 1);
-            const float x = __shfl_sync(0xffffffffu, sc[c][2 * half], src);
-            const float y = __shfl_sync(0xffffffffu, sc[c][2 * half + 1], src);
-            split_tf32(gid & 1 ? y : x, b_big[c][half][i], b_small[c][half][i]);
+            split_pair16<T>(sc[u][c][2 * i], sc[u][c][2 * i + 1], hi[u][c][i], lo[u][c][i]);
+            hi[u][c][i] = transpose8x8(hi[u][c][i]);
+            lo[u][c][i] = transpose8x8(lo[u][c][i]);
           }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const unsigned char* r0 = v_ptr + (half * 8 + tig) * L::kRowV + gid * 16;
-        const unsigned char* r1 = r0 + 4 * L::kRowV;
+      for (int i = 0; i < kMTiles; ++i)
 #pragma unroll
-        for (int i = 0; i < kMTiles; i += 2) {
-          const float4 x = *reinterpret_cast<const float4*>(r0 + i * 64);
-          const float4 y = *reinterpret_cast<const float4*>(r1 + i * 64);
-          uint32_t big[2][4], small[2][4];
-          split_tf32(x.x, big[0][0], small[0][0]);
-          split_tf32(x.y, big[0][1], small[0][1]);
-          split_tf32(y.x, big[0][2], small[0][2]);
-          split_tf32(y.y, big[0][3], small[0][3]);
-          split_tf32(x.z, big[1][0], small[1][0]);
-          split_tf32(x.w, big[1][1], small[1][1]);
-          split_tf32(y.z, big[1][2], small[1][2]);
-          split_tf32(y.w, big[1][3], small[1][3]);
+        for (int u = 0; u < kSubs; ++u) {
+          uint32_t a[4];
+          ldmatrix4_trans((v_addr ^ ((i & 3) << 5)) + (i >> 2) * L::kColumn + u * kBox * 128, a);
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, lo[u][c][0], lo[u][c][1]);
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              mma_tf32(o[c][i + u], small[u], b_big[c][half][0], b_big[c][half][1]);
-              mma_tf32(o[c][i + u], big[u], b_small[c][half][0], b_small[c][half][1]);
-              mma_tf32(o[c][i + u], big[u], b_big[c][half][0], b_big[c][half][1]);
-            }
+          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, hi[u][c][0], hi[u][c][1]);
         }
-      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // P of positions (2 tig, 2 tig + 1) of these 8, head gid, from the lanes that hold them
+          uint32_t big_p[kCols][2], small_p[kCols][2];
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int src = (tig * 2 + i) * 4 + (gid >> 1);
+              const float x = __shfl_sync(0xffffffffu, sc[u][c][2 * half], src);
+              const float y = __shfl_sync(0xffffffffu, sc[u][c][2 * half + 1], src);
+              split_tf32(gid & 1 ? y : x, big_p[c][i], small_p[c][i]);
+            }
+          const unsigned char* r0 =
+              v_ptr + (u * kBox + half * 8 + tig * 2) * 128 + ((gid ^ (tig * 2)) << 4);
+          const unsigned char* r1 =
+              v_ptr + (u * kBox + half * 8 + tig * 2 + 1) * 128 + ((gid ^ (tig * 2 + 1)) << 4);
+#pragma unroll
+          for (int i = 0; i < kMTiles; i += 2) {
+            const uint4 x = *reinterpret_cast<const uint4*>(r0 + (i >> 1) * L::kColumn);
+            const uint4 y = *reinterpret_cast<const uint4*>(r1 + (i >> 1) * L::kColumn);
+            uint32_t big[2][4], small[2][4];
+            cut_tf32(x.x, big[0][0], small[0][0]);
+            cut_tf32(x.y, big[0][1], small[0][1]);
+            cut_tf32(y.x, big[0][2], small[0][2]);
+            cut_tf32(y.y, big[0][3], small[0][3]);
+            cut_tf32(x.z, big[1][0], small[1][0]);
+            cut_tf32(x.w, big[1][1], small[1][1]);
+            cut_tf32(y.z, big[1][2], small[1][2]);
+            cut_tf32(y.w, big[1][3], small[1][3]);
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) {
+                mma_tf32(o[c][i + v], small[v], big_p[c][0], big_p[c][1]);
+                mma_tf32(o[c][i + v], big[v], small_p[c][0], small_p[c][1]);
+                mma_tf32(o[c][i + v], big[v], big_p[c][0], big_p[c][1]);
+              }
+          }
+        }
     }
     __syncwarp();
-    fill();
-    slot_out = slot_out + 1 == L::kSlots ? 0 : slot_out + 1;
+    if constexpr (L::kSlots % 2 == 0) fill_v();
+    else fill_k();
+    released();
 
     // ---- the end of the sequence's head block, or of this warp's share
     const bool ends = use.tile + 1 == use.tiles;
@@ -595,7 +782,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       const int64_t part = 2 * w + (begins ? 1 : 0);
       if (begins && !ends && g.jobs && lane == 0) {
         g.jobs[2 * w] = use.b;
-        g.jobs[2 * w + 1] = use.head;
+        g.jobs[2 * w + 1] = use.hk * g.blocks + use.block;
       }
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
@@ -636,8 +823,9 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
         }
       }
     }
-    use.next(g, heads);
+    use.next(g);
   }
+  if (kTma && t < count) give_up();  // only if the lengths change under the kernel
 }
 
 // Launches attend_kernel for g.a.kv's head_dim and g.block; one definition per
@@ -651,17 +839,55 @@ void launch_attend<__half>(const AttendArgs& g, cudaStream_t st);
 template <>
 void launch_attend<__nv_bfloat16>(const AttendArgs& g, cudaStream_t st);
 
+// The cache as [pages, kv_heads, page, head_dim] for boxes of 16 rows of 128
+// bytes; false when TMA cannot take it (a tile might leave its page, or a
+// stride is none of a tensor map's).
+template <typename T>
+bool make_map(const InfercPagedKv& kv, bool values, CUtensorMap* map) {
+  if (kv.page_size % kBox != 0 || kv.num_pages == 0) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size,
+                              (cuuint64_t)kv.kv_heads, (cuuint64_t)kv.num_pages};
+  const int64_t s[3] = {values ? kv.v_token_stride : kv.k_token_stride,
+                        values ? kv.v_head_stride : kv.k_head_stride,
+                        values ? kv.v_page_stride : kv.k_page_stride};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    if (s[i] <= 0) return false;
+    strides[i] = (cuuint64_t)s[i] * sizeof(T);
+  }
+  const cuuint32_t box[4] = {128 / sizeof(T), kBox, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = std::is_same_v<T, float>    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return tc::encode_fn()(map, type, 4, values ? kv.v : kv.k, dims, strides, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int kDim>
 void launch_attend_dim(const AttendArgs& g, cudaStream_t st) {
   using L = Layout<T, kDim>;
   static_assert(L::kSlots >= 3, "the ring needs three slots");
   const unsigned grid = (unsigned)((g.warps + kWarps - 1) / kWarps);
-  auto* kernel = g.block <= 8 ? attend_kernel<T, kDim, 1> : attend_kernel<T, kDim, 2>;
-  IDEV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
-  kernel<<<grid, kWarps * 32, L::kSmem, st>>>(g);
+  CUtensorMap k_map{}, v_map{};
+  const bool tma = make_map<T>(g.a.kv, false, &k_map) && make_map<T>(g.a.kv, true, &v_map);
+  const bool one = g.block <= 8;
+  auto* kernel = tma ? (one ? attend_kernel<T, kDim, 1, true> : attend_kernel<T, kDim, 2, true>)
+                     : (one ? attend_kernel<T, kDim, 1, false> : attend_kernel<T, kDim, 2, false>);
+  // one request per kernel and device
+  constexpr int kMost = 64;
+  static std::atomic<bool> ready[kMost][4];
+  int dev = 0;
+  IDEV_CUDA(cudaGetDevice(&dev));
+  std::atomic<bool>* known = dev < kMost ? &ready[dev][(tma ? 2 : 0) + (one ? 1 : 0)] : nullptr;
+  if (!known || !known->load(std::memory_order_relaxed)) {
+    IDEV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
+    if (known) known->store(true, std::memory_order_relaxed);
+  }
+  kernel<<<grid, kWarps * 32, L::kSmem, st>>>(g, k_map, v_map);
   IDEV_LAUNCHED();
 }
-
 
 template <typename T>
 void launch_attend_any(const AttendArgs& g, cudaStream_t st) {
@@ -673,13 +899,18 @@ void launch_attend_any(const AttendArgs& g, cudaStream_t st) {
   else launch_attend_dim<T, 256>(g, st);
 }
 
+// Positions per tile and resident blocks per SM of the kernel for a head_dim.
+struct Shape {
+  int tile, blocks;
+};
 template <typename T>
-int blocks_per_sm(int d) {
-  return d <= 64    ? Layout<T, 64>::kBlocks
-         : d <= 96  ? Layout<T, 96>::kBlocks
-         : d <= 128 ? Layout<T, 128>::kBlocks
-         : d <= 192 ? Layout<T, 192>::kBlocks
-                    : Layout<T, 256>::kBlocks;
+Shape shape_of(int d) {
+  auto of = [](auto l) { return Shape{decltype(l)::kTile, decltype(l)::kBlocks}; };
+  return d <= 64    ? of(Layout<T, 64>())
+         : d <= 96  ? of(Layout<T, 96>())
+         : d <= 128 ? of(Layout<T, 128>())
+         : d <= 192 ? of(Layout<T, 192>())
+                    : of(Layout<T, 256>());
 }
 
 }  // namespace paged

@@ -5,6 +5,7 @@
 // a few operations per value, so they are bound by HBM, and by launch latency
 // when few tokens are in flight.
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <string>
 
@@ -14,11 +15,19 @@ namespace inferc_dev {
 
 namespace paged {
 
-__device__ int g_range;  // an index pointed outside its buffer
+// [0]: an index pointed outside its buffer; [1]: a wait for a copy gave up
+__device__ int g_flags[2];
 
 int* range_flag_ptr() {
-  int* p = nullptr;
-  IDEV_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_range));
+  constexpr int kMost = 64;
+  static std::atomic<int*> known[kMost];  // one lookup per device
+  int dev = 0;
+  IDEV_CUDA(cudaGetDevice(&dev));
+  int* p = dev < kMost ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (!p) {
+    IDEV_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_flags));
+    if (dev < kMost) known[dev].store(p, std::memory_order_relaxed);
+  }
   return p;
 }
 
@@ -63,14 +72,14 @@ void check_kv(const InfercPagedKv* kv, const char* op) {
 
 }  // namespace paged
 
-int read_and_clear_paged_range() {
-  int v = 0;
-  IDEV_CUDA(cudaMemcpyFromSymbol(&v, paged::g_range, sizeof(int)));
-  if (v) {
-    const int z = 0;
-    IDEV_CUDA(cudaMemcpyToSymbol(paged::g_range, &z, sizeof(int)));
+int read_and_clear_paged() {
+  int v[2] = {0, 0};
+  IDEV_CUDA(cudaMemcpyFromSymbol(v, paged::g_flags, sizeof v));
+  if (v[0] | v[1]) {
+    const int z[2] = {0, 0};
+    IDEV_CUDA(cudaMemcpyToSymbol(paged::g_flags, z, sizeof z));
   }
-  return v;
+  return v[0] | v[1] << 1;
 }
 
 namespace paged {

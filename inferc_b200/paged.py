@@ -10,7 +10,6 @@ inferc_dev_stream_synchronize (INFERC_ERR_RANGE) and never followed.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -20,43 +19,55 @@ from .lib import HeadRotary as _Rotary
 from .lib import PagedKv as _Kv
 
 _DTYPES = {torch.float32: 1, torch.float16: 10, torch.bfloat16: 16}
+_F32, _I32 = torch.float32, torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_nothing = contextlib.nullcontext()
+_current_device = torch._C._cuda_getDevice
+_call = _lib.load  # the library, loaded on first use
+
+# These functions run once per layer and step, so their checks read each
+# attribute once and build no message before it is needed.
 
 
-def _need(ok: bool, name: str, what: str) -> None:
-    if not ok:
-        raise RuntimeError(f"{name}: {what}")
+def _run(dev: int, fn, *args) -> None:
+    """Calls an entry point on the tensors' device and its current stream."""
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc)
 
 
-def _on(device: torch.device):
-    """The device's context, entered only when it is not the current one."""
-    if device.index == torch.cuda.current_device():
-        return _nothing
-    return torch.cuda.device(device)
-
-
-def _rows(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device,
+def _rows(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, dev: int,
           heads: int | None, dim: int, rows: int | None) -> tuple[int, int, int]:
     """(address, row stride, head stride) of a [rows, heads, dim] tensor."""
-    if t.dtype != dtype or t.device != device:
-        raise RuntimeError(f"{name}: {what} must be {dtype} on {device}")
-    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads) or \
-            (rows is not None and t.shape[0] != rows):
-        raise RuntimeError(f"{name}: {what} must be [{rows or 'rows'}, {heads or 'heads'}, {dim}],"
-                           f" got {list(t.shape)}")
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise RuntimeError(f"{name}: {what} must be {dtype} on CUDA device {dev}")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads) or \
+            (rows is not None and shape[0] != rows):
+        raise RuntimeError(f"{name}: {what} must be [{'rows' if rows is None else rows}, "
+                           f"{'heads' if heads is None else heads}, {dim}], got {list(shape)}")
     a, b, c = t.stride()
     if c != 1:
         raise RuntimeError(f"{name}: the last dimension of {what} must be contiguous")
     return t.data_ptr(), a, b
 
 
-def _ints(name: str, what: str, t: torch.Tensor, shape: tuple, device: torch.device) -> int:
-    if t.dtype != torch.int32 or t.device != device or t.shape != shape or \
+def _flat(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple,
+          dev: int) -> int:
+    """Address of a contiguous tensor of the given type and shape."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or \
             not t.is_contiguous():
-        raise RuntimeError(f"{name}: {what} must be a contiguous int32 tensor {list(shape)} on "
-                           f"{device}")
+        raise RuntimeError(f"{name}: {what} must be a contiguous {dtype} tensor {list(shape)} on "
+                           f"CUDA device {dev}")
     return t.data_ptr()
+
+
+def _need(ok: bool, name: str, what: str) -> None:
+    if not ok:
+        raise RuntimeError(f"{name}: {what}")
 
 
 class PagedKV:
@@ -88,7 +99,7 @@ class PagedKV:
               and lens.shape[0] == page_table.shape[0] and lens.is_contiguous(), n,
               "lens must be a contiguous int32 tensor [batch]")
         self.k, self.v, self.page_table, self.lens = k_cache, v_cache, page_table, lens
-        self.dtype, self.device = k_cache.dtype, dev
+        self.dtype, self.dev = k_cache.dtype, k_cache.get_device()
         pages, self.kv_heads, self.page, self.head_dim = k_cache.shape
         self.batch, self.max_pages = page_table.shape
         self.capacity = self.max_pages * self.page
@@ -103,53 +114,48 @@ class PagedKV:
 
     def _workspace(self, q_heads: int, weights: bool) -> int:
         """Scratch bytes of one attention call (sizes only, so computed once)."""
-        key = (q_heads, weights)
-        if key not in self._scratch:
-            got = _lib.load().inferc_dev_paged_decode_attention_workspace(self.ref, q_heads,
-                                                                          int(weights))
+        got = self._scratch.get((q_heads, weights))
+        if got is None:
+            got = _call().inferc_dev_paged_decode_attention_workspace(self.ref, q_heads,
+                                                                      int(weights))
             if got < 0:
-                raise RuntimeError(_lib.load().inferc_dev_last_error_string().decode())
-            self._scratch[key] = got
-        return self._scratch[key]
+                raise RuntimeError(_call().inferc_dev_last_error_string().decode())
+            self._scratch[(q_heads, weights)] = got
+        return got
 
 
 def _weights(name: str, what: str, kv: PagedKV, w: torch.Tensor) -> tuple[int, int, int]:
-    if w.dtype != torch.float32 or w.device != kv.device or w.dim() != 3 or \
-            w.shape[0] != kv.batch or w.shape[1] != kv.kv_heads or w.shape[2] < kv.capacity or \
-            (w.shape[2] > 1 and w.stride(2) != 1):
+    shape, (a, b, c) = w.shape, w.stride() if w.dim() == 3 else (0, 0, 0)
+    if w.dtype is not _F32 or w.get_device() != kv.dev or len(shape) != 3 or \
+            shape[0] != kv.batch or shape[1] != kv.kv_heads or shape[2] < kv.capacity or \
+            (shape[2] > 1 and c != 1):
         raise RuntimeError(f"{name}: {what} must be float32 [{kv.batch}, {kv.kv_heads}, "
-                           f">= {kv.capacity}] on {kv.device}, contiguous in its last dimension")
-    return w.data_ptr(), w.stride(0), w.stride(1)
+                           f">= {kv.capacity}] on CUDA device {kv.dev}, contiguous in its last "
+                           "dimension")
+    return w.data_ptr(), a, b
 
 
-def _rotary(name: str, dev: torch.device, dim: int, tokens: int, q_gamma, k_gamma, eps: float,
-            cos, sin, positions, interleaved: bool) -> _Rotary:
+def _rotary(name: str, dev: int, dim: int, tokens: int, q_gamma, k_gamma, eps: float, cos, sin,
+            positions, interleaved: bool) -> _Rotary:
     gq = gk = c = s = p = None
-    table_len = stride = rot = 0
+    table_len = half = 0
     if q_gamma is not None:
-        _need(q_gamma.dtype == torch.float32 and q_gamma.device == dev
-              and q_gamma.shape == (dim,) and q_gamma.is_contiguous(), name,
-              f"q_gamma must be float32 [{dim}] on {dev}")
-        gq = q_gamma.data_ptr()
+        gq = _flat(name, "q_gamma", q_gamma, _F32, (dim,), dev)
     if k_gamma is not None:
-        _need(k_gamma.dtype == torch.float32 and k_gamma.device == dev
-              and k_gamma.shape == (dim,) and k_gamma.is_contiguous(), name,
-              f"k_gamma must be float32 [{dim}] on {dev}")
-        gk = k_gamma.data_ptr()
-    if (cos is None) != (sin is None):
-        raise RuntimeError(f"{name}: cos and sin come together")
-    if cos is not None:
-        _need(cos.dim() == 2 and cos.dtype == torch.float32 and sin.dtype == torch.float32
-              and cos.device == dev and sin.device == dev and cos.shape == sin.shape
-              and cos.is_contiguous() and sin.is_contiguous(), name,
-              "cos and sin must be contiguous float32 tables [positions, rotary_dim / 2]")
-        table_len, half = cos.shape
-        _need(half >= 1 and table_len >= 1 and 2 * half <= dim, name,
-              "rotary_dim must be at most head_dim")
-        c, s, stride, rot = cos.data_ptr(), sin.data_ptr(), half, 2 * half
+        gk = _flat(name, "k_gamma", k_gamma, _F32, (dim,), dev)
+    if cos is not None and sin is not None:
+        shape = cos.shape
+        if len(shape) != 2 or shape[0] < 1 or not 1 <= shape[1] <= dim // 2:
+            raise RuntimeError(f"{name}: cos and sin must be [positions, rotary_dim / 2], with "
+                               "rotary_dim at most head_dim")
+        table_len, half = shape
+        c = _flat(name, "cos", cos, _F32, shape, dev)
+        s = _flat(name, "sin", sin, _F32, shape, dev)
         if positions is not None:
-            p = _ints(name, "positions", positions, (tokens,), dev)
-    return _Rotary(gq, gk, c, s, p, table_len, stride, eps, rot, int(interleaved))
+            p = _flat(name, "positions", positions, _I32, (tokens,), dev)
+    elif cos is not None or sin is not None:
+        raise RuntimeError(f"{name}: cos and sin come together")
+    return _Rotary(gq, gk, c, s, p, table_len, half, eps, 2 * half, interleaved)
 
 
 def RotaryTable(positions: int, rotary_dim: int, base: float = 10000.0, device="cuda"
@@ -173,23 +179,27 @@ def QKNormRotary(q: torch.Tensor, k: torch.Tensor, q_gamma=None, k_gamma=None, e
     kv_heads, d], e.g. column blocks of one projection; positions int32 [T]
     (None: 0..T-1). q_out / k_out may be q / k themselves."""
     name = "QKNormRotary"
-    _need(q.is_cuda and q.dtype in _DTYPES and q.dim() == 3, name,
-          "q must be [tokens, heads, head_dim], float32, float16 or bfloat16, on a CUDA device")
-    tokens, heads, dim = q.shape
-    dev, dt = q.device, q.dtype
+    dt, dev, shape = q.dtype, q.get_device(), q.shape
+    if dev < 0 or dt not in _DTYPES or len(shape) != 3:
+        raise RuntimeError(f"{name}: q must be [tokens, heads, head_dim], float32, float16 or "
+                           "bfloat16, on a CUDA device")
+    tokens, heads, dim = shape
     a = _rows(name, "q", q, dt, dev, None, dim, None)
     b = _rows(name, "k", k, dt, dev, None, dim, tokens)
+    kv_heads = k.shape[1]
     if q_out is None:
-        q_out = torch.empty((tokens, heads, dim), dtype=dt, device=dev)
+        q_out = q.new_empty(shape)
+        c = (q_out.data_ptr(), heads * dim, dim)
+    else:
+        c = _rows(name, "q_out", q_out, dt, dev, heads, dim, tokens)
     if k_out is None:
-        k_out = torch.empty((tokens, k.shape[1], dim), dtype=dt, device=dev)
-    c = _rows(name, "q_out", q_out, dt, dev, heads, dim, tokens)
-    e = _rows(name, "k_out", k_out, dt, dev, k.shape[1], dim, tokens)
+        k_out = k.new_empty((tokens, kv_heads, dim))
+        e = (k_out.data_ptr(), kv_heads * dim, dim)
+    else:
+        e = _rows(name, "k_out", k_out, dt, dev, kv_heads, dim, tokens)
     rot = _rotary(name, dev, dim, tokens, q_gamma, k_gamma, eps, cos, sin, positions, interleaved)
-    with _on(dev):
-        _lib.check(_lib.load().inferc_dev_qk_norm_rotary(
-            ctypes.byref(rot), _DTYPES[dt], *a, *b, *c, *e, tokens, heads, k.shape[1], dim,
-            _raw_stream(dev.index)))
+    _run(dev, _call().inferc_dev_qk_norm_rotary, ctypes.byref(rot), _DTYPES[dt], *a, *b, *c, *e,
+         tokens, heads, kv_heads, dim)
     return q_out, k_out
 
 
@@ -197,7 +207,7 @@ def _cu(name: str, kv: PagedKV, cu_tokens, tokens: int):
     if cu_tokens is None:
         _need(tokens == kv.batch, name, "without cu_tokens there is one token per sequence")
         return None
-    return _ints(name, "cu_tokens", cu_tokens, (kv.batch + 1,), kv.device)
+    return _flat(name, "cu_tokens", cu_tokens, _I32, (kv.batch + 1,), kv.dev)
 
 
 def PagedKVAppend(kv: PagedKV, k: torch.Tensor, v: torch.Tensor,
@@ -206,13 +216,12 @@ def PagedKVAppend(kv: PagedKV, k: torch.Tensor, v: torch.Tensor,
     sequences: rows cu_tokens[b]..cu_tokens[b+1]-1 belong to sequence b (None:
     one row per sequence), whose lens count them already."""
     name = "PagedKVAppend"
-    a = _rows(name, "k", k, kv.dtype, kv.device, kv.kv_heads, kv.head_dim, None)
-    b = _rows(name, "v", v, kv.dtype, kv.device, kv.kv_heads, kv.head_dim, k.shape[0])
-    cu = _cu(name, kv, cu_tokens, k.shape[0])
-    with _on(kv.device):
-        _lib.check(_lib.load().inferc_dev_paged_kv_append(
-            kv.ref, None, None, 0, 0, *a, *b, None, 0, 0, 0, cu, k.shape[0],
-            _raw_stream(kv.device.index)))
+    a = _rows(name, "k", k, kv.dtype, kv.dev, kv.kv_heads, kv.head_dim, None)
+    tokens = k.shape[0]
+    b = _rows(name, "v", v, kv.dtype, kv.dev, kv.kv_heads, kv.head_dim, tokens)
+    cu = _cu(name, kv, cu_tokens, tokens)
+    _run(kv.dev, _call().inferc_dev_paged_kv_append, kv.ref, None, None, 0, 0, *a, *b, None, 0, 0,
+         0, cu, tokens)
 
 
 def QKNormRotaryAppend(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -224,19 +233,20 @@ def QKNormRotaryAppend(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.T
     slot in the cache (give them where earlier positions were evicted). Rows of
     q_out behind the last sequence are left as they are."""
     name = "QKNormRotaryAppend"
-    dev, dt, dim = kv.device, kv.dtype, kv.head_dim
+    dev, dt, dim = kv.dev, kv.dtype, kv.head_dim
     a = _rows(name, "q", q, dt, dev, None, dim, None)
-    tokens, heads = q.shape[0], q.shape[1]
+    tokens, heads, _ = q.shape
     b = _rows(name, "k", k, dt, dev, kv.kv_heads, dim, tokens)
     c = _rows(name, "v", v, dt, dev, kv.kv_heads, dim, tokens)
     if q_out is None:
-        q_out = torch.empty((tokens, heads, dim), dtype=dt, device=dev)
-    e = _rows(name, "q_out", q_out, dt, dev, heads, dim, tokens)
+        q_out = q.new_empty((tokens, heads, dim))
+        e = (q_out.data_ptr(), heads * dim, dim)
+    else:
+        e = _rows(name, "q_out", q_out, dt, dev, heads, dim, tokens)
     rot = _rotary(name, dev, dim, tokens, q_gamma, k_gamma, eps, cos, sin, positions, interleaved)
     cu = _cu(name, kv, cu_tokens, tokens)
-    with _on(dev):
-        _lib.check(_lib.load().inferc_dev_paged_kv_append(
-            kv.ref, ctypes.byref(rot), *a, *b, *c, *e, heads, cu, tokens, _raw_stream(dev.index)))
+    _run(dev, _call().inferc_dev_paged_kv_append, kv.ref, ctypes.byref(rot), *a, *b, *c, *e, heads,
+         cu, tokens)
     return q_out
 
 
@@ -250,21 +260,22 @@ def PagedDecodeAttention(q: torch.Tensor, kv: PagedKV, scale: float | None = Non
     page], to which each position's softmax weight is added, summed over the
     query heads of its key head."""
     name = "PagedDecodeAttention"
-    dev, dt, dim = kv.device, kv.dtype, kv.head_dim
-    a = _rows(name, "q", q, dt, dev, None, dim, kv.batch)
+    dev, dt, dim, batch = kv.dev, kv.dtype, kv.head_dim, kv.batch
+    a = _rows(name, "q", q, dt, dev, None, dim, batch)
     heads = q.shape[1]
-    _need(heads >= 1 and heads % kv.kv_heads == 0, name,
-          "the query heads must be a multiple of kv_heads")
+    if heads < 1 or heads % kv.kv_heads:
+        raise RuntimeError(f"{name}: the query heads must be a multiple of kv_heads")
     if out is None:
-        out = torch.empty((kv.batch, heads, dim), dtype=dt, device=dev)
-    b = _rows(name, "out", out, dt, dev, heads, dim, kv.batch)
+        out = q.new_empty((batch, heads, dim))
+        b = (out.data_ptr(), heads * dim, dim)
+    else:
+        b = _rows(name, "out", out, dt, dev, heads, dim, batch)
     w = (None, 0, 0) if weights is None else _weights(name, "weights", kv, weights)
     size = kv._workspace(heads, weights is not None)
-    with _on(dev):
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        _lib.check(_lib.load().inferc_dev_paged_decode_attention(
-            kv.ref, *a, heads, dim ** -0.5 if scale is None else scale, *b, *w,
-            ws.data_ptr() if size else None, size, _raw_stream(dev.index)))
+    # scratch of this call alone, in stream order, so that calls on other streams may overlap
+    ws = kv.lens.new_empty((size + 3) // 4) if size else None
+    _run(dev, _call().inferc_dev_paged_decode_attention, kv.ref, *a, heads,
+         dim ** -0.5 if scale is None else scale, *b, *w, ws.data_ptr() if size else None, size)
     return out
 
 
@@ -281,9 +292,9 @@ def PagedKVEvict(kv: PagedKV, weights: torch.Tensor, keep: int, recent: int = 0,
     new lengths, a tensor apart from kv.lens; the old positions, int32 [batch,
     kv_heads, keep], -1 behind the last; and the weights."""
     name = "PagedKVEvict"
-    dev = kv.device
-    _need(keep >= 1 and 0 <= recent <= keep, name,
-          "keep must be at least 1 and recent in [0, keep]")
+    dev, batch = kv.dev, kv.batch
+    if keep < 1 or not 0 <= recent <= keep:
+        raise RuntimeError(f"{name}: keep must be at least 1 and recent in [0, keep]")
     w = _weights(name, "weights", kv, weights)
     wo = (None, 0, 0)
     if weights_out is None:
@@ -292,20 +303,22 @@ def PagedKVEvict(kv: PagedKV, weights: torch.Tensor, keep: int, recent: int = 0,
         wo = _weights(name, "weights_out", kv, weights_out)
     dst = (None, 0, 0)
     if dst_table is not None:
-        _need(dst_table.dtype == torch.int32 and dst_table.device == dev and dst_table.dim() == 2
-              and dst_table.shape[0] == kv.batch
-              and (dst_table.shape[1] <= 1 or dst_table.stride(1) == 1), name,
-              "dst_table must be int32 [batch, pages] with contiguous rows")
-        pages = dst_table.shape[1]
-        dst = (dst_table.data_ptr(), pages,
-               max(dst_table.stride(0), pages) if kv.batch <= 1 else dst_table.stride(0))
+        shape = dst_table.shape
+        if dst_table.dtype is not _I32 or dst_table.get_device() != dev or len(shape) != 2 or \
+                shape[0] != batch or (shape[1] > 1 and dst_table.stride(1) != 1):
+            raise RuntimeError(f"{name}: dst_table must be int32 [batch, pages] with contiguous "
+                               f"rows on CUDA device {dev}")
+        dst = (dst_table.data_ptr(), shape[1],
+               max(dst_table.stride(0), shape[1]) if batch <= 1 else dst_table.stride(0))
     if lens_out is None:
-        lens_out = torch.empty((kv.batch,), dtype=torch.int32, device=dev)
+        lens_out = kv.lens.new_empty(batch)
+        a = lens_out.data_ptr()
+    else:
+        a = _flat(name, "lens_out", lens_out, _I32, (batch,), dev)
     if kept is None:
-        kept = torch.empty((kv.batch, kv.kv_heads, keep), dtype=torch.int32, device=dev)
-    a = _ints(name, "lens_out", lens_out, (kv.batch,), dev)
-    b = _ints(name, "kept", kept, (kv.batch, kv.kv_heads, keep), dev)
-    with _on(dev):
-        _lib.check(_lib.load().inferc_dev_paged_kv_evict(
-            kv.ref, *dst, *w, *wo, keep, recent, a, b, _raw_stream(dev.index)))
+        kept = kv.lens.new_empty((batch, kv.kv_heads, keep))
+        b = kept.data_ptr()
+    else:
+        b = _flat(name, "kept", kept, _I32, (batch, kv.kv_heads, keep), dev)
+    _run(dev, _call().inferc_dev_paged_kv_evict, kv.ref, *dst, *w, *wo, keep, recent, a, b)
     return lens_out, kept, weights_out

@@ -32,8 +32,8 @@ extern "C" int check_div(uint32_t d) {
   return 0;
 }
 
-extern "C" int check_shares(int64_t total, int64_t warps, int64_t least) {
-  const int64_t n = warps_used(total, warps, least);
+extern "C" int check_shares(int64_t total, int64_t warps) {
+  const int64_t n = warps_used(total, warps);
   CHECK(n >= 1 && n <= warps && n <= total);
   CHECK(first_tile(0, total, n) == 0 && first_tile(n, total, n) == total);
   for (int64_t w = 0; w < n; ++w) {
@@ -56,7 +56,7 @@ def plan(tmp_path_factory):
                     str(d / "plan.so")], check=True)
     lib = ctypes.CDLL(str(d / "plan.so"))
     lib.check_div.argtypes = [ctypes.c_uint32]
-    lib.check_shares.argtypes = [ctypes.c_int64] * 3
+    lib.check_shares.argtypes = [ctypes.c_int64] * 2
     return lib
 
 
@@ -70,5 +70,4 @@ def test_shares_cover_every_tile_once(plan):
     for total in list(range(1, 60)) + [1183, 1184, 1185, 4735, 4736, 4737, 99991, 10 ** 9 + 7,
                                        2 ** 45 + 3]:
         for warps in (1, 2, 7, 60, 592, 1184, 9472):
-            for least in (1, 2, 4, 8):
-                assert plan.check_shares(total, warps, least) == 0, (total, warps, least)
+            assert plan.check_shares(total, warps) == 0, (total, warps)
