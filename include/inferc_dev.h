@@ -360,8 +360,8 @@ typedef struct InfercPagedKv {
  * NULL: the token's row index (qk_norm_rotary) or its slot in the cache
  * (append). */
 typedef struct InfercHeadRotary {
-  const float* q_gamma;     /* DEVICE [head_dim] or NULL */
-  const float* k_gamma;     /* DEVICE [head_dim] or NULL */
+  const float* q_gamma;     /* DEVICE [head_dim], 16-byte aligned, or NULL */
+  const float* k_gamma;     /* DEVICE [head_dim], 16-byte aligned, or NULL */
   const float* cos;         /* DEVICE */
   const float* sin;         /* DEVICE */
   const int32_t* positions; /* DEVICE [tokens] or NULL */

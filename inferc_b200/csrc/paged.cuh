@@ -16,29 +16,43 @@ namespace paged {
 
 enum DType : int { F32 = 1, F16 = 10, BF16 = 16 };  // ONNX TensorProto codes
 
-// Eight consecutive values of a row (one 16-byte load of a 16-bit type, two
-// of fp32), widened to fp32.
+// Eight consecutive values of a row as they lie in memory (one 16-byte load of
+// a 16-bit type, two of fp32), to be widened when they are used.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-  if constexpr (std::is_same_v<T, float>) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0];
-    const float4 b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Raw8 {
+  static constexpr int kParts = sizeof(T) / 2;
+  uint4 part[kParts] = {};
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 f;
-      if constexpr (std::is_same_v<T, __half>)
-        f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      else
-        f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
+    for (int i = 0; i < kParts; ++i) part[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void widen(float* x) const {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const uint32_t w[4] = {part[i].x, part[i].y, part[i].z, part[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (std::is_same_v<T, float>) {
+          x[4 * i + j] = __uint_as_float(w[j]);
+        } else {
+          float2 f;
+          if constexpr (std::is_same_v<T, __half>)
+            f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          else
+            f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+          x[2 * j] = f.x;
+          x[2 * j + 1] = f.y;
+        }
+      }
     }
   }
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  Raw8<T> raw;
+  raw.load(p);
+  raw.widen(x);
 }
 
 template <typename T>

@@ -9,7 +9,11 @@
 #include <cstring>
 #include <string>
 
+#include <cooperative_groups.h>
+
 #include "paged.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace inferc_dev {
 
@@ -100,8 +104,7 @@ struct RowArgs {
   Heads q, k, v;
   const int32_t* cu;
   int64_t tokens;
-  int d;
-  bool norm_q, norm_k, turn;
+  int d, turn;  // turn: how the pairs lie (Turn)
 };
 
 // Largest b in [0, n) with cu[b] <= t, one warp, 32 probes a step; -1 if none.
@@ -120,123 +123,217 @@ __device__ __forceinline__ int64_t find_seq(const int32_t* cu, int64_t n, int64_
   return n > 0 && cu[lo] <= t ? lo : -1;
 }
 
-// One warp per (token, block of heads). A head's row is spread over G lanes,
-// 8 values (16 bytes of a 16-bit type) each, so the mean of squares is a
-// log2(G)-step shuffle and a row is read and written once, in whole sectors.
-template <typename T, int G>
-__global__ void rows_kernel(const __grid_constant__ RowArgs r, int head_blocks, int64_t warps) {
+// How a row's pairs lie in its lanes.
+enum Turn : int {
+  kNone = 0,     // no rotation
+  kLanes = 1,    // (i, i + half), half a multiple of 8: the partner lane holds all eight
+  kWithin = 2,   // (2 i, 2 i + 1): in the lane itself
+  kAcross = 3    // (i, i + half) at an odd offset: through shared memory
+};
+
+// What one lane needs of a token, the same for all its heads.
+struct LaneTurn {
+  float c[8], s[8];  // s negated where the column is a pair's first
+  uint32_t in;       // bit i: column i is rotated
+};
+
+// Norm and rotation of the heads [h0, h1) of one kind (queries, keys or
+// values) of one token by one warp: G lanes share a row, 8 values each, and 64
+// bytes a lane are fetched before the first are used.
+template <typename T, int G, int kTurn>
+__device__ __forceinline__ void rows_of(const T* src, int64_t src_head, T* dst, int64_t dst_head,
+                                        int h0, int h1, const float* gamma, float eps, int d,
+                                        const LaneTurn& lt, int half, float* stage) {
+  constexpr int kAtOnce = 32 / G, kAhead = sizeof(T) == 4 ? 2 : 4;
+  const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
+  const bool column = c * 8 < d;
+  const float inv_d = 1.0f / (float)d;
+  float gam[8];
+  if (gamma && column) load8(gamma + c * 8, gam);
+  src += (h0 + sub) * src_head + c * 8;
+  dst += (h0 + sub) * dst_head + c * 8;
+  const int64_t src_step = kAtOnce * src_head, dst_step = kAtOnce * dst_head;
+  for (int hb = h0; hb < h1; hb += kAtOnce * kAhead) {
+    Raw8<T> raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      raw[u] = Raw8<T>();
+      if (column && hb + u * kAtOnce + sub < h1) raw[u].load(src);
+      src += src_step;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (hb + u * kAtOnce >= h1) break;  // the same for the whole warp
+      float x[8];
+      raw[u].widen(x);
+      if (gamma) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = rsqrtf(sum * inv_d + eps);
+        if (column)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * gam[i];
+      }
+      if constexpr (kTurn != kNone) {
+        float y[8];
+        if constexpr (kTurn == kWithin) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+        } else if constexpr (kTurn == kLanes) {
+          const int partner = (c * 8 < half ? c + half / 8 : c - half / 8) & (G - 1);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], (lane - c) + partner);
+        } else {
+          __syncwarp();
+          store8(stage + lane * 8, x);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int col = c * 8 + i;
+            y[i] = lt.in >> i & 1 ? stage[(lane - c) * 8 + (col < half ? col + half : col - half)]
+                                  : 0.f;
+          }
+        }
+        if constexpr (kTurn == kLanes) {  // a lane's columns are rotated all or none
+          if (lt.in)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * lt.c[i] + y[i] * lt.s[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (lt.in >> i & 1) x[i] = x[i] * lt.c[i] + y[i] * lt.s[i];
+        }
+      }
+      if (column && hb + u * kAtOnce + sub < h1) store8(dst, x);
+      dst += dst_step;
+    }
+  }
+}
+
+// One warp per (token, block of `per_warp` heads), the heads numbered queries,
+// keys, values. The cosines and sines of the token's position stay in
+// registers for all its heads: read for each head again they were twice the
+// bytes of a 16-bit row (8190 tokens of 40 bf16 heads of 128: 110 us; so
+// XX us, XX of measured HBM).
+template <typename T, int G, int kTurn>
+__global__ void __launch_bounds__(256, 2) rows_kernel(const __grid_constant__ RowArgs r, int per_warp,
+                                                   int head_blocks, int64_t warps) {
+  __shared__ __align__(16) float stage[8][32 * 8];
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (w >= warps) return;
-  const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
+  const int lane = threadIdx.x & 31, c = lane % G;
   const int64_t t = w / head_blocks;
-  const int head = (int)(w % head_blocks) * (32 / G) + sub;
+  const int first = (int)(w - t * head_blocks) * per_warp;
+  const int total = r.q.heads + r.k.heads + r.v.heads;
+  const int last = min(first + per_warp, total);
   int64_t pos = t, b = t;
   const bool paged = r.a.kv.batch > 0;
+  const InfercPagedKv& kv = r.a.kv;
   int page = 0;
   uint32_t slot = 0;
   if (paged) {
-    int64_t first = t, count = 1;
+    int64_t begin = t, count = 1;
     if (r.cu) {
-      if (t >= r.cu[r.a.kv.batch]) return;  // behind the last sequence
-      b = find_seq(r.cu, r.a.kv.batch, t, lane);
+      if (t >= r.cu[kv.batch]) return;  // behind the last sequence
+      b = find_seq(r.cu, kv.batch, t, lane);
       if (b < 0) { *r.a.flag = 1; return; }
-      first = r.cu[b];
-      count = r.cu[b + 1] - first;
+      begin = r.cu[b];
+      count = r.cu[b + 1] - begin;
     }
-    const int64_t len = r.a.kv.lens[b];
-    pos = len - count + (t - first);
-    if (pos < 0 || pos >= len || len > r.a.kv.max_pages * r.a.kv.page_size) {
+    const int64_t len = kv.lens[b];
+    pos = len - count + (t - begin);
+    if (pos < 0 || pos >= len || len > kv.max_pages * kv.page_size) {
       *r.a.flag = 1;
       return;
     }
     const uint32_t index = r.a.page.div((uint32_t)pos);
     slot = (uint32_t)pos - index * r.a.page.d;
-    page = page_of(r.a, r.a.kv.page_table + b * r.a.kv.table_stride, index);
+    page = page_of(r.a, kv.page_table + b * kv.table_stride, index);
     if (page < 0) return;
   }
   if (r.rot.positions) pos = r.rot.positions[t];
-  if (r.turn && (pos < 0 || pos >= r.rot.table_len)) { *r.a.flag = 1; return; }
+  if (kTurn != kNone && (pos < 0 || pos >= r.rot.table_len)) { *r.a.flag = 1; return; }
 
-  const int total = r.q.heads + r.k.heads + r.v.heads;
-  const bool live = head < total && c * 8 < r.d;
-  const bool is_q = head < r.q.heads, is_k = !is_q && head < r.q.heads + r.k.heads;
-  const int h = is_q ? head : is_k ? head - r.q.heads : head - r.q.heads - r.k.heads;
-  const Heads& s = is_q ? r.q : is_k ? r.k : r.v;
-  T* dst = reinterpret_cast<T*>(s.dst) + t * s.dst_token + h * s.dst_head;
-  if (paged && !is_q) {
-    const InfercPagedKv& kv = r.a.kv;
-    dst = is_k ? reinterpret_cast<T*>(kv.k) + page * kv.k_page_stride + h * kv.k_head_stride +
-                     (int64_t)slot * kv.k_token_stride
-               : reinterpret_cast<T*>(kv.v) + page * kv.v_page_stride + h * kv.v_head_stride +
-                     (int64_t)slot * kv.v_token_stride;
-  }
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live) load8(reinterpret_cast<const T*>(s.src) + t * s.src_token + h * s.src_head + c * 8, x);
-
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (live && ((is_q && r.norm_q) || (is_k && r.norm_k))) {
-    const float inv = 1.0f / sqrtf(sum / (float)r.d + r.rot.eps);
-    const float* gamma = (is_q ? r.rot.q_gamma : r.rot.k_gamma) + c * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * gamma[i];
-  }
-  if (r.turn) {
-    const int half = r.rot.rotary_dim / 2;
+  const int half = r.rot.rotary_dim / 2;
+  LaneTurn lt;
+  lt.in = 0;
+  if (kTurn != kNone && first < r.q.heads + r.k.heads) {
     const float* cs = r.rot.cos + pos * r.rot.table_stride;
     const float* sn = r.rot.sin + pos * r.rot.table_stride;
-    const bool turns = live && (is_q || is_k);
-    float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int col = c * 8 + i;
-      const bool in = col < 2 * half;
-      const bool second = r.rot.interleaved ? (i & 1) : col >= half;
-      const int pair = r.rot.interleaved ? col >> 1 : second ? col - half : col;
-      float other;
-      if (r.rot.interleaved) {
-        other = x[i ^ 1];
-      } else if (half % 8 == 0) {
-        const int src = second ? c - half / 8 : c + half / 8;
-        other = __shfl_sync(0xffffffffu, x[i], (lane - c) + (src & (G - 1)));
-      } else {
-        // pairs that straddle lanes at an odd offset: each value of the partner lanes in turn
-        const int pc = second ? col - half : col + half;
-        other = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float z = __shfl_sync(0xffffffffu, x[j], (lane - c) + ((pc >> 3) & (G - 1)));
-          if ((pc & 7) == j) other = z;
-        }
-      }
-      y[i] = x[i];
-      if (turns && in) {
-        const float co = cs[pair], si = sn[pair];
-        y[i] = second ? x[i] * co + other * si : x[i] * co - other * si;
+      const bool second = kTurn == kWithin ? i & 1 : col >= half;
+      const int pair = kTurn == kWithin ? col >> 1 : second ? col - half : col;
+      lt.c[i] = lt.s[i] = 0.f;
+      if (col < 2 * half) {
+        lt.in |= 1u << i;
+        lt.c[i] = cs[pair];
+        lt.s[i] = second ? sn[pair] : -sn[pair];
       }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i];
   }
-  if (live) store8(dst + c * 8, x);
+  float* st = stage[threadIdx.x >> 5];
+  {
+    const int h0 = first, h1 = min(last, r.q.heads);
+    if (h0 < h1)
+      rows_of<T, G, kTurn>(reinterpret_cast<const T*>(r.q.src) + t * r.q.src_token, r.q.src_head,
+                    reinterpret_cast<T*>(r.q.dst) + t * r.q.dst_token, r.q.dst_head, h0, h1,
+                    r.rot.q_gamma, r.rot.eps, r.d, lt, half, st);
+  }
+  {
+    const int h0 = max(first - r.q.heads, 0), h1 = min(last - r.q.heads, r.k.heads);
+    if (h0 < h1) {
+      T* dst = reinterpret_cast<T*>(r.k.dst) + t * r.k.dst_token;
+      if (paged)
+        dst = reinterpret_cast<T*>(kv.k) + page * kv.k_page_stride +
+              (int64_t)slot * kv.k_token_stride;
+      rows_of<T, G, kTurn>(reinterpret_cast<const T*>(r.k.src) + t * r.k.src_token, r.k.src_head, dst,
+                    paged ? kv.k_head_stride : r.k.dst_head, h0, h1, r.rot.k_gamma, r.rot.eps, r.d,
+                           lt, half, st);
+    }
+  }
+  {
+    const int before = r.q.heads + r.k.heads;
+    const int h0 = max(first - before, 0), h1 = min(last - before, r.v.heads);
+    if (h0 < h1)
+      rows_of<T, G, kNone>(reinterpret_cast<const T*>(r.v.src) + t * r.v.src_token, r.v.src_head,
+                    reinterpret_cast<T*>(kv.v) + page * kv.v_page_stride +
+                        (int64_t)slot * kv.v_token_stride,
+                    kv.v_head_stride, h0, h1, nullptr, 0.f, r.d, lt, half, st);
+  }
+}
+
+template <typename T, int G>
+void launch_rows_of(const RowArgs& r, cudaStream_t st) {
+  const int heads = r.q.heads + r.k.heads + r.v.heads;
+  // All heads of a token in one warp when there are tokens for every warp the
+  // SMs hold (16 each); else as few as keep them all busy, so that a decode
+  // step's few tokens do not wait for one another.
+  const int unit = 32 / G;  // heads that a warp takes at once
+  int per_warp = (int)((r.tokens * heads + 148 * 16 - 1) / (148 * 16));
+  per_warp = std::min((per_warp + unit - 1) / unit * unit, (heads + unit - 1) / unit * unit);
+  const int blocks = (heads + per_warp - 1) / per_warp;
+  const int64_t warps = r.tokens * blocks;
+  const int64_t grid = (warps + 7) / 8;
+  IDEV_CHECK_ARG(grid <= INT32_MAX, "too many tokens in one call");
+  auto* kernel = r.turn == kNone    ? rows_kernel<T, G, kNone>
+                 : r.turn == kLanes  ? rows_kernel<T, G, kLanes>
+                 : r.turn == kWithin ? rows_kernel<T, G, kWithin>
+                                     : rows_kernel<T, G, kAcross>;
+  kernel<<<(unsigned)grid, 256, 0, st>>>(r, per_warp, blocks, warps);
+  IDEV_LAUNCHED();
 }
 
 template <typename T>
 void launch_rows(const RowArgs& r, cudaStream_t st) {
-  const int heads = r.q.heads + r.k.heads + r.v.heads;
-  if (r.tokens == 0 || heads == 0) return;
-  const int g = r.d <= 64 ? 8 : r.d <= 128 ? 16 : 32;
-  const int blocks = (heads + 32 / g - 1) / (32 / g);
-  const int64_t warps = r.tokens * blocks;
-  const int64_t grid = (warps + 7) / 8;
-  IDEV_CHECK_ARG(grid <= INT32_MAX, "too many tokens in one call");
-  if (g == 8) rows_kernel<T, 8><<<(unsigned)grid, 256, 0, st>>>(r, blocks, warps);
-  else if (g == 16) rows_kernel<T, 16><<<(unsigned)grid, 256, 0, st>>>(r, blocks, warps);
-  else rows_kernel<T, 32><<<(unsigned)grid, 256, 0, st>>>(r, blocks, warps);
-  IDEV_LAUNCHED();
+  if (r.tokens == 0 || r.q.heads + r.k.heads + r.v.heads == 0) return;
+  if (r.d <= 64) launch_rows_of<T, 8>(r, st);
+  else if (r.d <= 128) launch_rows_of<T, 16>(r, st);
+  else launch_rows_of<T, 32>(r, st);
 }
 
 void dispatch_rows(int dtype, const RowArgs& r, cudaStream_t st) {
@@ -251,18 +348,23 @@ void set_rotary(RowArgs& r, const InfercHeadRotary* rot, const char* op) {
   const std::string o = std::string(op) + ": ";
   IDEV_CHECK_ARG(rot->rotary_dim >= 0 && rot->rotary_dim % 2 == 0 && rot->rotary_dim <= r.d,
                  o + "rotary_dim must be even and at most head_dim");
-  IDEV_CHECK_ARG(!(rot->q_gamma || rot->k_gamma) || rot->eps >= 0.f, o + "eps must not be negative");
+  IDEV_CHECK_ARG(!(rot->q_gamma || rot->k_gamma) ||
+                     (rot->eps >= 0.f && aligned16(rot->q_gamma) && aligned16(rot->k_gamma)),
+                 o + "eps must not be negative, gammas 16-byte aligned");
   if (rot->rotary_dim > 0)
     IDEV_CHECK_ARG(rot->cos && rot->sin && rot->table_len >= 1 &&
                        rot->table_stride >= rot->rotary_dim / 2,
                    o + "rotation needs cos and sin tables [table_len, rotary_dim / 2]");
   r.rot = *rot;
-  r.norm_q = rot->q_gamma != nullptr;
-  r.norm_k = rot->k_gamma != nullptr;
-  r.turn = rot->rotary_dim > 0;
+  r.turn = rot->rotary_dim == 0       ? kNone
+           : rot->interleaved         ? kWithin
+           : rot->rotary_dim % 16 == 0 ? kLanes
+                                       : kAcross;
 }
 
 // ------------------------------------------------------------------ evict
+
+constexpr int kMoveCluster = 8;  // blocks at most that share a (sequence, key head)
 
 struct EvictArgs {
   Args a;
@@ -277,8 +379,10 @@ struct EvictArgs {
   int32_t* kept;
 };
 
-constexpr int kSelThreads = 1024;
+constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kDeep = 4;              // 16-byte loads a lane has in flight, of K and of V
+constexpr int kKeysHeld = 16 * 1024;  // weights a block keeps in shared memory
 
 // Order of weights as unsigned numbers: -0 equals 0, every NaN is the largest.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -300,185 +404,253 @@ __device__ __forceinline__ uint64_t block_exclusive(uint64_t v, uint64_t* warp_s
   __syncthreads();  // warp_sums of the previous call are read
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
-  if (warp == 0) {
-    uint64_t x = warp_sums[lane];
+  uint64_t before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t n = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += n;
-    }
-    warp_sums[lane] = x;
+  for (int i = 0; i < kEvictWarps; ++i) {
+    const uint64_t x = warp_sums[i];
+    if (i < warp) before += x;
+    all += x;
   }
-  __syncthreads();
-  *total = warp_sums[31];
-  return s - v + (warp ? warp_sums[warp - 1] : 0);
+  *total = all;
+  return before + s - v;
 }
 
-// One block per (sequence, key head): finds the weight of rank keep - recent
-// by three histograms of 11, 11 and 10 bits of its key, then walks the
-// positions in order, packing what stays. A position's new place is the
-// number of larger weights before it plus the equal ones before it that stay,
-// so ties go to the lowest index whatever the threads' order.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictArgs e) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint64_t sums[32];
-  __shared__ uint32_t s_prefix, s_need;
-  const int hk = (int)e.a.kv.kv_heads;
-  const int64_t b = blockIdx.x / hk;
-  const int h = blockIdx.x % hk, tid = threadIdx.x;
+// One cluster per (sequence, key head).
+//
+// Choice: the weight of rank keep - recent by histograms of 11, 11 and 10 bits
+// of its key (each block counts its slice of the positions, the blocks add up
+// each other's counts through distributed shared memory), ending early when a
+// bin stays whole. A position's new place is the number of larger weights
+// before it plus the equal ones before it that stay, so ties go to the lowest
+// position whatever the threads' order.
+//
+// Move: rows go to the front in steps of the whole cluster. In place, a row's
+// source lies at or behind its destination (kept[i] >= i), so of a step's rows
+// all loads come before any store (a cluster barrier), and the sources of later
+// steps lie behind what earlier ones wrote. A warp looks up the pages of its
+// rows one row per lane and passes the addresses on by shuffles: the kLanes
+// lanes of a row fetch 16 bytes each. (One thread per 16 bytes, each finding
+// its own page, took 98 instructions per piece and 131 us for 543 MB; so XX.)
+template <int kLanes, int kTurns, bool kInPlace>
+__global__ void __launch_bounds__(kEvictThreads, 2)
+    evict_kernel(const __grid_constant__ EvictArgs e, int keys_held) {
+  __shared__ __align__(16) uint32_t hist[3][kBins];
+  __shared__ uint64_t sums[kEvictWarps];
+  __shared__ uint64_t s_count;  // larger (high half) and equal weights in this block's slice
+  __shared__ uint32_t s_bin, s_left, s_whole;
+  extern __shared__ uint32_t keys[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const InfercPagedKv& kv = e.a.kv;
+  const int hk = (int)kv.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t job = blockIdx.x / blocks;
+  const int64_t b = job / hk;
+  const int h = (int)(job - b * hk);
   const int n = seq_len(e.a, b);
   const int m = min(n, e.keep);
-  float* w = e.w + b * e.w_batch + h * e.w_head;
+  const float* w = e.w + b * e.w_batch + h * e.w_head;
   float* wo = e.w_out + b * e.wo_batch + h * e.wo_head;
-  int32_t* kept = e.kept + ((int64_t)b * hk + h) * e.keep;
-  if (h == 0 && tid == 0) e.lens_out[b] = m;
-  for (int i = m + tid; i < e.keep; i += kSelThreads) kept[i] = -1;
+  int32_t* kept = e.kept + job * e.keep;
+  const int all_threads = blocks * kEvictThreads, all_tid = rank * kEvictThreads + tid;
+  if (h == 0 && all_tid == 0) e.lens_out[b] = m;
+  for (int i = m + all_tid; i < e.keep; i += all_threads) kept[i] = -1;
+
+  // ---- choice
   if (n <= e.keep) {
-    for (int i = tid; i < n; i += kSelThreads) {
-      kept[i] = i;
-      if (wo != w) wo[i] = w[i];
-    }
-    return;
-  }
-  const int limit = n - e.recent, need = e.keep - e.recent;
-  uint32_t prefix = 0, mask = 0, left = need;
-  if (need > 0) {
-    const int shifts[3] = {21, 10, 0};
-    const uint32_t widths[3] = {2047u, 2047u, 1023u};
-    for (int pass = 0; pass < 3; ++pass) {
-      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int j = tid; j < limit; j += kSelThreads) {
-        const uint32_t k = weight_key(w[j]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shifts[pass]) & widths[pass]], 1u);
-      }
-      __syncthreads();
-      // bins from the largest down; this thread's two are 2 tid and 2 tid + 1
-      const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
-      uint64_t total;
-      const uint32_t before = (uint32_t)block_exclusive((uint64_t)hi + lo, sums, &total);
-      if (before < left && left <= before + hi + lo) {
-        const bool first = left <= before + hi;
-        s_prefix = (uint32_t)(kBins - 1 - 2 * tid - (first ? 0 : 1));
-        s_need = left - before - (first ? 0 : hi);
-      }
-      __syncthreads();
-      prefix |= s_prefix << shifts[pass];
-      mask |= widths[pass] << shifts[pass];
-      left = s_need;
-    }
-  }
-  // `prefix` is the key of that weight; `left` positions with this very key stay
-  uint64_t done = 0;  // larger ones so far (high half), equal ones (low half)
-  for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    float v = 0.f;
-    bool gt = false, eq = false;
-    if (j < n) v = w[j];
-    if (j < limit && need > 0) {
-      const uint32_t k = weight_key(v);
-      gt = k > prefix;
-      eq = k == prefix;
-    }
-    uint64_t total;
-    const uint64_t at =
-        done + block_exclusive(((uint64_t)gt << 32) | (uint64_t)eq, sums, &total);
-    const uint32_t eq_before = (uint32_t)at, gt_before = (uint32_t)(at >> 32);
-    // (the scan's barriers also separate this chunk's reads from the writes below)
-    if (gt || (eq && eq_before < left)) {
-      const uint32_t to = gt_before + min(eq_before, left);
-      kept[to] = j;
-      wo[to] = v;
-    } else if (j >= limit && j < n) {
-      kept[need + j - limit] = j;
-      wo[need + j - limit] = v;
-    }
-    done += total;
-  }
-  __syncthreads();
-  for (int j = e.keep + tid; j < n; j += kSelThreads) wo[j] = 0.f;
-}
-
-constexpr int kMoveThreads = 256, kMoveItems = 4, kMoveCluster = 8;
-
-// Moves the kept rows of one (sequence, key head) of the keys or the values
-// to the front. In place, a row's source lies at or behind its destination
-// (kept[i] >= i), so of a stretch of rows all loads come before any store
-// (a barrier over the cluster that shares the sequence), and later stretches'
-// sources lie behind what earlier ones wrote.
-template <bool kInPlace>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictArgs e,
-                                                                  int lanes, FastDiv by_lanes) {
-  const int part = blockIdx.x % kMoveCluster;
-  int64_t job = blockIdx.x / kMoveCluster;
-  const bool is_v = job & 1;
-  job >>= 1;
-  const int hk = (int)e.a.kv.kv_heads;
-  const int64_t b = job / hk;
-  const int h = (int)(job % hk);
-  const InfercPagedKv& kv = e.a.kv;
-  const int es = kv.dtype == F32 ? 4 : 2;
-  char* base = reinterpret_cast<char*>(is_v ? kv.v : kv.k) +
-               h * (is_v ? kv.v_head_stride : kv.k_head_stride) * es;
-  const int64_t page_bytes = (is_v ? kv.v_page_stride : kv.k_page_stride) * es;
-  const int64_t slot_bytes = (is_v ? kv.v_token_stride : kv.k_token_stride) * es;
-  const int32_t* src_row = kv.page_table + b * kv.table_stride;
-  const int32_t* dst_row = kInPlace ? src_row : e.dst_table + b * e.dst_stride;
-  pdl_wait();
-  const int m = min(e.lens_out[b], e.keep);
-  const int32_t* kept = e.kept + ((int64_t)b * hk + h) * e.keep;
-  const int per_block = kMoveThreads * kMoveItems;
-  // items (row, 16-byte piece), counted in 32 bits: m * lanes < 2^31 is checked by the host
-  const uint32_t items = (uint32_t)m * lanes;
-  for (uint32_t i0 = 0; i0 < items; i0 += per_block * kMoveCluster) {
-    uint4 val[kMoveItems];
-    char* to[kMoveItems];
+    for (int i = all_tid; i < n; i += all_threads) kept[i] = i;
+    if (kInPlace && !e.dst_table && wo == w) return;  // the whole cluster
+  } else {
+    const int limit = n - e.recent, need = e.keep - e.recent;
+    // slices are multiples of 4 so that a thread's four positions are in one
+    const int slice = ((n + blocks - 1) / blocks + 3) & ~3;
+    const int s0 = min(rank * slice, n), s1 = min(s0 + slice, n);
+    const int c1 = min(s1, limit);  // candidates: [s0, c1)
+    const bool held = slice <= keys_held;
+    auto key_at = [&](int j) { return held ? keys[j - s0] : weight_key(w[j]); };
+    for (int i = tid; i < 3 * kBins; i += kEvictThreads) (&hist[0][0])[i] = 0;
+    if (held)
+      for (int j = s0 + tid; j < c1; j += kEvictThreads) keys[j - s0] = weight_key(w[j]);
+    __syncthreads();
+    uint32_t prefix = 0, mask = 0, left = need;
+    if (need > 0) {
+      for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t width = pass == 2 ? 1023u : 2047u;
+        for (int j = s0 + tid; j < c1; j += kEvictThreads) {
+          const uint32_t k = key_at(j);
+          if ((k & mask) == prefix) atomicAdd(&hist[pass][(k >> shift) & width], 1u);
+        }
+        cluster.sync();
+        // bins from the largest down, four a thread
+        const int low = kBins - 4 - 4 * tid;
+        uint4 c = make_uint4(0, 0, 0, 0);
+        for (int r = 0; r < blocks; ++r) {
+          const uint4 x = *reinterpret_cast<const uint4*>(
+              cluster.map_shared_rank(&hist[pass][low], r));
+          c.x += x.x; c.y += x.y; c.z += x.z; c.w += x.w;
+        }
+        uint64_t total;
+        const uint32_t before =
+            (uint32_t)block_exclusive((uint64_t)c.x + c.y + c.z + c.w, sums, &total);
+        const uint32_t count[4] = {c.w, c.z, c.y, c.x};
+        uint32_t run = before;
 #pragma unroll
-    for (int u = 0; u < kMoveItems; ++u) {
-      const uint32_t i = i0 + part * per_block + u * kMoveThreads + threadIdx.x;
-      to[u] = nullptr;
-      if (i >= items) continue;
-      const uint32_t row = by_lanes.div(i), piece = i - row * lanes;
-      const uint32_t from = (uint32_t)kept[row];
-      if (kInPlace && from == row) continue;
-      const uint32_t sp = e.a.page.div(from), dp = e.a.page.div(row);
-      const int src = page_of(e.a, src_row, sp), dst = page_of(e.a, dst_row, dp);
-      if (src < 0 || dst < 0) continue;
-      val[u] = *reinterpret_cast<const uint4*>(base + src * page_bytes +
-                                               (from - sp * e.a.page.d) * slot_bytes + piece * 16);
-      to[u] = base + dst * page_bytes + (row - dp * e.a.page.d) * slot_bytes + piece * 16;
+        for (int i = 0; i < 4; ++i) {
+          if (run < left && left <= run + count[i]) {
+            s_bin = low + 3 - i;
+            s_left = left - run;
+            s_whole = left - run == count[i];
+          }
+          run += count[i];
+        }
+        __syncthreads();
+        prefix |= s_bin << shift;
+        mask |= width << shift;
+        left = s_left;
+        if (s_whole) break;  // the same in every block
+      }
+    }
+    // (k & mask) > prefix stays, and of those equal to it the first `left`
+    uint64_t mine = 0;
+    if (need > 0)
+      for (int j = s0 + tid; j < c1; j += kEvictThreads) {
+        const uint32_t k = key_at(j) & mask;
+        mine += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
+      }
+    uint64_t total;
+    block_exclusive(mine, sums, &total);
+    if (tid == 0) s_count = total;
+    cluster.sync();
+    uint64_t done = 0;  // in the slices before this one, then in what is done of it
+    for (int r = 0; r < rank; ++r) done += *cluster.map_shared_rank(&s_count, r);
+    for (int j0 = s0; j0 < c1; j0 += kEvictThreads * 4) {
+      const int j = j0 + tid * 4;
+      uint32_t stays = 0;  // bits 0..3 larger, 4..7 equal
+      uint64_t v = 0;
+      if (need > 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j + i < c1) {
+            const uint32_t k = key_at(j + i) & mask;
+            stays |= (uint32_t)(k > prefix) << i | (uint32_t)(k == prefix) << (4 + i);
+            v += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
+          }
+      uint64_t at = done + block_exclusive(v, sums, &total);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t larger = stays >> i & 1, equal = stays >> (4 + i) & 1;
+        const uint32_t eq_before = (uint32_t)at, gt_before = (uint32_t)(at >> 32);
+        const uint32_t to = gt_before + min(eq_before, left);
+        if ((larger || (equal && eq_before < left)) && to < (uint32_t)need) kept[to] = j + i;
+        at += ((uint64_t)larger << 32) | equal;
+      }
+      done += total;
+    }
+    for (int j = max(s0, limit) + tid; j < s1; j += kEvictThreads) kept[need + j - limit] = j;
+  }
+  cluster.sync();  // `kept` is whole (and no block leaves while another reads its counts)
+
+  // ---- move
+  constexpr int kAtOnce = 32 / kLanes, kRows = kDeep / kTurns * kAtOnce;  // rows per warp and step
+  const int es = kv.dtype == F32 ? 4 : 2;
+  const int pieces = kv.head_dim * es / 16;
+  const int32_t* src_row = kv.page_table + b * kv.table_stride;
+  const int32_t* dst_row = e.dst_table ? e.dst_table + b * e.dst_stride : src_row;
+  const char* k_head = static_cast<const char*>(kv.k) + h * kv.k_head_stride * es;
+  const char* v_head = static_cast<const char*>(kv.v) + h * kv.v_head_stride * es;
+  const int step = blocks * kEvictWarps * kRows;
+  for (int base = 0; base < m; base += step) {
+    const int row = base + (rank * kEvictWarps + warp) * kRows + lane;
+    const bool mine = lane < kRows && row < m;
+    bool ok = false;
+    int64_t sk = 0, sv = 0, dk = 0, dv = 0;
+    float weight = 0.f;
+    if (mine) {
+      // (below n unless the weights change under the kernel)
+      const uint32_t from = min((uint32_t)kept[row], (uint32_t)(n - 1));
+      weight = w[from];
+      if (e.dst_table || from != (uint32_t)row) {
+        const uint32_t sp = e.a.page.div(from), dp = e.a.page.div(row);
+        const int src = page_of(e.a, src_row, sp), dst = page_of(e.a, dst_row, dp);
+        const int64_t ss = from - sp * e.a.page.d, ds = row - dp * e.a.page.d;
+        ok = src >= 0 && dst >= 0;
+        if (ok) {
+          sk = (src * kv.k_page_stride + ss * kv.k_token_stride) * es;
+          sv = (src * kv.v_page_stride + ss * kv.v_token_stride) * es;
+          dk = (dst * kv.k_page_stride + ds * kv.k_token_stride) * es;
+          dv = (dst * kv.v_page_stride + ds * kv.v_token_stride) * es;
+        }
+      }
+    }
+    uint4 k_val[kDeep], v_val[kDeep];
+    auto row_at = [&](int u) { return u / kTurns * kAtOnce + lane / kLanes; };
+    auto piece_at = [&](int u) { return lane % kLanes + u % kTurns * 32; };
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      const int r = row_at(u), piece = piece_at(u);
+      const int64_t from_k = __shfl_sync(0xffffffffu, sk, r);
+      const int64_t from_v = __shfl_sync(0xffffffffu, sv, r);
+      const bool live = __shfl_sync(0xffffffffu, (int)ok, r) && piece < pieces;
+      if (live) {
+        k_val[u] = *reinterpret_cast<const uint4*>(k_head + from_k + piece * 16);
+        v_val[u] = *reinterpret_cast<const uint4*>(v_head + from_v + piece * 16);
+      }
     }
     if (kInPlace) {
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
 #pragma unroll
-    for (int u = 0; u < kMoveItems; ++u)
-      if (to[u]) *reinterpret_cast<uint4*>(to[u]) = val[u];
+    for (int u = 0; u < kDeep; ++u) {
+      const int r = row_at(u), piece = piece_at(u);
+      const int64_t to_k = __shfl_sync(0xffffffffu, dk, r);
+      const int64_t to_v = __shfl_sync(0xffffffffu, dv, r);
+      const bool live = __shfl_sync(0xffffffffu, (int)ok, r) && piece < pieces;
+      if (live) {
+        *reinterpret_cast<uint4*>(const_cast<char*>(k_head) + to_k + piece * 16) = k_val[u];
+        *reinterpret_cast<uint4*>(const_cast<char*>(v_head) + to_v + piece * 16) = v_val[u];
+      }
+    }
+    if (mine) wo[row] = weight;
   }
+  // every load of w is done: in place, before the last step's barrier
+  for (int j = m + all_tid; j < n; j += all_threads) wo[j] = 0.f;
 }
 
 void launch_evict(const EvictArgs& e, cudaStream_t st) {
   const InfercPagedKv& kv = e.a.kv;
   const int64_t jobs = kv.batch * kv.kv_heads;
-  evict_select_kernel<<<(unsigned)jobs, kSelThreads, 0, st>>>(e);
-  IDEV_LAUNCHED();
-  const int lanes = kv.head_dim * elem_bytes(kv.dtype) / 16;
+  const int64_t capacity = kv.max_pages * kv.page_size;
+  // Blocks per (sequence, key head): enough for two per SM, but none with
+  // fewer positions than threads.
+  int blocks = 1;
+  while (blocks < kMoveCluster && jobs * blocks < 2 * 148 && capacity > blocks * kEvictThreads)
+    blocks *= 2;
+  const int64_t slice = ((capacity + blocks - 1) / blocks + 3) / 4 * 4;
+  const int held = (int)std::min<int64_t>(slice, kKeysHeld);
+  const int pieces = kv.head_dim * elem_bytes(kv.dtype) / 16;
+  const bool in_place = !e.dst_table || e.w_out == e.w;
+  using Kernel = void (*)(EvictArgs, int);
+  Kernel kernel = pieces <= 8    ? (in_place ? evict_kernel<8, 1, true> : evict_kernel<8, 1, false>)
+                  : pieces <= 16 ? (in_place ? evict_kernel<16, 1, true> : evict_kernel<16, 1, false>)
+                  : pieces <= 32 ? (in_place ? evict_kernel<32, 1, true> : evict_kernel<32, 1, false>)
+                                 : (in_place ? evict_kernel<32, 2, true> : evict_kernel<32, 2, false>);
+  const size_t smem = (size_t)held * 4;
+  if (smem > 16 * 1024)  // with the histograms, past the 48 KB every kernel may have
+    IDEV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kKeysHeld * 4));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(jobs * 2 * kMoveCluster));
-  cfg.blockDim = dim3(kMoveThreads);
+  cfg.gridDim = dim3((unsigned)(jobs * blocks));
+  cfg.blockDim = dim3(kEvictThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kMoveCluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = e.dst_table ? 1 : 2;
-  const FastDiv by((uint32_t)lanes);
-  if (e.dst_table) IDEV_CUDA(cudaLaunchKernelEx(&cfg, evict_move_kernel<false>, e, lanes, by));
-  else IDEV_CUDA(cudaLaunchKernelEx(&cfg, evict_move_kernel<true>, e, lanes, by));
+  cfg.numAttrs = 1;
+  IDEV_CUDA(cudaLaunchKernelEx(&cfg, kernel, e, held));
 }
 
 }  // namespace
