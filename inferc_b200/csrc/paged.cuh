@@ -26,6 +26,22 @@ struct Raw8 {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) part[i] = reinterpret_cast<const uint4*>(p)[i];
   }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) reinterpret_cast<uint4*>(p)[i] = part[i];
+  }
+  // The same of another lane of the warp.
+  __device__ __forceinline__ Raw8 from_lane(int lane) const {
+    Raw8 r;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      r.part[i].x = __shfl_sync(0xffffffffu, part[i].x, lane);
+      r.part[i].y = __shfl_sync(0xffffffffu, part[i].y, lane);
+      r.part[i].z = __shfl_sync(0xffffffffu, part[i].z, lane);
+      r.part[i].w = __shfl_sync(0xffffffffu, part[i].w, lane);
+    }
+    return r;
+  }
   __device__ __forceinline__ void widen(float* x) const {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {

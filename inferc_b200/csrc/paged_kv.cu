@@ -107,20 +107,30 @@ struct RowArgs {
   int d, turn;  // turn: how the pairs lie (Turn)
 };
 
-// Largest b in [0, n) with cu[b] <= t, one warp, 32 probes a step; -1 if none.
-__device__ __forceinline__ int64_t find_seq(const int32_t* cu, int64_t n, int64_t t, int lane) {
-  int64_t lo = 0, size = n;
-  while (size > 1) {
-    const int64_t step = (size + 31) / 32;
-    const int64_t at = lo + lane * step;
-    const bool below = lane * step < size && cu[at] <= t;
-    const int below_n = __popc(__ballot_sync(0xffffffffu, below));
-    if (below_n == 0) return -1;
-    const int64_t skip = (below_n - 1) * step;
-    lo += skip;
-    size = min(step, size - skip);
+// The sequence that token t belongs to, where its tokens begin and how many
+// they are, by one warp: 32 boundaries a step, so that up to 31 sequences cost
+// one load. b: -1 behind the last sequence, -2 when cu is no list of boundaries.
+struct Owner {
+  int64_t b, begin, count;
+};
+__device__ __forceinline__ Owner owner_of_token(const int32_t* cu, int64_t n, int64_t t, int lane) {
+  int64_t lo = 0, size = n + 1;  // the last boundary at t or below is in [lo, lo + size)
+  for (;;) {
+    const int64_t step = (size + 31) / 32, at = lane * step;
+    const int64_t mine = at < size ? cu[lo + at] : INT64_MAX;
+    const int below = __popc(__ballot_sync(0xffffffffu, mine <= t));
+    if (below == 0) return {-2, 0, 0};
+    if (step == 1) {
+      const int64_t b = lo + below - 1;
+      if (b == n) return {-1, 0, 0};
+      const int64_t begin = __shfl_sync(0xffffffffu, mine, below - 1);
+      int64_t end = __shfl_sync(0xffffffffu, mine, below & 31);
+      if (below == size || below == 32) end = cu[b + 1];
+      return {b, begin, end - begin};
+    }
+    lo += (below - 1) * step;
+    size = min(step, size - (below - 1) * step);
   }
-  return n > 0 && cu[lo] <= t ? lo : -1;
 }
 
 // How a row's pairs lie in its lanes.
@@ -131,190 +141,250 @@ enum Turn : int {
   kAcross = 3    // (i, i + half) at an odd offset: through shared memory
 };
 
-// What one lane needs of a token, the same for all its heads.
-struct LaneTurn {
-  float c[8], s[8];  // s negated where the column is a pair's first
-  uint32_t in;       // bit i: column i is rotated
-};
+// Eight floats of a table row from `p`, two at a time 16 bytes where they are aligned.
+__device__ __forceinline__ void table8(const float* p, bool vector, float* x) {
+  if (vector) {
+    load8(p, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+  }
+}
 
-// Norm and rotation of the heads [h0, h1) of one kind (queries, keys or
-// values) of one token by one warp: G lanes share a row, 8 values each, and 64
-// bytes a lane are fetched before the first are used.
+// Rows a group of lanes fetches before it uses the first: 64 bytes a lane.
+template <typename T>
+constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+
+// Rows [hb, h1) as far as they go; behind the last, the last once more (its
+// results are not stored). Lanes without columns keep zeros.
+template <typename T, int G>
+__device__ __forceinline__ void fetch_rows(const T* src, int64_t src_head, int hb, int h1, int d,
+                                           Raw8<T> (&raw)[kAhead<T>]) {
+  const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
+#pragma unroll
+  for (int u = 0; u < kAhead<T>; ++u)
+    if (c * 8 < d && hb < h1)
+      raw[u].load(src + min(hb + u * (32 / G) + sub, h1 - 1) * src_head + c * 8);
+}
+
+// Norm and rotation of the heads [h0, h1) of the queries or the keys of one
+// token by one warp: G lanes share a row, 8 values each. With gamma, c and s folded,
+//   y_i = inv * (x_i * own_i + x_partner * other_i),
+// own_i = gamma_i c_i, other_i = -+ gamma_partner s_i (once per token), so that
+// a row costs one exchange of its raw values and three operations per value.
 template <typename T, int G, int kTurn>
 __device__ __forceinline__ void rows_of(const T* src, int64_t src_head, T* dst, int64_t dst_head,
-                                        int h0, int h1, const float* gamma, float eps, int d,
-                                        const LaneTurn& lt, int half, float* stage) {
-  constexpr int kAtOnce = 32 / G, kAhead = sizeof(T) == 4 ? 2 : 4;
+                                        int h0, int h1, const float* gamma,
+                                        const InfercHeadRotary& rot, int64_t pos, int d,
+                                        float* stage, Raw8<T> (&raw)[kAhead<T>], bool fetched) {
+  constexpr int kAtOnce = 32 / G;
   const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
   const bool column = c * 8 < d;
   const float inv_d = 1.0f / (float)d;
-  float gam[8];
-  if (gamma && column) load8(gamma + c * 8, gam);
-  src += (h0 + sub) * src_head + c * 8;
   dst += (h0 + sub) * dst_head + c * 8;
-  const int64_t src_step = kAtOnce * src_head, dst_step = kAtOnce * dst_head;
-  for (int hb = h0; hb < h1; hb += kAtOnce * kAhead) {
-    Raw8<T> raw[kAhead];
+  const int64_t dst_step = kAtOnce * dst_head;
+  const int half = rot.rotary_dim / 2;
+  const int partner = (c * 8 < half ? c + half / 8 : c - half / 8) & (G - 1);  // kLanes
+
+  float own[8], other[8];
+  uint32_t in = 0;  // columns that are rotated
+  bool ready = false;
+  // One row: what `r` holds, to `to` where `live`.
+  auto row = [&](const Raw8<T>& r, T* to, bool live) {
+    float x[8], y[8], inv = 1.f;
+    r.widen(x);
+    if (gamma) {
+      float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      raw[u] = Raw8<T>();
-      if (column && hb + u * kAtOnce + sub < h1) raw[u].load(src);
-      src += src_step;
+      for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      inv = rsqrtf(sum * inv_d + rot.eps);
+    }
+    if constexpr (kTurn == kWithin) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+    } else if constexpr (kTurn == kLanes) {
+      r.from_lane(lane - c + partner).widen(y);
+    } else if constexpr (kTurn == kAcross) {
+      __syncwarp();
+      store8(stage + lane * 8, x);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = c * 8 + i;
+        y[i] = in >> i & 1 ? stage[(lane - c) * 8 + (col < half ? col + half : col - half)] : 0.f;
+      }
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (hb + u * kAtOnce >= h1) break;  // the same for the whole warp
-      float x[8];
-      raw[u].widen(x);
-      if (gamma) {
-        float sum = 0.f;
+    for (int i = 0; i < 8; ++i) x[i] *= own[i];
+    if constexpr (kTurn == kLanes) {  // a lane's columns are rotated all or none
+      if (in)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+        for (int i = 0; i < 8; ++i) x[i] += y[i] * other[i];
+    } else if constexpr (kTurn != kNone) {
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = rsqrtf(sum * inv_d + eps);
-        if (column)
+      for (int i = 0; i < 8; ++i)
+        if (in >> i & 1) x[i] += y[i] * other[i];
+    }
+    if (gamma)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * gam[i];
-      }
-      if constexpr (kTurn != kNone) {
-        float y[8];
-        if constexpr (kTurn == kWithin) {
+      for (int i = 0; i < 8; ++i) x[i] *= inv;
+    if (live) store8(to, x);
+  };
+  for (int hb = h0; hb < h1; hb += kAtOnce * kAhead<T>) {
+    if (!fetched) fetch_rows<T, G>(src, src_head, hb, h1, d, raw);
+    fetched = false;
+    if (!ready) {  // behind the first rows' loads
+      ready = true;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        } else if constexpr (kTurn == kLanes) {
-          const int partner = (c * 8 < half ? c + half / 8 : c - half / 8) & (G - 1);
+      for (int i = 0; i < 8; ++i) own[i] = 1.f, other[i] = 0.f;
+      if (gamma && column) load8(gamma + c * 8, own);
+      if (kTurn != kNone && column && c * 8 < 2 * half) {
+        const float* cs = rot.cos + pos * rot.table_stride;
+        const float* sn = rot.sin + pos * rot.table_stride;
+        if constexpr (kTurn == kLanes) {
+          float co[8], si[8], g[8];
+          const int first = c * 8 < half ? c * 8 : c * 8 - half;
+          const bool vector = rot.table_stride % 4 == 0 && aligned16(rot.cos) && aligned16(rot.sin);
+          table8(cs + first, vector, co);
+          table8(sn + first, vector, si);
+          in = 0xff;
+          if (gamma) load8(gamma + partner * 8, g);
+          else
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], (lane - c) + partner);
+            for (int i = 0; i < 8; ++i) g[i] = 1.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) other[i] = (c * 8 < half ? -si[i] : si[i]) * g[i];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) own[i] *= co[i];
         } else {
-          __syncwarp();
-          store8(stage + lane * 8, x);
-          __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int col = c * 8 + i;
-            y[i] = lt.in >> i & 1 ? stage[(lane - c) * 8 + (col < half ? col + half : col - half)]
-                                  : 0.f;
+            const bool second = kTurn == kWithin ? i & 1 : col >= half;
+            const int pair = kTurn == kWithin ? col >> 1 : second ? col - half : col;
+            const int to = kTurn == kWithin ? col ^ 1 : second ? col - half : col + half;
+            if (col < 2 * half) {
+              in |= 1u << i;
+              own[i] *= cs[pair];
+              other[i] = (second ? sn[pair] : -sn[pair]) * (gamma ? gamma[to] : 1.f);
+            }
           }
         }
-        if constexpr (kTurn == kLanes) {  // a lane's columns are rotated all or none
-          if (lt.in)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * lt.c[i] + y[i] * lt.s[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (lt.in >> i & 1) x[i] = x[i] * lt.c[i] + y[i] * lt.s[i];
-        }
       }
-      if (column && hb + u * kAtOnce + sub < h1) store8(dst, x);
-      dst += dst_step;
+    }
+    if (hb + kAtOnce * kAhead<T> <= h1) {  // all live: their chains run side by side
+#pragma unroll
+      for (int u = 0; u < kAhead<T>; ++u, dst += dst_step) row(raw[u], dst, column);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAhead<T>; ++u, dst += dst_step)
+        if (hb + u * kAtOnce < h1)  // the same for the whole warp
+          row(raw[u], dst, column && hb + u * kAtOnce + sub < h1);
     }
   }
 }
 
 // One warp per (token, block of `per_warp` heads), the heads numbered queries,
-// keys, values. The cosines and sines of the token's position stay in
-// registers for all its heads: read for each head again they were twice the
-// bytes of a 16-bit row (8190 tokens of 40 bf16 heads of 128: 110 us; so
+// keys, values. What a token's position and the gammas give stays in registers
+// for all its heads: read for each head again, the cosines and sines were twice
+// the bytes of a 16-bit row (8190 tokens of 40 bf16 heads of 128: 110 us; so
 // XX us, XX of measured HBM).
 template <typename T, int G, int kTurn>
-__global__ void __launch_bounds__(256, 2) rows_kernel(const __grid_constant__ RowArgs r, int per_warp,
-                                                   int head_blocks, int64_t warps) {
-  __shared__ __align__(16) float stage[8][32 * 8];
+__global__ void __launch_bounds__(256, 3)
+    rows_kernel(const __grid_constant__ RowArgs r, int per_warp, int head_blocks, int64_t warps) {
+  __shared__ __align__(16) float stage[kTurn == kAcross ? 8 : 1][32 * 8];
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (w >= warps) return;
-  const int lane = threadIdx.x & 31, c = lane % G;
-  const int64_t t = w / head_blocks;
+  const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
+  const int64_t t = divide(w, head_blocks);
   const int first = (int)(w - t * head_blocks) * per_warp;
   const int total = r.q.heads + r.k.heads + r.v.heads;
   const int last = min(first + per_warp, total);
-  int64_t pos = t, b = t;
   const bool paged = r.a.kv.batch > 0;
   const InfercPagedKv& kv = r.a.kv;
+  // The first rows are on their way while the token's place is looked up.
+  Raw8<T> raw[kAhead<T>];
+  const int begin_kind = first < r.q.heads ? 0 : 1;
+  {
+    const Heads& s = begin_kind ? r.k : r.q;
+    const int before = begin_kind ? r.q.heads : 0;
+    fetch_rows<T, G>(reinterpret_cast<const T*>(s.src) + t * s.src_token, s.src_head,
+                     first - before, min(last - before, s.heads), r.d, raw);
+  }
+  int64_t pos = t, b = t;
   int page = 0;
   uint32_t slot = 0;
+  if (r.rot.positions) pos = r.rot.positions[t];
   if (paged) {
     int64_t begin = t, count = 1;
     if (r.cu) {
-      if (t >= r.cu[kv.batch]) return;  // behind the last sequence
-      b = find_seq(r.cu, kv.batch, t, lane);
-      if (b < 0) { *r.a.flag = 1; return; }
-      begin = r.cu[b];
-      count = r.cu[b + 1] - begin;
+      const Owner o = owner_of_token(r.cu, kv.batch, t, lane);
+      if (o.b == -1) return;  // behind the last sequence
+      if (o.b < 0) { *r.a.flag = 1; return; }
+      b = o.b;
+      begin = o.begin;
+      count = o.count;
     }
-    const int64_t len = kv.lens[b];
-    pos = len - count + (t - begin);
-    if (pos < 0 || pos >= len || len > kv.max_pages * kv.page_size) {
+    const int64_t len = kv.lens[b], at = len - count + (t - begin);
+    if (at < 0 || at >= len || len > kv.max_pages * kv.page_size) {
       *r.a.flag = 1;
       return;
     }
-    const uint32_t index = r.a.page.div((uint32_t)pos);
-    slot = (uint32_t)pos - index * r.a.page.d;
+    const uint32_t index = r.a.page.div((uint32_t)at);
+    slot = (uint32_t)at - index * r.a.page.d;
     page = page_of(r.a, kv.page_table + b * kv.table_stride, index);
     if (page < 0) return;
+    if (!r.rot.positions) pos = at;
   }
-  if (r.rot.positions) pos = r.rot.positions[t];
   if (kTurn != kNone && (pos < 0 || pos >= r.rot.table_len)) { *r.a.flag = 1; return; }
 
-  const int half = r.rot.rotary_dim / 2;
-  LaneTurn lt;
-  lt.in = 0;
-  if (kTurn != kNone && first < r.q.heads + r.k.heads) {
-    const float* cs = r.rot.cos + pos * r.rot.table_stride;
-    const float* sn = r.rot.sin + pos * r.rot.table_stride;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int col = c * 8 + i;
-      const bool second = kTurn == kWithin ? i & 1 : col >= half;
-      const int pair = kTurn == kWithin ? col >> 1 : second ? col - half : col;
-      lt.c[i] = lt.s[i] = 0.f;
-      if (col < 2 * half) {
-        lt.in |= 1u << i;
-        lt.c[i] = cs[pair];
-        lt.s[i] = second ? sn[pair] : -sn[pair];
-      }
+#pragma unroll 1
+  for (int kind = begin_kind; kind < 2; ++kind) {
+    const Heads& s = kind ? r.k : r.q;
+    const int before = kind ? r.q.heads : 0;
+    const int h0 = max(first - before, 0), h1 = min(last - before, s.heads);
+    if (h0 >= h1) continue;
+    T* dst = reinterpret_cast<T*>(s.dst) + t * s.dst_token;
+    int64_t dst_head = s.dst_head;
+    if (paged && kind) {
+      dst = reinterpret_cast<T*>(kv.k) + page * kv.k_page_stride +
+            (int64_t)slot * kv.k_token_stride;
+      dst_head = kv.k_head_stride;
     }
+    rows_of<T, G, kTurn>(reinterpret_cast<const T*>(s.src) + t * s.src_token, s.src_head, dst,
+                         dst_head, h0, h1, kind ? r.rot.k_gamma : r.rot.q_gamma, r.rot, pos, r.d,
+                         stage[kTurn == kAcross ? threadIdx.x >> 5 : 0], raw, kind == begin_kind);
   }
-  float* st = stage[threadIdx.x >> 5];
-  {
-    const int h0 = first, h1 = min(last, r.q.heads);
-    if (h0 < h1)
-      rows_of<T, G, kTurn>(reinterpret_cast<const T*>(r.q.src) + t * r.q.src_token, r.q.src_head,
-                    reinterpret_cast<T*>(r.q.dst) + t * r.q.dst_token, r.q.dst_head, h0, h1,
-                    r.rot.q_gamma, r.rot.eps, r.d, lt, half, st);
-  }
-  {
-    const int h0 = max(first - r.q.heads, 0), h1 = min(last - r.q.heads, r.k.heads);
-    if (h0 < h1) {
-      T* dst = reinterpret_cast<T*>(r.k.dst) + t * r.k.dst_token;
-      if (paged)
-        dst = reinterpret_cast<T*>(kv.k) + page * kv.k_page_stride +
-              (int64_t)slot * kv.k_token_stride;
-      rows_of<T, G, kTurn>(reinterpret_cast<const T*>(r.k.src) + t * r.k.src_token, r.k.src_head, dst,
-                    paged ? kv.k_head_stride : r.k.dst_head, h0, h1, r.rot.k_gamma, r.rot.eps, r.d,
-                           lt, half, st);
+  // values: as they are
+  const int before = r.q.heads + r.k.heads;
+  const T* src = reinterpret_cast<const T*>(r.v.src) + t * r.v.src_token + c * 8;
+  T* dst = reinterpret_cast<T*>(kv.v) + page * kv.v_page_stride +
+           (int64_t)slot * kv.v_token_stride + c * 8;
+  if (c * 8 < r.d)
+#pragma unroll 4
+    for (int h = max(first - before, 0) + sub; h < min(last - before, r.v.heads); h += 32 / G) {
+      Raw8<T> raw;
+      raw.load(src + h * r.v.src_head);
+      raw.store(dst + h * kv.v_head_stride);
     }
-  }
-  {
-    const int before = r.q.heads + r.k.heads;
-    const int h0 = max(first - before, 0), h1 = min(last - before, r.v.heads);
-    if (h0 < h1)
-      rows_of<T, G, kNone>(reinterpret_cast<const T*>(r.v.src) + t * r.v.src_token, r.v.src_head,
-                    reinterpret_cast<T*>(kv.v) + page * kv.v_page_stride +
-                        (int64_t)slot * kv.v_token_stride,
-                    kv.v_head_stride, h0, h1, nullptr, 0.f, r.d, lt, half, st);
-  }
 }
+
+#ifndef SPREAD
+#define SPREAD 1
+#endif
+constexpr int kSpread = SPREAD;
 
 template <typename T, int G>
 void launch_rows_of(const RowArgs& r, cudaStream_t st) {
   const int heads = r.q.heads + r.k.heads + r.v.heads;
-  // All heads of a token in one warp when there are tokens for every warp the
-  // SMs hold (16 each); else as few as keep them all busy, so that a decode
-  // step's few tokens do not wait for one another.
+  // Heads of a token per warp: what spreads the rows over four times the warps
+  // that the SMs hold (24 each), so that the last ones leave no SM idle for
+  // long and a decode step's few tokens do not wait for one another.
   const int unit = 32 / G;  // heads that a warp takes at once
-  int per_warp = (int)((r.tokens * heads + 148 * 16 - 1) / (148 * 16));
+  const int64_t spread = (int64_t)148 * 24 * kSpread;
+  int per_warp = (int)((r.tokens * heads + spread - 1) / spread);
   per_warp = std::min((per_warp + unit - 1) / unit * unit, (heads + unit - 1) / unit * unit);
   const int blocks = (heads + per_warp - 1) / per_warp;
   const int64_t warps = r.tokens * blocks;
@@ -383,6 +453,7 @@ constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kDeep = 4;              // 16-byte loads a lane has in flight, of K and of V
 constexpr int kKeysHeld = 16 * 1024;  // weights a block keeps in shared memory
+constexpr int kChooseAlone = 8 * 1024;  // positions up to which every block chooses by itself
 
 // Order of weights as unsigned numbers: -0 equals 0, every NaN is the largest.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -418,9 +489,11 @@ __device__ __forceinline__ uint64_t block_exclusive(uint64_t v, uint64_t* warp_s
 // One cluster per (sequence, key head).
 //
 // Choice: the weight of rank keep - recent by histograms of 11, 11 and 10 bits
-// of its key (each block counts its slice of the positions, the blocks add up
-// each other's counts through distributed shared memory), ending early when a
-// bin stays whole. A position's new place is the number of larger weights
+// of its key, ending early when a bin stays whole. Up to kChooseAlone positions
+// every block of the cluster counts all of them, which costs less than the
+// cluster barriers it saves (1024 positions: XX against 14 us); beyond, each
+// counts its slice and the blocks add up each other's counts through
+// distributed shared memory. A position's new place is the number of larger weights
 // before it plus the equal ones before it that stay, so ties go to the lowest
 // position whatever the threads' order.
 //
@@ -452,18 +525,33 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
   float* wo = e.w_out + b * e.wo_batch + h * e.wo_head;
   int32_t* kept = e.kept + job * e.keep;
   const int all_threads = blocks * kEvictThreads, all_tid = rank * kEvictThreads + tid;
+  // rows per warp and step of the move, and whether this block moves row r
+  constexpr int kAtOnce = 32 / kLanes, kRows = kDeep / kTurns * kAtOnce;
+  constexpr int kBlockRows = kEvictWarps * kRows;
+  const bool alone = kv.max_pages * kv.page_size <= kChooseAlone;
+  const int slices = alone ? 1 : blocks, at_slice = alone ? 0 : rank;
+  auto sync = [&]() {
+    if (alone) __syncthreads();
+    else cluster.sync();
+  };
+  auto keep_row = [&](int r, int from) {
+    if (!alone || (r / kBlockRows) % blocks == rank) kept[r] = from;
+  };
   if (h == 0 && all_tid == 0) e.lens_out[b] = m;
   for (int i = m + all_tid; i < e.keep; i += all_threads) kept[i] = -1;
 
   // ---- choice
   if (n <= e.keep) {
-    for (int i = all_tid; i < n; i += all_threads) kept[i] = i;
+    if (alone)
+      for (int i = tid; i < n; i += kEvictThreads) keep_row(i, i);
+    else
+      for (int i = all_tid; i < n; i += all_threads) kept[i] = i;
     if (kInPlace && !e.dst_table && wo == w) return;  // the whole cluster
   } else {
     const int limit = n - e.recent, need = e.keep - e.recent;
     // slices are multiples of 4 so that a thread's four positions are in one
-    const int slice = ((n + blocks - 1) / blocks + 3) & ~3;
-    const int s0 = min(rank * slice, n), s1 = min(s0 + slice, n);
+    const int slice = ((n + slices - 1) / slices + 3) & ~3;
+    const int s0 = min(at_slice * slice, n), s1 = min(s0 + slice, n);
     const int c1 = min(s1, limit);  // candidates: [s0, c1)
     const bool held = slice <= keys_held;
     auto key_at = [&](int j) { return held ? keys[j - s0] : weight_key(w[j]); };
@@ -480,15 +568,18 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
           const uint32_t k = key_at(j);
           if ((k & mask) == prefix) atomicAdd(&hist[pass][(k >> shift) & width], 1u);
         }
-        cluster.sync();
+        sync();
         // bins from the largest down, four a thread
         const int low = kBins - 4 - 4 * tid;
         uint4 c = make_uint4(0, 0, 0, 0);
-        for (int r = 0; r < blocks; ++r) {
-          const uint4 x = *reinterpret_cast<const uint4*>(
-              cluster.map_shared_rank(&hist[pass][low], r));
-          c.x += x.x; c.y += x.y; c.z += x.z; c.w += x.w;
-        }
+        if (alone)
+          c = *reinterpret_cast<const uint4*>(&hist[pass][low]);
+        else
+          for (int r = 0; r < blocks; ++r) {
+            const uint4 x = *reinterpret_cast<const uint4*>(
+                cluster.map_shared_rank(&hist[pass][low], r));
+            c.x += x.x; c.y += x.y; c.z += x.z; c.w += x.w;
+          }
         uint64_t total;
         const uint32_t before =
             (uint32_t)block_exclusive((uint64_t)c.x + c.y + c.z + c.w, sums, &total);
@@ -511,18 +602,19 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
       }
     }
     // (k & mask) > prefix stays, and of those equal to it the first `left`
-    uint64_t mine = 0;
-    if (need > 0)
-      for (int j = s0 + tid; j < c1; j += kEvictThreads) {
-        const uint32_t k = key_at(j) & mask;
-        mine += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
-      }
-    uint64_t total;
-    block_exclusive(mine, sums, &total);
-    if (tid == 0) s_count = total;
-    cluster.sync();
-    uint64_t done = 0;  // in the slices before this one, then in what is done of it
-    for (int r = 0; r < rank; ++r) done += *cluster.map_shared_rank(&s_count, r);
+    uint64_t total, done = 0;  // larger and equal ones before; done: in what is walked already
+    if (!alone) {
+      uint64_t mine = 0;
+      if (need > 0)
+        for (int j = s0 + tid; j < c1; j += kEvictThreads) {
+          const uint32_t k = key_at(j) & mask;
+          mine += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
+        }
+      block_exclusive(mine, sums, &total);
+      if (tid == 0) s_count = total;
+      cluster.sync();
+      for (int r = 0; r < rank; ++r) done += *cluster.map_shared_rank(&s_count, r);
+    }
     for (int j0 = s0; j0 < c1; j0 += kEvictThreads * 4) {
       const int j = j0 + tid * 4;
       uint32_t stays = 0;  // bits 0..3 larger, 4..7 equal
@@ -541,34 +633,33 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
         const uint32_t larger = stays >> i & 1, equal = stays >> (4 + i) & 1;
         const uint32_t eq_before = (uint32_t)at, gt_before = (uint32_t)(at >> 32);
         const uint32_t to = gt_before + min(eq_before, left);
-        if ((larger || (equal && eq_before < left)) && to < (uint32_t)need) kept[to] = j + i;
+        if ((larger || (equal && eq_before < left)) && to < (uint32_t)need) keep_row(to, j + i);
         at += ((uint64_t)larger << 32) | equal;
       }
       done += total;
     }
-    for (int j = max(s0, limit) + tid; j < s1; j += kEvictThreads) kept[need + j - limit] = j;
+    for (int j = max(s0, limit) + tid; j < s1; j += kEvictThreads) keep_row(need + j - limit, j);
   }
-  cluster.sync();  // `kept` is whole (and no block leaves while another reads its counts)
+  sync();  // `kept` is whole (and no block leaves while another reads its counts)
 
   // ---- move
-  constexpr int kAtOnce = 32 / kLanes, kRows = kDeep / kTurns * kAtOnce;  // rows per warp and step
   const int es = kv.dtype == F32 ? 4 : 2;
   const int pieces = kv.head_dim * es / 16;
   const int32_t* src_row = kv.page_table + b * kv.table_stride;
   const int32_t* dst_row = e.dst_table ? e.dst_table + b * e.dst_stride : src_row;
   const char* k_head = static_cast<const char*>(kv.k) + h * kv.k_head_stride * es;
   const char* v_head = static_cast<const char*>(kv.v) + h * kv.v_head_stride * es;
-  const int step = blocks * kEvictWarps * kRows;
-  for (int base = 0; base < m; base += step) {
-    const int row = base + (rank * kEvictWarps + warp) * kRows + lane;
-    const bool mine = lane < kRows && row < m;
+  // A warp's 32 lanes look up the rows of 32 / kRows steps at once, so that the chain of kept
+  // position, page and address is waited for once in as many steps.
+  const int step = blocks * kBlockRows;
+  for (int base = 0; base < m; base += 32 / kRows * step) {
+    const int row = base + lane / kRows * step + rank * kBlockRows + warp * kRows + lane % kRows;
     bool ok = false;
     int64_t sk = 0, sv = 0, dk = 0, dv = 0;
-    float weight = 0.f;
-    if (mine) {
+    uint32_t from = 0;
+    if (row < m) {
       // (below n unless the weights change under the kernel)
-      const uint32_t from = min((uint32_t)kept[row], (uint32_t)(n - 1));
-      weight = w[from];
+      from = min((uint32_t)kept[row], (uint32_t)(n - 1));
       if (e.dst_table || from != (uint32_t)row) {
         const uint32_t sp = e.a.page.div(from), dp = e.a.page.div(row);
         const int src = page_of(e.a, src_row, sp), dst = page_of(e.a, dst_row, dp);
@@ -582,36 +673,41 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
         }
       }
     }
-    uint4 k_val[kDeep], v_val[kDeep];
-    auto row_at = [&](int u) { return u / kTurns * kAtOnce + lane / kLanes; };
-    auto piece_at = [&](int u) { return lane % kLanes + u % kTurns * 32; };
+    for (int s = 0; s < 32 / kRows && base + s * step < m; ++s) {
+      uint4 k_val[kDeep], v_val[kDeep];
+      auto row_at = [&](int u) { return s * kRows + u / kTurns * kAtOnce + lane / kLanes; };
+      auto piece_at = [&](int u) { return lane % kLanes + u % kTurns * 32; };
 #pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-      const int r = row_at(u), piece = piece_at(u);
-      const int64_t from_k = __shfl_sync(0xffffffffu, sk, r);
-      const int64_t from_v = __shfl_sync(0xffffffffu, sv, r);
-      const bool live = __shfl_sync(0xffffffffu, (int)ok, r) && piece < pieces;
-      if (live) {
-        k_val[u] = *reinterpret_cast<const uint4*>(k_head + from_k + piece * 16);
-        v_val[u] = *reinterpret_cast<const uint4*>(v_head + from_v + piece * 16);
+      for (int u = 0; u < kDeep; ++u) {
+        const int r = row_at(u), piece = piece_at(u);
+        const int64_t from_k = __shfl_sync(0xffffffffu, sk, r);
+        const int64_t from_v = __shfl_sync(0xffffffffu, sv, r);
+        const bool live = __shfl_sync(0xffffffffu, (int)ok, r) && piece < pieces;
+        if (live) {
+          k_val[u] = *reinterpret_cast<const uint4*>(k_head + from_k + piece * 16);
+          v_val[u] = *reinterpret_cast<const uint4*>(v_head + from_v + piece * 16);
+        }
       }
-    }
-    if (kInPlace) {
-      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    }
+      const bool weighs = lane / kRows == s && row < m;
+      float weight = 0.f;
+      if (weighs) weight = w[from];
+      if (kInPlace) {
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      }
 #pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-      const int r = row_at(u), piece = piece_at(u);
-      const int64_t to_k = __shfl_sync(0xffffffffu, dk, r);
-      const int64_t to_v = __shfl_sync(0xffffffffu, dv, r);
-      const bool live = __shfl_sync(0xffffffffu, (int)ok, r) && piece < pieces;
-      if (live) {
-        *reinterpret_cast<uint4*>(const_cast<char*>(k_head) + to_k + piece * 16) = k_val[u];
-        *reinterpret_cast<uint4*>(const_cast<char*>(v_head) + to_v + piece * 16) = v_val[u];
+      for (int u = 0; u < kDeep; ++u) {
+        const int r = row_at(u), piece = piece_at(u);
+        const int64_t to_k = __shfl_sync(0xffffffffu, dk, r);
+        const int64_t to_v = __shfl_sync(0xffffffffu, dv, r);
+        const bool live = __shfl_sync(0xffffffffu, (int)ok, r) && piece < pieces;
+        if (live) {
+          *reinterpret_cast<uint4*>(const_cast<char*>(k_head) + to_k + piece * 16) = k_val[u];
+          *reinterpret_cast<uint4*>(const_cast<char*>(v_head) + to_v + piece * 16) = v_val[u];
+        }
       }
+      if (weighs) wo[row] = weight;
     }
-    if (mine) wo[row] = weight;
   }
   // every load of w is done: in place, before the last step's barrier
   for (int j = m + all_tid; j < n; j += all_threads) wo[j] = 0.f;
@@ -626,7 +722,8 @@ void launch_evict(const EvictArgs& e, cudaStream_t st) {
   int blocks = 1;
   while (blocks < kMoveCluster && jobs * blocks < 2 * 148 && capacity > blocks * kEvictThreads)
     blocks *= 2;
-  const int64_t slice = ((capacity + blocks - 1) / blocks + 3) / 4 * 4;
+  const int slices = capacity <= kChooseAlone ? 1 : blocks;
+  const int64_t slice = ((capacity + slices - 1) / slices + 3) / 4 * 4;
   const int held = (int)std::min<int64_t>(slice, kKeysHeld);
   const int pieces = kv.head_dim * elem_bytes(kv.dtype) / 16;
   const bool in_place = !e.dst_table || e.w_out == e.w;
