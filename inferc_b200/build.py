@@ -1,9 +1,11 @@
-"""Builds libinferc_b200.so in-tree with nvcc for sm_100a (B200 only).
+"""Builds libinferc_b200.so in-tree with nvcc for sm_100a (B200 only), and the
+torch binding of the paged-cache operators (csrc/torch_paged.cpp) against it.
 
     python -m inferc_b200.build [--force]
 
-Objects go to inferc_b200/_build/ and the shared library to
-inferc_b200/libinferc_b200.so; both are git-ignored build products.
+Objects go to inferc_b200/_build/, the shared library to
+inferc_b200/libinferc_b200.so and the binding to inferc_b200/_paged.so; all are
+git-ignored build products.
 """
 from __future__ import annotations
 
@@ -18,6 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libinferc_b200.so")
+BINDING = os.path.join(HERE, "_paged.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
@@ -48,13 +51,35 @@ def _compile(src: str, force: bool, verbose_ptxas: bool) -> str:
     return obj
 
 
+def _build_binding(force: bool) -> None:
+    src = os.path.join(CSRC, "torch_paged.cpp")
+    if not (force or _stale(BINDING, [src, LIB] + _deps())):
+        return
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api",
+                                                       "include"),
+           sysconfig.get_paths()["include"],
+           os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    subprocess.run(
+        ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
+         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+         *[f"-I{i}" for i in inc], src, "-o", BINDING, LIB, f"-L{os.path.join(root, 'lib')}",
+         "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
+         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{os.path.join(root, 'lib')}"], check=True)
+
+
 def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cc")))
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(lambda s: _compile(s, force, verbose_ptxas), sources))
     if force or _stale(LIB, objs):
-        subprocess.run([NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart"], check=True)
+        subprocess.run([NVCC, *ARCH, "-shared", "-o", LIB, "-Xlinker",
+                        "-soname=libinferc_b200.so", *objs, "-lcudart"], check=True)
+    _build_binding(force)
     return LIB
 
 
