@@ -1,6 +1,6 @@
 // Attention of one new token per sequence over the paged cache: entry points,
-// the join of sequences that several warps read, and the running sums of
-// attention weights. paged_attention.cuh reads the cache.
+// and what follows the reading of the cache: the join of sequences that several
+// warps read and the running sums of attention weights. paged_attention.cuh reads the cache.
 #include <algorithm>
 #include <string>
 
@@ -11,7 +11,8 @@ namespace paged {
 namespace {
 
 constexpr int kSMs = 148;  // B200; elsewhere the grid runs in waves
-constexpr int kJoinMost = 512;  // threads of a join block: this many, or a quarter where there are jobs for every SM
+constexpr int kWholeTiles = 16;
+constexpr int kJoinMost = 512;  // threads of a block of finish_kernel, or a quarter of them
 
 // The parts of one (sequence, head block): warp `first`'s second slot, then
 // the first slots of the warps behind it.
@@ -23,46 +24,47 @@ struct Parts {
   }
 };
 
+// Where a (sequence, head block)'s parts are.
+__device__ __forceinline__ Parts parts_of(const AttendArgs& g, int64_t t0, int64_t tiles,
+                                          int64_t total, int64_t used) {
+  Parts p;
+  p.first = owner_of(t0, total, used);
+  p.count = (int)(owner_of(t0 + tiles - 1, total, used) - p.first) + 1;
+  return p;
+}
+
 // Joins what several warps left of a (sequence, head block):
 //   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-// One block per cut head block (or per share of its heads, grid.y). Its jobs
-// are found by (sequence, head block) where those are fewer than the warps,
-// else by the warp that left the first part. Bound by latency: each thread
-// takes four columns of a head and every `shares`-th part, fetches four parts'
-// columns, maxima and sums at once, and the shares meet in shared memory.
+// One block per cut head block (or per share `part` of `of` of its heads). Its
+// jobs are found by (sequence, head block) where those are fewer than the
+// warps, else by the warp that left the first part. Bound by latency: each
+// thread takes four columns of a head and every `shares`-th part, fetches four
+// parts' columns, maxima and sums at once, and the shares meet in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kJoinMost, 2) join_kernel(const __grid_constant__ AttendArgs g,
-                                                            bool by_warp) {
-  __shared__ float4 s_o[kJoinMost];
-  __shared__ float2 s_ml[kJoinMost];
+__device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp, int part, int of,
+                                     float4* s_o, float2* s_ml) {
   constexpr int kAtOnce = 4;
   const InfercPagedKv& kv = g.a.kv;
   const int tid = threadIdx.x, threads = blockDim.x;
   const int heads = (int)kv.kv_heads * g.blocks, d = kv.head_dim;
-  pdl_launch_dependents();
-  pdl_wait();
   const int64_t total = g.before[kv.batch];
   if (total == 0) return;
-  int64_t b = blockIdx.x / heads;
-  int head = blockIdx.x % heads;
+  int64_t b = job / heads;
+  int head = job % heads;
   if (by_warp) {
-    b = g.jobs[2 * (int64_t)blockIdx.x];
-    head = g.jobs[2 * (int64_t)blockIdx.x + 1];
+    b = g.jobs[2 * job];
+    head = g.jobs[2 * job + 1];
     if (b < 0) return;
   }
-  const int64_t begin = g.before[b], tiles = (g.before[b + 1] - begin) / heads;
+  const int64_t begin = g.before[b], tiles = divide(g.before[b + 1] - begin, heads);
   if (tiles == 0) return;
   const int64_t used = warps_used(total, g.warps);
-  const int64_t t0 = begin + head * tiles;
-  Parts parts;
-  parts.first = owner_of(t0, total, used);
-  parts.count = (int)(owner_of(t0 + tiles - 1, total, used) - parts.first) + 1;
+  const Parts parts = parts_of(g, begin + head * tiles, tiles, total, used);
   if (parts.count == 1) return;
 
   const int hk = head / g.blocks, q0 = hk * g.group + (head % g.blocks) * g.block;
   const int cols = min(g.block, hk * g.group + g.group - q0);
-  const int h0 = cols * (int)blockIdx.y / (int)gridDim.y;
-  const int h1 = cols * ((int)blockIdx.y + 1) / (int)gridDim.y;
+  const int h0 = cols * part / of, h1 = cols * (part + 1) / of;
   const int quads = d / 4, items = (h1 - h0) * quads;  // float4s of the result
   for (int base = 0; base < items; base += threads) {
     const int n = min(items - base, threads);
@@ -131,11 +133,6 @@ __global__ void __launch_bounds__(kJoinMost, 2) join_kernel(const __grid_constan
       out[1] = T(o.y * inv);
       out[2] = T(o.z * inv);
       out[3] = T(o.w * inv);
-      if (g.stats && quad == 0) {
-        const int64_t r = b * (int64_t)(kv.kv_heads * g.group) + q0 + h;
-        g.stats[2 * r] = to;
-        g.stats[2 * r + 1] = inv;
-      }
     }
     __syncthreads();
   }
@@ -143,66 +140,130 @@ __global__ void __launch_bounds__(kJoinMost, 2) join_kernel(const __grid_constan
 
 // Adds each position's softmax weight, 2^(s - M) / L summed over the query
 // heads of its key head in their order, to the running sum. The positions are
-// cut among the warps like the tiles.
-constexpr int kSumThreads = 256;
-
-__global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant__ AttendArgs g,
-                                                           int64_t warps) {
+// cut among the warps like the tiles. A head's M and L come from its parts where
+// it was cut (each lane takes some of them), else from what its warp left.
+__device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int64_t warps,
+                                            float2* stats) {
   const InfercPagedKv& kv = g.a.kv;
   const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * (kSumThreads / 32) + (threadIdx.x >> 5);
-  const int hk_n = (int)kv.kv_heads;
+  const int hk_n = (int)kv.kv_heads, heads = hk_n * g.blocks;
   const int64_t q_heads = kv.kv_heads * g.group;
-  pdl_wait();
+  // The sequence that holds the first tile, 32 probes a step; the first step's loads do not
+  // wait for the total.
+  int64_t b = 0, size = kv.batch;
+  int64_t step = (size + 31) / 32;
+  int64_t probe = lane * step < size ? g.before[lane * step] : INT64_MAX;
+  const int64_t cut_total = g.before[kv.batch];
   // tiles of one head per key head, not per block of query heads
-  const int64_t total = g.before[kv.batch] / g.blocks;
+  const int64_t total = divide(cut_total, g.blocks);
   if (total == 0) return;
   const int64_t used = warps_used(total, warps);
   if (w >= used) return;
   const int64_t t0 = first_tile(w, total, used), t1 = first_tile(w + 1, total, used);
-  // the sequence that holds t0: 32 probes a step
-  int64_t b = 0, size = kv.batch;
-  while (size > 1) {
-    const int64_t step = (size + 31) / 32;
-    const bool below = lane * step < size && g.before[b + lane * step] / g.blocks <= t0;
-    const int n = __popc(__ballot_sync(0xffffffffu, below));
+  for (;;) {
+    const int n = __popc(__ballot_sync(0xffffffffu, probe <= t0 * g.blocks));
     b += (n - 1) * step;
     size = min(step, size - (n - 1) * step);
+    if (size <= 1) break;
+    step = (size + 31) / 32;
+    probe = lane * step < size ? g.before[b + lane * step] : INT64_MAX;
   }
+  const bool vec = aligned16(g.w) && g.w_batch % 4 == 0 && g.w_head % 4 == 0;
+  const int64_t cut_used = warps_used(cut_total, g.warps);
   int64_t t = t0;
   while (t < t1) {
-    const int64_t first = g.before[b] / g.blocks, after = g.before[b + 1] / g.blocks;
+    const int64_t first = g.before[b], after = g.before[b + 1];
     if (first == after) {
       ++b;
       continue;
     }
-    const int64_t tiles = (after - first) / hk_n;
-    const int h = (int)((t - first) / tiles);
-    const int64_t from = (t - first) - h * tiles;  // tiles of this head: [from, upto)
+    const int64_t tiles = divide(after - first, heads);
+    const int64_t at = t - divide(first, g.blocks);
+    const int h = (int)divide(at, tiles);
+    const int64_t from = at - h * tiles;  // tiles of this head: [from, upto)
     const int64_t upto = min(tiles, from + (t1 - t));
     const int n = min((int64_t)seq_len(g.a, b), upto * g.tile);
     const int64_t r = b * q_heads + (int64_t)h * g.group;
     const float* s = g.scores + r * g.capacity;
     float* sum = g.w + b * g.w_batch + h * g.w_head;
-    // four positions a lane; g.capacity and the tiles are multiples of 4
-    for (int j = (int)from * g.tile + lane * 4; j < n; j += 128) {
-      float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < g.group; i0 += g.block) {
+      const int cols = min(g.block, g.group - i0);
+      const int64_t head = (int64_t)h * g.blocks + i0 / g.block;
+      Parts parts{0, 1};
+      if (g.part_ml) parts = parts_of(g, first + head * tiles, tiles, cut_total, cut_used);
+      // lanes h and h + 16 take head h, every second part each
+      const int mine = lane & 15;
+      float2 st = make_float2(0.f, 0.f);
+      if (parts.count == 1) {
+        if (mine < cols) st = reinterpret_cast<const float2*>(g.stats)[r + i0 + mine];
+      } else {
+        float m = -INFINITY, l = 0.f;
+        if (mine < cols)
 #pragma unroll 4
-      for (int i = 0; i < g.group; ++i) {
-        const float2 st = reinterpret_cast<const float2*>(g.stats)[r + i];
-        const float4 x = *reinterpret_cast<const float4*>(s + i * g.capacity + j);
-        p.x += ex2(x.x - st.x) * st.y;
-        p.y += ex2(x.y - st.x) * st.y;
-        p.z += ex2(x.z - st.x) * st.y;
-        p.w += ex2(x.w - st.x) * st.y;
+          for (int p = lane >> 4; p < parts.count; p += 2) {
+            const float2 ml =
+                reinterpret_cast<const float2*>(g.part_ml)[parts.slot(p) * g.block + mine];
+            const float top = fmaxf(m, ml.x), to = top == -INFINITY ? 0.f : top;
+            l = l * ex2(m - to) + ml.y * ex2(ml.x - to);
+            m = top;
+          }
+        const float top = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        const float to = top == -INFINITY ? 0.f : top;
+        l *= ex2(m - to);
+        // both lanes add in the same order
+        const float other = __shfl_xor_sync(0xffffffffu, l, 16);
+        l = lane < 16 ? l + other : other + l;
+        st = make_float2(to, l == 0.f ? 0.f : 1.f / l);
       }
-      sum[j] += p.x;
-      if (j + 1 < n) sum[j + 1] += p.y;
-      if (j + 2 < n) sum[j + 2] += p.z;
-      if (j + 3 < n) sum[j + 3] += p.w;
+      __syncwarp();
+      if (lane < cols) stats[lane] = st;
+      __syncwarp();
+      // four positions a lane; g.capacity and the tiles are multiples of 4
+#pragma unroll 2
+      for (int j = (int)from * g.tile + lane * 4; j < n; j += 128) {
+        const bool four = vec && j + 4 <= n;
+        float4 p = make_float4(0.f, 0.f, 0.f, 0.f), old = p;
+        if (four) old = *reinterpret_cast<const float4*>(sum + j);
+#pragma unroll 4
+        for (int i = 0; i < cols; ++i) {
+          const float2 st = stats[i];
+          const float4 x = *reinterpret_cast<const float4*>(s + (i0 + i) * g.capacity + j);
+          p.x += ex2(x.x - st.x) * st.y;
+          p.y += ex2(x.y - st.x) * st.y;
+          p.z += ex2(x.z - st.x) * st.y;
+          p.w += ex2(x.w - st.x) * st.y;
+        }
+        if (four) {
+          *reinterpret_cast<float4*>(sum + j) =
+              make_float4(old.x + p.x, old.y + p.y, old.z + p.z, old.w + p.w);
+        } else {
+          sum[j] += p.x;
+          if (j + 1 < n) sum[j + 1] += p.y;
+          if (j + 2 < n) sum[j + 2] += p.z;
+          if (j + 3 < n) sum[j + 3] += p.w;
+        }
+      }
     }
     t += upto - from;
     if (upto == tiles && h + 1 == hk_n) ++b;
+  }
+}
+
+// Behind attend_kernel: the first jobs * of blocks join, the others add weights.
+template <typename T>
+__global__ void __launch_bounds__(kJoinMost, 2) finish_kernel(const __grid_constant__ AttendArgs g,
+                                                              int jobs, bool by_warp, int of,
+                                                              int64_t sum_warps) {
+  __shared__ float4 s_o[kJoinMost];
+  __shared__ float2 s_ml[kJoinMost];
+  pdl_launch_dependents();
+  pdl_wait();
+  if ((int)blockIdx.x < jobs * of) {
+    join<T>(g, blockIdx.x / of, by_warp, blockIdx.x % of, of, s_o, s_ml);
+  } else {
+    const int warp = threadIdx.x >> 5;
+    add_weights(g, (int64_t)(blockIdx.x - jobs * of) * (blockDim.x / 32) + warp, sum_warps,
+                s_ml + warp * 16);
   }
 }
 
@@ -235,20 +296,26 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
   const int64_t tiles = (g.capacity + g.tile - 1) / g.tile;
   const int64_t most = kv.batch * kv.kv_heads * g.blocks * tiles;
   g.warps = std::max<int64_t>(1, std::min<int64_t>((int64_t)kSMs * shape.blocks * kWarps, most));
-  p.cut = tiles > 1;
+  // Short sequences of few heads: a block each (see attend_kernel). At most one wave of blocks,
+  // whose warps take four tiles each at most; one request of 160 positions and 12 fp32 heads:
+  // XX us against 9.4 us.
+  const int64_t pairs = kv.batch * kv.kv_heads;
+  g.whole = g.blocks == 1 && tiles <= kWholeTiles && pairs <= kSMs * shape.blocks;
+  if (g.whole) g.warps = pairs * kWarps;
+  p.cut = tiles > 1 && !g.whole;
   auto take = [&](int64_t bytes) {
     char* at = ws + p.bytes;
     p.bytes += align16(bytes);
     return at;
   };
-  if (p.cut || weights) g.before = reinterpret_cast<int64_t*>(take((kv.batch + 1) * 8));
+  if (p.cut || (weights && !g.whole)) g.before = reinterpret_cast<int64_t*>(take((kv.batch + 1) * 8));
   if (p.cut) {
     g.jobs = reinterpret_cast<int32_t*>(take(g.warps * 8));
     g.part_ml = reinterpret_cast<float*>(take(2 * g.warps * g.block * 8));
     g.part_o = reinterpret_cast<float*>(take(2 * g.warps * g.block * kv.head_dim * 4));
   }
+  if (weights && !g.whole) g.stats = reinterpret_cast<float*>(take(kv.batch * q_heads * 8));
   if (weights) {
-    g.stats = reinterpret_cast<float*>(take(kv.batch * q_heads * 8));
     g.scores = reinterpret_cast<float*>(take(kv.batch * q_heads * g.capacity * 4));
   }
   return p;
@@ -266,21 +333,24 @@ void run(const Plan& p, cudaStream_t st) {
   const AttendArgs& g = p.g;
   const InfercPagedKv& kv = g.a.kv;
   launch_attend<T>(g, st);
+  if (g.whole || (!p.cut && !g.w)) return;
+  int64_t jobs = 0;
+  int of = 1;
+  bool by_warp = false;
   if (p.cut) {
     const int64_t pairs = kv.batch * kv.kv_heads * g.blocks;
-    const bool by_warp = pairs > g.warps;
-    const int64_t jobs = by_warp ? g.warps : pairs;
+    by_warp = pairs > g.warps;
+    jobs = by_warp ? g.warps : pairs;
     // few jobs: their heads go to blocks of their own
-    const int split = (int)std::min<int64_t>(g.block, std::max<int64_t>(1, 4 * kSMs / jobs));
-    launch_pdl(join_kernel<T>, dim3((unsigned)jobs, (unsigned)split),
-               dim3(jobs * split > kSMs ? kJoinMost / 4 : kJoinMost), 0, st, g,
-               by_warp);
+    of = (int)std::min<int64_t>(g.block, std::max<int64_t>(1, 4 * kSMs / jobs));
   }
-  if (g.w) {
-    const int64_t warps = (int64_t)kSMs * 64;
-    launch_pdl(sums_kernel, dim3((unsigned)(warps * 32 / kSumThreads)), dim3(kSumThreads), 0, st, g,
-               warps);
-  }
+  const int threads = jobs * of > kSMs || g.w ? kJoinMost / 4 : kJoinMost;
+  // sums: as many warps as the SMs hold, no more than there are tiles
+  const int64_t tiles = kv.batch * kv.kv_heads * ((g.capacity + g.tile - 1) / g.tile);
+  const int64_t sum_warps = g.w ? std::min<int64_t>((int64_t)kSMs * 32, tiles) : 0;
+  const int64_t grid = jobs * of + (sum_warps * 32 + threads - 1) / threads;
+  launch_pdl(finish_kernel<T>, dim3((unsigned)grid), dim3(threads), 0, st, g, (int)jobs, by_warp,
+             of, sum_warps);
 }
 
 }  // namespace

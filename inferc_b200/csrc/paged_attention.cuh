@@ -61,6 +61,7 @@ struct AttendArgs {
   int block;        // query heads per block (at most 16)
   int blocks;       // blocks per key head
   int tile;         // positions per tile
+  bool whole;       // one block of the grid reads one (sequence, key head), see attend_kernel
   int64_t warps;    // in the grid
   int64_t* before;  // [batch + 1] tiles before each sequence
   int32_t* jobs;    // [warps, 2] (sequence, head block) whose first part this warp left; -1
@@ -215,6 +216,70 @@ struct Cursor {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ void zero_heads(const AttendArgs& g, int64_t b, int h0, int h1) {
+  const int pieces = g.a.kv.head_dim / 8;
+  const float zero[8] = {};
+  for (int i = threadIdx.x; i < (h1 - h0) * pieces; i += blockDim.x)
+    store8(reinterpret_cast<T*>(g.out) + b * g.o_batch + (h0 + i / pieces) * g.o_head +
+               (i % pieces) * 8,
+           zero);
+}
+
+// What a whole block left in shared memory (one part per warp), joined: the
+// output of one (sequence, key head) and, where they are kept, its weights.
+template <typename T>
+__device__ __forceinline__ void join_whole(const AttendArgs& g, int b, int hk, int len,
+                                           const float2* ml, const float* o, int part) {
+  const InfercPagedKv& kv = g.a.kv;
+  const int d = kv.head_dim, quads = d / 4, cols = g.group;
+  for (int i = threadIdx.x; i < cols * quads; i += kWarps * 32) {
+    const int h = i / quads, quad = i - h * quads;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int p = 0; p < kWarps; ++p) m = fmaxf(m, ml[p * 16 + h].x);
+    const float to = m == -INFINITY ? 0.f : m;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < kWarps; ++p) {
+      const float2 x = ml[p * 16 + h];
+      if (x.y == 0.f) continue;  // a warp without tiles left nothing
+      const float f = ex2(x.x - to);
+      const float4 v = reinterpret_cast<const float4*>(o + p * part + h * d)[quad];
+      l += f * x.y;
+      sum.x += f * v.x;
+      sum.y += f * v.y;
+      sum.z += f * v.z;
+      sum.w += f * v.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: every page was bad
+    T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + (hk * g.group + h) * g.o_head + quad * 4;
+    out[0] = T(sum.x * inv);
+    out[1] = T(sum.y * inv);
+    out[2] = T(sum.z * inv);
+    out[3] = T(sum.w * inv);
+  }
+  if (!g.w) return;
+  const float* s = g.scores + (b * (int64_t)(kv.kv_heads * g.group) + hk * g.group) * g.capacity;
+  float* w = g.w + b * g.w_batch + hk * g.w_head;
+  for (int j = threadIdx.x; j < len; j += kWarps * 32) {
+    float sum = 0.f;
+    for (int h = 0; h < cols; ++h) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int p = 0; p < kWarps; ++p) m = fmaxf(m, ml[p * 16 + h].x);
+      const float to = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int p = 0; p < kWarps; ++p) {
+        const float2 x = ml[p * 16 + h];
+        l += x.y == 0.f ? 0.f : ex2(x.x - to) * x.y;
+      }
+      sum += ex2(s[h * g.capacity + j] - to) * (l == 0.f ? 0.f : 1.f / l);
+    }
+    w[j] += sum;
+  }
+}
+
 template <typename T, int kDim, int kCols, bool kTma>
 __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     attend_kernel(const __grid_constant__ AttendArgs g, const __grid_constant__ CUtensorMap k_map,
@@ -226,92 +291,15 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int64_t s_before[kThreads + 1];
+  __shared__ int64_t s_before[kThreads];
   __shared__ int64_t s_warp[kWarps];
+  __shared__ float2 s_ml[kWarps * 16];  // g.whole: each warp's maxima and sums
   const InfercPagedKv& kv = g.a.kv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gid = lane >> 2, tig = lane & 3;
   const int heads = (int)kv.kv_heads * g.blocks;
   const int batch = (int)kv.batch;
   const int d = kv.head_dim;
-  pdl_launch_dependents();
-  if constexpr (kTma)
-    if (tid == 0) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)));
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)));
-    }
-
-  // Tiles before each thread's run of sequences, and in all.
-  const int run = (batch + kThreads - 1) / kThreads;
-  const int run0 = min(tid * run, batch), run1 = min(run0 + run, batch);
-  int64_t mine = 0;
-  for (int b = run0; b < run1; ++b)
-    mine += (int64_t)((seq_len(g.a, b) + kTile - 1) / kTile) * heads;
-  int64_t scan = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += x;
-  }
-  if (lane == 31) s_warp[warp] = scan;
-  __syncthreads();
-  int64_t total = 0, ahead = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) ahead += s_warp[i];
-    total += s_warp[i];
-  }
-  s_before[tid] = ahead + scan - mine;
-  if (tid == 0) s_before[kThreads] = total;
-  if (blockIdx.x == 0 && g.before) {
-    int64_t at = ahead + scan - mine;
-    for (int b = run0; b < run1; ++b) {
-      g.before[b] = at;
-      at += (int64_t)((seq_len(g.a, b) + kTile - 1) / kTile) * heads;
-    }
-    if (tid == 0) g.before[batch] = total;
-  }
-  // A sequence of length 0 gives zeros.
-  for (int64_t b = blockIdx.x; b < batch; b += gridDim.x) {
-    if (seq_len(g.a, b) > 0) continue;
-    const int pieces = d / 8;
-    const int q_heads = (int)kv.kv_heads * g.group;
-    const float zero[8] = {};
-    for (int i = tid; i < q_heads * pieces; i += kThreads)
-      store8(reinterpret_cast<T*>(g.out) + b * g.o_batch + (int64_t)(i / pieces) * g.o_head +
-                 (i % pieces) * 8,
-             zero);
-  }
-  __syncthreads();
-
-  const int64_t w = (int64_t)blockIdx.x * kWarps + warp;
-  if (g.jobs && lane == 0 && w < g.warps) g.jobs[2 * w] = -1;
-  const int64_t used = warps_used(total, g.warps);
-  if (w >= used) return;
-  const int64_t t0 = first_tile(w, total, used);
-  const int count = (int)(first_tile(w + 1, total, used) - t0);
-
-  // The tile t0: the thread whose run holds it, then the sequence, then the head.
-  Cursor<kTile> load;
-  {
-    int lo = -1;  // runs that begin at t0 or before it, less one
-#pragma unroll
-    for (int i = 0; i < kThreads; i += 32)
-      lo += __popc(__ballot_sync(0xffffffffu, s_before[i + lane] <= t0));
-    int64_t left = t0 - s_before[lo];
-    load.open(g, min(lo * run, batch));
-    while (load.b < batch && left >= (int64_t)load.tiles * heads) {
-      left -= (int64_t)load.tiles * heads;
-      load.open(g, load.b + 1);
-    }
-    if (load.b >= batch) return;  // only if the lengths change under the kernel
-    const int head = (int)divide(left, load.tiles);
-    load.hk = head / g.blocks;
-    load.block = head - load.hk * g.blocks;
-    load.tile = (int)(left - (int64_t)head * load.tiles);
-  }
-  Cursor<kTile> use = load;
-
   unsigned char* ring = smem + warp * L::kSlots * L::kSlot;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * L::kSlots * L::kSlot) +
                    warp * L::kSlots;
@@ -329,6 +317,89 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
   }
   __syncwarp();
+  if constexpr (kTma)
+    if (tid == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)));
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)));
+    }
+
+  pdl_launch_dependents();
+  pdl_wait();  // lengths, tables, queries and caches may come from the kernel before
+
+  int64_t w = (int64_t)blockIdx.x * kWarps + warp;
+  int count = 0;
+  Cursor<kTile> load;
+  if (g.whole) {
+    // Short sequences, few heads: the block's four warps share one (sequence, key head) and
+    // join their parts in shared memory, which spares the search and a second kernel.
+    load.b = blockIdx.x / (int)kv.kv_heads;
+    load.hk = blockIdx.x - load.b * (int)kv.kv_heads;
+    load.block = 0;
+    load.len = seq_len(g.a, load.b);
+    load.tiles = (load.len + kTile - 1) / kTile;
+    load.tile = load.tiles * warp / kWarps;
+    count = load.tiles * (warp + 1) / kWarps - load.tile;
+  } else {
+    // Tiles before each thread's run of sequences, and in all.
+    const int run = (batch + kThreads - 1) / kThreads;
+    const int run0 = min(tid * run, batch), run1 = min(run0 + run, batch);
+    int64_t mine = 0;
+    for (int b = run0; b < run1; ++b)
+      mine += (int64_t)((seq_len(g.a, b) + kTile - 1) / kTile) * heads;
+    int64_t scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += x;
+    }
+    if (lane == 31) s_warp[warp] = scan;
+    __syncthreads();
+    int64_t total = 0, ahead = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) ahead += s_warp[i];
+      total += s_warp[i];
+    }
+    s_before[tid] = ahead + scan - mine;
+    if (blockIdx.x == 0 && g.before) {
+      int64_t at = ahead + scan - mine;
+      for (int b = run0; b < run1; ++b) {
+        g.before[b] = at;
+        at += (int64_t)((seq_len(g.a, b) + kTile - 1) / kTile) * heads;
+      }
+      if (tid == 0) g.before[batch] = total;
+    }
+    // A sequence of length 0 gives zeros.
+    for (int64_t b = blockIdx.x; b < batch; b += gridDim.x)
+      if (seq_len(g.a, b) == 0)
+        zero_heads<T>(g, b, 0, (int)kv.kv_heads * g.group);
+    __syncthreads();
+
+    if (g.jobs && lane == 0 && w < g.warps) g.jobs[2 * w] = -1;
+    const int64_t used = warps_used(total, g.warps);
+    if (w >= used) return;
+    const int64_t t0 = first_tile(w, total, used);
+    count = (int)(first_tile(w + 1, total, used) - t0);
+
+    // The tile t0: the thread whose run holds it, then the sequence, then the head.
+    int lo = -1;  // runs that begin at t0 or before it, less one
+#pragma unroll
+    for (int i = 0; i < kThreads; i += 32)
+      lo += __popc(__ballot_sync(0xffffffffu, s_before[i + lane] <= t0));
+    int64_t left = t0 - s_before[lo];
+    load.open(g, min(lo * run, batch));
+    while (load.b < batch && left >= (int64_t)load.tiles * heads) {
+      left -= (int64_t)load.tiles * heads;
+      load.open(g, load.b + 1);
+    }
+    if (load.b >= batch) return;  // only if the lengths change under the kernel
+    const int head = (int)divide(left, load.tiles);
+    load.hk = head / g.blocks;
+    load.block = head - load.hk * g.blocks;
+    load.tile = (int)(left - (int64_t)head * load.tiles);
+  }
+  Cursor<kTile> use = load;
+  const int whole_len = load.len;
 
   // ---- loads: one slot at a time, the keys of a tile, then its values.
   // Kept from a tile's keys to its values:
@@ -501,6 +572,10 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     }
   };
 
+  // g.whole: a warp's part, [head][head_dim], takes its ring's memory once all loads have arrived
+  constexpr int kPart = L::kSlots * L::kSlot / 4;
+  static_assert(kPart >= kCols * 8 * kDim, "a part fits a ring");
+
   // ---- the state of one (sequence, head block)
   constexpr int kKSteps = kWide ? kDim / 8 : kDim / 16;  // steps along head_dim
   constexpr int kMTiles = kDim / 16;                     // blocks of 16 columns of V
@@ -551,10 +626,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     }
 
     // ---- scores
-    if (!wait()) {
-      give_up();
-      return;
-    }
+    if (!wait()) break;
     const uint32_t mask = masks[slot_out];
     float sc[kSubs][kCols][4];
     {
@@ -687,10 +759,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       }
 
     // ---- values
-    if (!wait()) {
-      give_up();
-      return;
-    }
+    if (!wait()) break;
     unsigned char* v_ptr = ring + slot_out * L::kSlot;
     if (kTma && mask != (kTile == 32 ? 0xffffffffu : 0xffffu)) {  // rows that do not exist
 #pragma unroll
@@ -778,7 +847,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     // ---- the end of the sequence's head block, or of this warp's share
     const bool ends = use.tile + 1 == use.tiles;
     if (ends || t + 1 == count) {
-      const bool whole = begins && ends;
+      const bool whole = begins && ends && !g.whole;
       const int64_t part = 2 * w + (begins ? 1 : 0);
       if (begins && !ends && g.jobs && lane == 0) {
         g.jobs[2 * w] = use.b;
@@ -797,7 +866,9 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
           if (h < cols) {
             if (gid == 0) {
               const float base = m[c][i] == -INFINITY ? 0.f : m[c][i];
-              if (!whole) {
+              if (g.whole) {
+                s_ml[warp * 16 + h] = make_float2(m[c][i], x);
+              } else if (!whole) {
                 g.part_ml[(part * g.block + h) * 2] = m[c][i];
                 g.part_ml[(part * g.block + h) * 2 + 1] = x;
               } else if (g.stats) {
@@ -807,7 +878,8 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
               }
             }
             T* out = reinterpret_cast<T*>(g.out) + use.b * g.o_batch + (q0 + h) * g.o_head;
-            float* po = g.part_o + (part * g.block + h) * d;
+            float* po = g.whole ? reinterpret_cast<float*>(ring) + h * d
+                                : g.part_o + (part * g.block + h) * d;
 #pragma unroll
             for (int j = 0; j < kMTiles; ++j)
 #pragma unroll
@@ -825,7 +897,18 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     }
     use.next(g);
   }
-  if (kTma && t < count) give_up();  // only if the lengths change under the kernel
+  if (kTma && t < count) give_up();  // a wait ran out, or the lengths changed under the kernel
+  if (!g.whole) return;
+  if (count == 0 && lane < 16) s_ml[warp * 16 + lane] = make_float2(-INFINITY, 0.f);
+  __syncthreads();
+  if (whole_len == 0) {
+    zero_heads<T>(g, blockIdx.x / (int)kv.kv_heads,
+                  (blockIdx.x % (int)kv.kv_heads) * g.group,
+                  (blockIdx.x % (int)kv.kv_heads + 1) * g.group);
+    return;
+  }
+  join_whole<T>(g, blockIdx.x / (int)kv.kv_heads, blockIdx.x % (int)kv.kv_heads, whole_len, s_ml,
+                reinterpret_cast<const float*>(smem), kPart);
 }
 
 // Launches attend_kernel for g.a.kv's head_dim and g.block; one definition per
@@ -885,8 +968,7 @@ void launch_attend_dim(const AttendArgs& g, cudaStream_t st) {
     IDEV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
     if (known) known->store(true, std::memory_order_relaxed);
   }
-  kernel<<<grid, kWarps * 32, L::kSmem, st>>>(g, k_map, v_map);
-  IDEV_LAUNCHED();
+  launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), L::kSmem, st, g, k_map, v_map);
 }
 
 template <typename T>

@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(256, 3)
     rows_kernel(const __grid_constant__ RowArgs r, int per_warp, int head_blocks, int64_t warps) {
   __shared__ __align__(16) float stage[kTurn == kAcross ? 8 : 1][32 * 8];
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  pdl_wait();
   if (w >= warps) return;
   const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
   const int64_t t = divide(w, head_blocks);
@@ -394,8 +395,7 @@ void launch_rows_of(const RowArgs& r, cudaStream_t st) {
                  : r.turn == kLanes  ? rows_kernel<T, G, kLanes>
                  : r.turn == kWithin ? rows_kernel<T, G, kWithin>
                                      : rows_kernel<T, G, kAcross>;
-  kernel<<<(unsigned)grid, 256, 0, st>>>(r, per_warp, blocks, warps);
-  IDEV_LAUNCHED();
+  launch_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, st, r, per_warp, blocks, warps);
 }
 
 template <typename T>
@@ -519,6 +519,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
   const int64_t job = blockIdx.x / blocks;
   const int64_t b = job / hk;
   const int h = (int)(job - b * hk);
+  pdl_wait();
   const int n = seq_len(e.a, b);
   const int m = min(n, e.keep);
   const float* w = e.w + b * e.w_batch + h * e.w_head;
@@ -741,12 +742,14 @@ void launch_evict(const EvictArgs& e, cudaStream_t st) {
   cfg.blockDim = dim3(kEvictThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   IDEV_CUDA(cudaLaunchKernelEx(&cfg, kernel, e, held));
 }
 
