@@ -25,8 +25,8 @@ struct Parts {
 };
 
 // Where a (sequence, head block)'s parts are.
-__device__ __forceinline__ Parts parts_of(const AttendArgs& g, int64_t t0, int64_t tiles,
-                                          int64_t total, int64_t used) {
+__device__ __forceinline__ Parts parts_of(int64_t t0, int64_t tiles, int64_t total,
+                                          int64_t used) {
   Parts p;
   p.first = owner_of(t0, total, used);
   p.count = (int)(owner_of(t0 + tiles - 1, total, used) - p.first) + 1;
@@ -59,7 +59,7 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
   const int64_t begin = g.before[b], tiles = divide(g.before[b + 1] - begin, heads);
   if (tiles == 0) return;
   const int64_t used = warps_used(total, g.warps);
-  const Parts parts = parts_of(g, begin + head * tiles, tiles, total, used);
+  const Parts parts = parts_of(begin + head * tiles, tiles, total, used);
   if (parts.count == 1) return;
 
   const int hk = head / g.blocks, q0 = hk * g.group + (head % g.blocks) * g.block;
@@ -139,58 +139,59 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
 }
 
 // Adds each position's softmax weight, 2^(s - M) / L summed over the query
-// heads of its key head in their order, to the running sum. The positions are
-// cut among the warps like the tiles. A head's M and L come from its parts where
-// it was cut (each lane takes some of them), else from what its warp left.
-__device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int64_t warps,
+// heads of its key head in their order, to the running sum: piece `piece` of
+// `pieces` of the tiles that attend_kernel's warp w read (its first tile is in
+// g.starts, so that nothing is searched for). A head's M and L come from its parts
+// where it was cut (each lane takes some of them), else from what its warp left.
+__device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int piece, int pieces,
                                             float2* stats) {
   const InfercPagedKv& kv = g.a.kv;
   const int lane = threadIdx.x & 31;
-  const int hk_n = (int)kv.kv_heads, heads = hk_n * g.blocks;
+  const int heads = (int)kv.kv_heads * g.blocks;
   const int64_t q_heads = kv.kv_heads * g.group;
-  // The sequence that holds the first tile, 32 probes a step; the first step's loads do not
-  // wait for the total.
-  int64_t b = 0, size = kv.batch;
-  int64_t step = (size + 31) / 32;
-  int64_t probe = lane * step < size ? g.before[lane * step] : INT64_MAX;
-  const int64_t cut_total = g.before[kv.batch];
-  // tiles of one head per key head, not per block of query heads
-  const int64_t total = divide(cut_total, g.blocks);
+  if (w >= g.warps) return;
+  const int4 start = g.starts[w];
+  const int64_t total = g.before[kv.batch];
   if (total == 0) return;
-  const int64_t used = warps_used(total, warps);
+  const int64_t used = warps_used(total, g.warps);
   if (w >= used) return;
-  const int64_t t0 = first_tile(w, total, used), t1 = first_tile(w + 1, total, used);
-  for (;;) {
-    const int n = __popc(__ballot_sync(0xffffffffu, probe <= t0 * g.blocks));
-    b += (n - 1) * step;
-    size = min(step, size - (n - 1) * step);
-    if (size <= 1) break;
-    step = (size + 31) / 32;
-    probe = lane * step < size ? g.before[b + lane * step] : INT64_MAX;
-  }
+  const int64_t w0 = first_tile(w, total, used), w1 = first_tile(w + 1, total, used);
+  const int64_t t1 = w0 + divide((w1 - w0) * (piece + 1), pieces);
+  int64_t t = w0 + divide((w1 - w0) * piece, pieces);
+  if (t == t1) return;
   const bool vec = aligned16(g.w) && g.w_batch % 4 == 0 && g.w_head % 4 == 0;
-  const int64_t cut_used = warps_used(cut_total, g.warps);
-  int64_t t = t0;
-  while (t < t1) {
-    const int64_t first = g.before[b], after = g.before[b + 1];
-    if (first == after) {
-      ++b;
-      continue;
+  // the head block that holds tile t, its place there
+  int b = start.x, head = start.y;
+  int64_t from = start.z + (t - w0);
+  int len = seq_len(g.a, b), tiles = (len + g.tile - 1) / g.tile;
+  auto next = [&]() {
+    if (++head < heads) return;
+    head = 0;
+    tiles = 0;
+    while (tiles == 0 && ++b < (int)kv.batch) {
+      len = seq_len(g.a, b);
+      tiles = (len + g.tile - 1) / g.tile;
     }
-    const int64_t tiles = divide(after - first, heads);
-    const int64_t at = t - divide(first, g.blocks);
-    const int h = (int)divide(at, tiles);
-    const int64_t from = at - h * tiles;  // tiles of this head: [from, upto)
-    const int64_t upto = min(tiles, from + (t1 - t));
-    const int n = min((int64_t)seq_len(g.a, b), upto * g.tile);
+  };
+  while (b < (int)kv.batch && from >= tiles) {
+    from -= tiles;
+    next();
+  }
+  // (b stays below batch unless the lengths change under the kernel)
+  for (; t < t1 && b < (int)kv.batch; next(), from = 0) {
+    const int64_t upto = min((int64_t)tiles, from + (t1 - t));
+    const int64_t head0 = t - from;  // tile 0 of this head block
+    t += upto - from;
+    if (head % g.blocks) continue;  // summed with the first block of its key head
+    const int h = head / g.blocks;
+    const int n = (int)min((int64_t)len, upto * g.tile);
     const int64_t r = b * q_heads + (int64_t)h * g.group;
     const float* s = g.scores + r * g.capacity;
     float* sum = g.w + b * g.w_batch + h * g.w_head;
     for (int i0 = 0; i0 < g.group; i0 += g.block) {
       const int cols = min(g.block, g.group - i0);
-      const int64_t head = (int64_t)h * g.blocks + i0 / g.block;
       Parts parts{0, 1};
-      if (g.part_ml) parts = parts_of(g, first + head * tiles, tiles, cut_total, cut_used);
+      if (g.part_ml) parts = parts_of(head0 + i0 / g.block * tiles, tiles, total, used);
       // lanes h and h + 16 take head h, every second part each
       const int mine = lane & 15;
       float2 st = make_float2(0.f, 0.f);
@@ -244,8 +245,6 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int6
         }
       }
     }
-    t += upto - from;
-    if (upto == tiles && h + 1 == hk_n) ++b;
   }
 }
 
@@ -253,7 +252,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int6
 template <typename T>
 __global__ void __launch_bounds__(kJoinMost, 2) finish_kernel(const __grid_constant__ AttendArgs g,
                                                               int jobs, bool by_warp, int of,
-                                                              int64_t sum_warps) {
+                                                              int pieces) {
   __shared__ float4 s_o[kJoinMost];
   __shared__ float2 s_ml[kJoinMost];
   pdl_launch_dependents();
@@ -262,8 +261,9 @@ __global__ void __launch_bounds__(kJoinMost, 2) finish_kernel(const __grid_const
     join<T>(g, blockIdx.x / of, by_warp, blockIdx.x % of, of, s_o, s_ml);
   } else {
     const int warp = threadIdx.x >> 5;
-    add_weights(g, (int64_t)(blockIdx.x - jobs * of) * (blockDim.x / 32) + warp, sum_warps,
-                s_ml + warp * 16);
+    const int64_t i = (int64_t)(blockIdx.x - jobs * of) * (blockDim.x / 32) + warp;
+    const int64_t w = divide(i, pieces);
+    add_weights(g, w, (int)(i - w * pieces), pieces, s_ml + warp * 16);
   }
 }
 
@@ -314,7 +314,10 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
     g.part_ml = reinterpret_cast<float*>(take(2 * g.warps * g.block * 8));
     g.part_o = reinterpret_cast<float*>(take(2 * g.warps * g.block * kv.head_dim * 4));
   }
-  if (weights && !g.whole) g.stats = reinterpret_cast<float*>(take(kv.batch * q_heads * 8));
+  if (weights && !g.whole) {
+    g.starts = reinterpret_cast<int4*>(take(g.warps * 16));
+    g.stats = reinterpret_cast<float*>(take(kv.batch * q_heads * 8));
+  }
   if (weights) {
     g.scores = reinterpret_cast<float*>(take(kv.batch * q_heads * g.capacity * 4));
   }
@@ -345,12 +348,11 @@ void run(const Plan& p, cudaStream_t st) {
     of = (int)std::min<int64_t>(g.block, std::max<int64_t>(1, 4 * kSMs / jobs));
   }
   const int threads = jobs * of > kSMs || g.w ? kJoinMost / 4 : kJoinMost;
-  // sums: as many warps as the SMs hold, no more than there are tiles
-  const int64_t tiles = kv.batch * kv.kv_heads * ((g.capacity + g.tile - 1) / g.tile);
-  const int64_t sum_warps = g.w ? std::min<int64_t>((int64_t)kSMs * 32, tiles) : 0;
-  const int64_t grid = jobs * of + (sum_warps * 32 + threads - 1) / threads;
+  // sums: as many warps as the SMs hold
+  const int pieces = g.w ? (int)std::max<int64_t>(1, (int64_t)kSMs * 32 / g.warps) : 0;
+  const int64_t grid = jobs * of + (g.warps * pieces * 32 + threads - 1) / threads;
   launch_pdl(finish_kernel<T>, dim3((unsigned)grid), dim3(threads), 0, st, g, (int)jobs, by_warp,
-             of, sum_warps);
+             of, pieces);
 }
 
 }  // namespace

@@ -65,6 +65,7 @@ struct AttendArgs {
   int64_t warps;    // in the grid
   int64_t* before;  // [batch + 1] tiles before each sequence
   int32_t* jobs;    // [warps, 2] (sequence, head block) whose first part this warp left; -1
+  int4* starts;     // [warps] (sequence, head block, tile) where a warp's share begins
   float* part_ml;   // [2 warps, block, 2] maximum and sum of a part
   float* part_o;    // [2 warps, block, head_dim]
   float* scores;    // [batch, q_heads, capacity] or nullptr
@@ -397,6 +398,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     load.hk = head / g.blocks;
     load.block = head - load.hk * g.blocks;
     load.tile = (int)(left - (int64_t)head * load.tiles);
+    if (g.starts && lane == 0) g.starts[w] = make_int4(load.b, head, load.tile, 0);
   }
   Cursor<kTile> use = load;
   const int whole_len = load.len;
