@@ -140,24 +140,23 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
 
 // Adds each position's softmax weight, 2^(s - M) / L summed over the query
 // heads of its key head in their order, to the running sum: piece `piece` of
-// `pieces` of the tiles that attend_kernel's warp w read (its first tile is in
-// g.starts, so that nothing is searched for). A head's M and L come from its parts
+// 2^`log_pieces` of the tiles that attend_kernel's warp w read (its first tile
+// is in g.starts, so that nothing is searched for). A head's M and L come from its parts
 // where it was cut (each lane takes some of them), else from what its warp left.
-__device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int piece, int pieces,
-                                            float2* stats) {
+__device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int piece,
+                                            int log_pieces, float2* stats) {
   const InfercPagedKv& kv = g.a.kv;
   const int lane = threadIdx.x & 31;
   const int heads = (int)kv.kv_heads * g.blocks;
   const int64_t q_heads = kv.kv_heads * g.group;
-  if (w >= g.warps) return;
   const int4 start = g.starts[w];
   const int64_t total = g.before[kv.batch];
   if (total == 0) return;
   const int64_t used = warps_used(total, g.warps);
   if (w >= used) return;
   const int64_t w0 = first_tile(w, total, used), w1 = first_tile(w + 1, total, used);
-  const int64_t t1 = w0 + divide((w1 - w0) * (piece + 1), pieces);
-  int64_t t = w0 + divide((w1 - w0) * piece, pieces);
+  const int64_t t1 = w0 + ((w1 - w0) * (piece + 1) >> log_pieces);
+  int64_t t = w0 + ((w1 - w0) * piece >> log_pieces);
   if (t == t1) return;
   const bool vec = aligned16(g.w) && g.w_batch % 4 == 0 && g.w_head % 4 == 0;
   // the head block that holds tile t, its place there
@@ -191,7 +190,8 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int 
     for (int i0 = 0; i0 < g.group; i0 += g.block) {
       const int cols = min(g.block, g.group - i0);
       Parts parts{0, 1};
-      if (g.part_ml) parts = parts_of(head0 + i0 / g.block * tiles, tiles, total, used);
+      const int64_t t0 = head0 + i0 / g.block * tiles;
+      if (g.part_ml && (t0 < w0 || t0 + tiles > w1)) parts = parts_of(t0, tiles, total, used);
       // lanes h and h + 16 take head h, every second part each
       const int mine = lane & 15;
       float2 st = make_float2(0.f, 0.f);
@@ -251,8 +251,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int 
 // Behind attend_kernel: the first jobs * of blocks join, the others add weights.
 template <typename T>
 __global__ void __launch_bounds__(kJoinMost, 2) finish_kernel(const __grid_constant__ AttendArgs g,
-                                                              int jobs, bool by_warp, int of,
-                                                              int pieces) {
+                                                              int jobs, bool by_warp, int of) {
   __shared__ float4 s_o[kJoinMost];
   __shared__ float2 s_ml[kJoinMost];
   pdl_launch_dependents();
@@ -261,9 +260,7 @@ __global__ void __launch_bounds__(kJoinMost, 2) finish_kernel(const __grid_const
     join<T>(g, blockIdx.x / of, by_warp, blockIdx.x % of, of, s_o, s_ml);
   } else {
     const int warp = threadIdx.x >> 5;
-    const int64_t i = (int64_t)(blockIdx.x - jobs * of) * (blockDim.x / 32) + warp;
-    const int64_t w = divide(i, pieces);
-    add_weights(g, w, (int)(i - w * pieces), pieces, s_ml + warp * 16);
+    add_weights(g, blockIdx.x - jobs * of, warp, 31 - __clz(blockDim.x / 32), s_ml + warp * 16);
   }
 }
 
@@ -348,11 +345,10 @@ void run(const Plan& p, cudaStream_t st) {
     of = (int)std::min<int64_t>(g.block, std::max<int64_t>(1, 4 * kSMs / jobs));
   }
   const int threads = jobs * of > kSMs || g.w ? kJoinMost / 4 : kJoinMost;
-  // sums: as many warps as the SMs hold
-  const int pieces = g.w ? (int)std::max<int64_t>(1, (int64_t)kSMs * 32 / g.warps) : 0;
-  const int64_t grid = jobs * of + (g.warps * pieces * 32 + threads - 1) / threads;
+  // sums: a block for the share of each warp of attend_kernel
+  const int64_t grid = jobs * of + (g.w ? g.warps : 0);
   launch_pdl(finish_kernel<T>, dim3((unsigned)grid), dim3(threads), 0, st, g, (int)jobs, by_warp,
-             of, pieces);
+             of);
 }
 
 }  // namespace
