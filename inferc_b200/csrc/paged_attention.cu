@@ -12,7 +12,8 @@ namespace {
 
 constexpr int kSMs = 148;  // B200; elsewhere the grid runs in waves
 constexpr int kWholeTiles = 16;
-constexpr int kJoinMost = 512;  // threads of a block of finish_kernel, or a quarter of them
+constexpr int kJoinThreads = 256;
+constexpr int kLogPieces = 3;  // pieces of a warp's share, one per warp of a block
 
 // The parts of one (sequence, head block): warp `first`'s second slot, then
 // the first slots of the warps behind it.
@@ -35,42 +36,70 @@ __device__ __forceinline__ Parts parts_of(int64_t t0, int64_t tiles, int64_t tot
 
 // Joins what several warps left of a (sequence, head block):
 //   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-// One block per cut head block (or per share `part` of `of` of its heads). Its
-// jobs are found by (sequence, head block) where those are fewer than the
-// warps, else by the warp that left the first part. Bound by latency: each
-// thread takes four columns of a head and every `shares`-th part, fetches four
-// parts' columns, maxima and sums at once, and the shares meet in shared memory.
+// Several blocks per head block (`of`), each for some of its columns. Where
+// those are fewer than the warps, the jobs are all (sequence, head block)s and
+// the parts follow from the lengths, which are read while attend_kernel still
+// runs; else a job is a warp that left a first part, and what it wrote. Bound by
+// latency: each thread takes four columns of a head and every `shares`-th part
+// and fetches four parts at once, so that up to 32 to 128 parts (by the columns)
+// cost one round trip, and the shares meet in shared memory.
 template <typename T>
 __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp, int part, int of,
-                                     float4* s_o, float2* s_ml) {
+                                     float4* s_o, float2* s_ml, int64_t* s_sum) {
   constexpr int kAtOnce = 4;
   const InfercPagedKv& kv = g.a.kv;
-  const int tid = threadIdx.x, threads = blockDim.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int heads = (int)kv.kv_heads * g.blocks, d = kv.head_dim;
-  const int64_t total = g.before[kv.batch];
-  if (total == 0) return;
-  int64_t b = job / heads;
-  int head = job % heads;
+  int64_t b;
+  int head;
+  Parts parts;
   if (by_warp) {
-    b = g.jobs[2 * job];
-    head = g.jobs[2 * job + 1];
-    if (b < 0) return;
+    pdl_wait();
+    const int4 left = g.jobs[job];
+    if (left.x < 0) return;
+    b = left.x;
+    head = left.y;
+    parts.first = job;
+    parts.count = left.z;
+  } else {
+    b = job / heads;
+    head = job - (int)b * heads;
+    int64_t all = 0, ahead = 0;  // tiles of one head: in all, and before sequence b
+    for (int i = tid; i < (int)kv.batch; i += kJoinThreads) {
+      const int64_t n = (seq_len(g.a, i) + g.tile - 1) / g.tile;
+      all += n;
+      if (i < b) ahead += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    }
+    if (lane == 0) s_sum[warp] = all, s_sum[kJoinThreads / 32 + warp] = ahead;
+    __syncthreads();
+    all = ahead = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) {
+      all += s_sum[i];
+      ahead += s_sum[kJoinThreads / 32 + i];
+    }
+    const int64_t tiles = (seq_len(g.a, b) + g.tile - 1) / g.tile;
+    if (tiles > 0)
+      parts = parts_of(ahead * heads + head * tiles, tiles, all * heads,
+                       warps_used(all * heads, g.warps));
+    pdl_wait();
+    if (tiles == 0 || parts.count == 1) return;
   }
-  const int64_t begin = g.before[b], tiles = divide(g.before[b + 1] - begin, heads);
-  if (tiles == 0) return;
-  const int64_t used = warps_used(total, g.warps);
-  const Parts parts = parts_of(begin + head * tiles, tiles, total, used);
-  if (parts.count == 1) return;
 
-  const int hk = head / g.blocks, q0 = hk * g.group + (head % g.blocks) * g.block;
+  const int hk = head / g.blocks, q0 = hk * g.group + (head - hk * g.blocks) * g.block;
   const int cols = min(g.block, hk * g.group + g.group - q0);
-  const int h0 = cols * part / of, h1 = cols * (part + 1) / of;
-  const int quads = d / 4, items = (h1 - h0) * quads;  // float4s of the result
-  for (int base = 0; base < items; base += threads) {
-    const int n = min(items - base, threads);
-    const int shares = min(threads / n, parts.count);
-    const int share = tid / n, item = base + tid % n;
-    const int h = h0 + item / quads, quad = item % quads;
+  const int quads = d / 4, items = cols * quads;  // float4s of the result
+  const int item1 = items * (part + 1) / of;
+  for (int base = items * part / of; base < item1; base += kJoinThreads) {
+    const int n = min(item1 - base, kJoinThreads);
+    const int shares = min(kJoinThreads / n, 32);
+    const int share = tid / n, item = base + tid - share * n;
+    const int h = item / quads, quad = item - h * quads;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (share < shares) {
@@ -110,7 +139,29 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
     s_ml[tid] = make_float2(m, l);
     s_o[tid] = o;
     __syncthreads();
-    if (share == 0) {
+    auto finish = [&](int h, int quad, float l, float4 o) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: every page was bad
+      T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + (q0 + h) * g.o_head + quad * 4;
+      out[0] = T(o.x * inv);
+      out[1] = T(o.y * inv);
+      out[2] = T(o.z * inv);
+      out[3] = T(o.w * inv);
+    };
+    if (shares > 8) {  // a warp per item, a lane per share
+      for (int i = warp; i < n; i += kJoinThreads / 32) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane < shares) ml = s_ml[lane * n + i], x = s_o[lane * n + i];
+        const float top = warp_max(ml.x), f = ex2(ml.x - (top == -INFINITY ? 0.f : top));
+        const float sum = warp_sum(f * ml.y);
+        x.x = warp_sum(f * x.x);
+        x.y = warp_sum(f * x.y);
+        x.z = warp_sum(f * x.z);
+        x.w = warp_sum(f * x.w);
+        const int h = (base + i) / quads;
+        if (lane == 0) finish(h, base + i - h * quads, sum, x);
+      }
+    } else if (share == 0) {
       float top = m;
       for (int s = 1; s < shares; ++s) top = fmaxf(top, s_ml[s * n + tid].x);
       const float to = top == -INFINITY ? 0.f : top;
@@ -127,12 +178,7 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
         o.z += f * x.z;
         o.w += f * x.w;
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: every page was bad
-      T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + (q0 + h) * g.o_head + quad * 4;
-      out[0] = T(o.x * inv);
-      out[1] = T(o.y * inv);
-      out[2] = T(o.z * inv);
-      out[3] = T(o.w * inv);
+      finish(h, quad, l, o);
     }
     __syncthreads();
   }
@@ -250,17 +296,20 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int 
 
 // Behind attend_kernel: the first jobs * of blocks join, the others add weights.
 template <typename T>
-__global__ void __launch_bounds__(kJoinMost, 2) finish_kernel(const __grid_constant__ AttendArgs g,
-                                                              int jobs, bool by_warp, int of) {
-  __shared__ float4 s_o[kJoinMost];
-  __shared__ float2 s_ml[kJoinMost];
+__global__ void __launch_bounds__(kJoinThreads, 4) finish_kernel(
+    const __grid_constant__ AttendArgs g, int jobs, bool by_warp, int of) {
+  static_assert(kJoinThreads / 32 == 1 << kLogPieces, "a warp per piece");
+  __shared__ float4 s_o[kJoinThreads];
+  __shared__ float2 s_ml[kJoinThreads];
+  __shared__ int64_t s_sum[kJoinThreads / 16];
   pdl_launch_dependents();
-  pdl_wait();
   if ((int)blockIdx.x < jobs * of) {
-    join<T>(g, blockIdx.x / of, by_warp, blockIdx.x % of, of, s_o, s_ml);
+    const int job = blockIdx.x / of;
+    join<T>(g, job, by_warp, blockIdx.x - job * of, of, s_o, s_ml, s_sum);
   } else {
+    pdl_wait();
     const int warp = threadIdx.x >> 5;
-    add_weights(g, blockIdx.x - jobs * of, warp, 31 - __clz(blockDim.x / 32), s_ml + warp * 16);
+    add_weights(g, blockIdx.x - jobs * of, warp, kLogPieces, s_ml + warp * 16);
   }
 }
 
@@ -307,7 +356,7 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
   };
   if (p.cut || (weights && !g.whole)) g.before = reinterpret_cast<int64_t*>(take((kv.batch + 1) * 8));
   if (p.cut) {
-    g.jobs = reinterpret_cast<int32_t*>(take(g.warps * 8));
+    g.jobs = reinterpret_cast<int4*>(take(g.warps * 16));
     g.part_ml = reinterpret_cast<float*>(take(2 * g.warps * g.block * 8));
     g.part_o = reinterpret_cast<float*>(take(2 * g.warps * g.block * kv.head_dim * 4));
   }
@@ -341,13 +390,14 @@ void run(const Plan& p, cudaStream_t st) {
     const int64_t pairs = kv.batch * kv.kv_heads * g.blocks;
     by_warp = pairs > g.warps;
     jobs = by_warp ? g.warps : pairs;
-    // few jobs: their heads go to blocks of their own
-    of = (int)std::min<int64_t>(g.block, std::max<int64_t>(1, 4 * kSMs / jobs));
+    // few jobs: several blocks each, of eight float4s of the result at least
+    of = (int)std::min<int64_t>(g.block * (kv.head_dim / 4) / 8,
+                                std::max<int64_t>(1, 4 * kSMs / jobs));
+    of = std::max(of, 1);
   }
-  const int threads = jobs * of > kSMs || g.w ? kJoinMost / 4 : kJoinMost;
   // sums: a block for the share of each warp of attend_kernel
   const int64_t grid = jobs * of + (g.w ? g.warps : 0);
-  launch_pdl(finish_kernel<T>, dim3((unsigned)grid), dim3(threads), 0, st, g, (int)jobs, by_warp,
+  launch_pdl(finish_kernel<T>, dim3((unsigned)grid), dim3(kJoinThreads), 0, st, g, (int)jobs, by_warp,
              of);
 }
 

@@ -64,7 +64,7 @@ struct AttendArgs {
   bool whole;       // one block of the grid reads one (sequence, key head), see attend_kernel
   int64_t warps;    // in the grid
   int64_t* before;  // [batch + 1] tiles before each sequence
-  int32_t* jobs;    // [warps, 2] (sequence, head block) whose first part this warp left; -1
+  int4* jobs;       // [warps] (sequence or -1, head block, parts) whose first part this warp left
   int4* starts;     // [warps] (sequence, head block, tile) where a warp's share begins
   float* part_ml;   // [2 warps, block, 2] maximum and sum of a part
   float* part_o;    // [2 warps, block, head_dim]
@@ -324,10 +324,12 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)));
     }
 
-  pdl_launch_dependents();
   pdl_wait();  // lengths, tables, queries and caches may come from the kernel before
+  // (finish_kernel reads the lengths as soon as every block has passed here)
+  pdl_launch_dependents();
 
   int64_t w = (int64_t)blockIdx.x * kWarps + warp;
+  int64_t total = 0, used = 0, t0 = 0;  // tiles, warps that share them, this warp's first
   int count = 0;
   Cursor<kTile> load;
   if (g.whole) {
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     }
     if (lane == 31) s_warp[warp] = scan;
     __syncthreads();
-    int64_t total = 0, ahead = 0;
+    int64_t ahead = 0;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       if (i < warp) ahead += s_warp[i];
@@ -376,10 +378,10 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
         zero_heads<T>(g, b, 0, (int)kv.kv_heads * g.group);
     __syncthreads();
 
-    if (g.jobs && lane == 0 && w < g.warps) g.jobs[2 * w] = -1;
-    const int64_t used = warps_used(total, g.warps);
+    if (g.jobs && lane == 0 && w < g.warps) g.jobs[w] = make_int4(-1, 0, 0, 0);
+    used = warps_used(total, g.warps);
     if (w >= used) return;
-    const int64_t t0 = first_tile(w, total, used);
+    t0 = first_tile(w, total, used);
     count = (int)(first_tile(w + 1, total, used) - t0);
 
     // The tile t0: the thread whose run holds it, then the sequence, then the head.
@@ -852,8 +854,9 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       const bool whole = begins && ends && !g.whole;
       const int64_t part = 2 * w + (begins ? 1 : 0);
       if (begins && !ends && g.jobs && lane == 0) {
-        g.jobs[2 * w] = use.b;
-        g.jobs[2 * w + 1] = use.hk * g.blocks + use.block;
+        const int64_t last = t0 + t + use.tiles - use.tile - 1;
+        g.jobs[w] = make_int4(use.b, use.hk * g.blocks + use.block,
+                              (int)(owner_of(last, total, used) - w) + 1, 0);
       }
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
