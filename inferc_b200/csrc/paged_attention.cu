@@ -12,8 +12,7 @@ namespace {
 
 constexpr int kSMs = 148;  // B200; elsewhere the grid runs in waves
 constexpr int kWholeTiles = 16;
-constexpr int kJoinThreads = 256;
-constexpr int kLogPieces = 3;  // pieces of a warp's share, one per warp of a block
+constexpr int kJoinThreads = 128;
 
 // The parts of one (sequence, head block): warp `first`'s second slot, then
 // the first slots of the warps behind it.
@@ -32,6 +31,34 @@ __device__ __forceinline__ Parts parts_of(int64_t t0, int64_t tiles, int64_t tot
   p.first = owner_of(t0, total, used);
   p.count = (int)(owner_of(t0 + tiles - 1, total, used) - p.first) + 1;
   return p;
+}
+
+// Tiles of one head block: of all sequences, and (*ahead) of those before b. By
+// the whole block; the lengths may be read while attend_kernel still runs.
+__device__ __forceinline__ int64_t all_tiles(const AttendArgs& g, int64_t b, int64_t* ahead_out,
+                                             int64_t* s_sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t all = 0, ahead = 0;
+  for (int i = threadIdx.x; i < (int)g.a.kv.batch; i += kJoinThreads) {
+    const int64_t n = (seq_len(g.a, i) + g.tile - 1) / g.tile;
+    all += n;
+    if (i < b) ahead += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+  }
+  if (lane == 0) s_sum[warp] = all, s_sum[kJoinThreads / 32 + warp] = ahead;
+  __syncthreads();
+  all = ahead = 0;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) {
+    all += s_sum[i];
+    ahead += s_sum[kJoinThreads / 32 + i];
+  }
+  *ahead_out = ahead;
+  return all;
 }
 
 // Joins what several warps left of a (sequence, head block):
@@ -64,25 +91,8 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
   } else {
     b = job / heads;
     head = job - (int)b * heads;
-    int64_t all = 0, ahead = 0;  // tiles of one head: in all, and before sequence b
-    for (int i = tid; i < (int)kv.batch; i += kJoinThreads) {
-      const int64_t n = (seq_len(g.a, i) + g.tile - 1) / g.tile;
-      all += n;
-      if (i < b) ahead += n;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, o);
-      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
-    }
-    if (lane == 0) s_sum[warp] = all, s_sum[kJoinThreads / 32 + warp] = ahead;
-    __syncthreads();
-    all = ahead = 0;
-#pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) {
-      all += s_sum[i];
-      ahead += s_sum[kJoinThreads / 32 + i];
-    }
+    int64_t ahead;
+    const int64_t all = all_tiles(g, b, &ahead, s_sum);
     const int64_t tiles = (seq_len(g.a, b) + g.tile - 1) / g.tile;
     if (tiles > 0)
       parts = parts_of(ahead * heads + head * tiles, tiles, all * heads,
@@ -184,26 +194,135 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
   }
 }
 
-// Adds each position's softmax weight, 2^(s - M) / L summed over the query
-// heads of its key head in their order, to the running sum: piece `piece` of
-// 2^`log_pieces` of the tiles that attend_kernel's warp w read (its first tile
-// is in g.starts, so that nothing is searched for). A head's M and L come from its parts
-// where it was cut (each lane takes some of them), else from what its warp left.
-__device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int piece,
-                                            int log_pieces, float2* stats) {
-  const InfercPagedKv& kv = g.a.kv;
+// (M, 1 / L) of `cols` heads from row `r` on, to stats, by one warp.
+__device__ __forceinline__ void head_stats(const AttendArgs& g, const Parts& parts, int cols,
+                                           int64_t r, float2* stats) {
   const int lane = threadIdx.x & 31;
+  // lanes h and h + 16 take head h, every second part each
+  const int mine = lane & 15;
+  float2 st = make_float2(0.f, 0.f);
+  if (parts.count == 1) {
+    if (mine < cols) st = reinterpret_cast<const float2*>(g.stats)[r + mine];
+  } else {
+    float m = -INFINITY, l = 0.f;
+    if (mine < cols)
+#pragma unroll 4
+      for (int p = lane >> 4; p < parts.count; p += 2) {
+        const float2 ml =
+            reinterpret_cast<const float2*>(g.part_ml)[parts.slot(p) * g.block + mine];
+        const float top = fmaxf(m, ml.x), to = top == -INFINITY ? 0.f : top;
+        l = l * ex2(m - to) + ml.y * ex2(ml.x - to);
+        m = top;
+      }
+    const float top = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    const float to = top == -INFINITY ? 0.f : top;
+    l *= ex2(m - to);
+    // both lanes add in the same order
+    const float other = __shfl_xor_sync(0xffffffffu, l, 16);
+    l = lane < 16 ? l + other : other + l;
+    st = make_float2(to, l == 0.f ? 0.f : 1.f / l);
+  }
+  __syncwarp();
+  if (lane < cols) stats[lane] = st;
+  __syncwarp();
+}
+
+// Positions [j0, n) of one key head: sum[j] += the weights of `cols` heads, whose
+// scores are `stride` floats apart. A lane takes four positions in kRuns runs of
+// 128 and fetches kCols heads of each before it uses the first (all of this
+// waits on memory, little of it); the heads' statistics are looked up meanwhile.
+template <int kCols, int kRuns, typename Stats>
+__device__ __forceinline__ void add_positions(const float* s, int64_t stride, int cols, float* sum,
+                                              int j0, int n, bool vec, const float2* stats,
+                                              Stats&& stats_of) {
+  const int lane = threadIdx.x & 31;
+  bool first = true;
+  for (int base = j0; base < n; base += 128 * kRuns) {
+    float4 p[kRuns], old[kRuns];
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) {
+      const int j = base + u * 128 + lane * 4;
+      p[u] = old[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j + 4 <= n && vec) {
+        old[u] = *reinterpret_cast<const float4*>(sum + j);
+      } else if (j < n) {
+        old[u].x = sum[j];
+        if (j + 1 < n) old[u].y = sum[j + 1];
+        if (j + 2 < n) old[u].z = sum[j + 2];
+        if (j + 3 < n) old[u].w = sum[j + 3];
+      }
+    }
+    for (int c0 = 0; c0 < cols; c0 += kCols) {
+      float4 x[kRuns][kCols];
+#pragma unroll
+      for (int u = 0; u < kRuns; ++u)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int j = base + u * 128 + lane * 4;
+          x[u][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+          // (the rows are padded to a multiple of four positions)
+          if (j < n && c0 + c < cols)
+            x[u][c] = *reinterpret_cast<const float4*>(s + (c0 + c) * stride + j);
+        }
+      if (first) {
+        first = false;
+        stats_of();
+      }
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        if (c0 + c >= cols) break;
+        const float2 st = stats[c0 + c];
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u) {
+          p[u].x += ex2(x[u][c].x - st.x) * st.y;
+          p[u].y += ex2(x[u][c].y - st.x) * st.y;
+          p[u].z += ex2(x[u][c].z - st.x) * st.y;
+          p[u].w += ex2(x[u][c].w - st.x) * st.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) {
+      const int j = base + u * 128 + lane * 4;
+      if (j + 4 <= n && vec) {
+        *reinterpret_cast<float4*>(sum + j) = make_float4(old[u].x + p[u].x, old[u].y + p[u].y,
+                                                          old[u].z + p[u].z, old[u].w + p[u].w);
+      } else if (j < n) {
+        sum[j] = old[u].x + p[u].x;
+        if (j + 1 < n) sum[j + 1] = old[u].y + p[u].y;
+        if (j + 2 < n) sum[j + 2] = old[u].z + p[u].z;
+        if (j + 3 < n) sum[j + 3] = old[u].w + p[u].w;
+      }
+    }
+  }
+}
+
+// Adds each position's softmax weight, 2^(s - M) / L summed over the query
+// heads of its key head in their order, to the running sum. The tiles are cut
+// among `warps` warps as they were among attend_kernel's, four tiles (128
+// positions) at least; where one of those began is in g.starts, so that nothing
+// is searched for. A head's M and L come from its parts where it was cut (each
+// lane takes some of them), else from what its warp left.
+__device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t i, int64_t warps,
+                                            float2* stats, int64_t* s_sum) {
+  const InfercPagedKv& kv = g.a.kv;
   const int heads = (int)kv.kv_heads * g.blocks;
   const int64_t q_heads = kv.kv_heads * g.group;
-  const int4 start = g.starts[w];
-  const int64_t total = g.before[kv.batch];
-  if (total == 0) return;
-  const int64_t used = warps_used(total, g.warps);
-  if (w >= used) return;
-  const int64_t w0 = first_tile(w, total, used), w1 = first_tile(w + 1, total, used);
-  const int64_t t1 = w0 + ((w1 - w0) * (piece + 1) >> log_pieces);
-  int64_t t = w0 + ((w1 - w0) * piece >> log_pieces);
+  int64_t ahead;
+  const int64_t total = all_tiles(g, 0, &ahead, s_sum) * heads;
+  const int64_t n = min(warps, (total + 3) / 4);
+  int64_t used = 1, t = 0, t1 = 0, w = 0, w0 = 0, w1 = 0;
+  if (i < n) {
+    used = warps_used(total, g.warps);
+    t = first_tile(i, total, n);
+    t1 = first_tile(i + 1, total, n);
+    w = owner_of(t, total, used);
+    w0 = first_tile(w, total, used);
+    w1 = first_tile(w + 1, total, used);
+  }
+  pdl_wait();
   if (t == t1) return;
+  const int4 start = g.starts[w];
   const bool vec = aligned16(g.w) && g.w_batch % 4 == 0 && g.w_head % 4 == 0;
   // the head block that holds tile t, its place there
   int b = start.x, head = start.y;
@@ -235,61 +354,16 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int 
     float* sum = g.w + b * g.w_batch + h * g.w_head;
     for (int i0 = 0; i0 < g.group; i0 += g.block) {
       const int cols = min(g.block, g.group - i0);
-      Parts parts{0, 1};
       const int64_t t0 = head0 + i0 / g.block * tiles;
+      Parts parts{0, 1};
       if (g.part_ml && (t0 < w0 || t0 + tiles > w1)) parts = parts_of(t0, tiles, total, used);
-      // lanes h and h + 16 take head h, every second part each
-      const int mine = lane & 15;
-      float2 st = make_float2(0.f, 0.f);
-      if (parts.count == 1) {
-        if (mine < cols) st = reinterpret_cast<const float2*>(g.stats)[r + i0 + mine];
-      } else {
-        float m = -INFINITY, l = 0.f;
-        if (mine < cols)
-#pragma unroll 4
-          for (int p = lane >> 4; p < parts.count; p += 2) {
-            const float2 ml =
-                reinterpret_cast<const float2*>(g.part_ml)[parts.slot(p) * g.block + mine];
-            const float top = fmaxf(m, ml.x), to = top == -INFINITY ? 0.f : top;
-            l = l * ex2(m - to) + ml.y * ex2(ml.x - to);
-            m = top;
-          }
-        const float top = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        const float to = top == -INFINITY ? 0.f : top;
-        l *= ex2(m - to);
-        // both lanes add in the same order
-        const float other = __shfl_xor_sync(0xffffffffu, l, 16);
-        l = lane < 16 ? l + other : other + l;
-        st = make_float2(to, l == 0.f ? 0.f : 1.f / l);
-      }
-      __syncwarp();
-      if (lane < cols) stats[lane] = st;
-      __syncwarp();
-      // four positions a lane; g.capacity and the tiles are multiples of 4
-#pragma unroll 2
-      for (int j = (int)from * g.tile + lane * 4; j < n; j += 128) {
-        const bool four = vec && j + 4 <= n;
-        float4 p = make_float4(0.f, 0.f, 0.f, 0.f), old = p;
-        if (four) old = *reinterpret_cast<const float4*>(sum + j);
-#pragma unroll 4
-        for (int i = 0; i < cols; ++i) {
-          const float2 st = stats[i];
-          const float4 x = *reinterpret_cast<const float4*>(s + (i0 + i) * g.capacity + j);
-          p.x += ex2(x.x - st.x) * st.y;
-          p.y += ex2(x.y - st.x) * st.y;
-          p.z += ex2(x.z - st.x) * st.y;
-          p.w += ex2(x.w - st.x) * st.y;
-        }
-        if (four) {
-          *reinterpret_cast<float4*>(sum + j) =
-              make_float4(old.x + p.x, old.y + p.y, old.z + p.z, old.w + p.w);
-        } else {
-          sum[j] += p.x;
-          if (j + 1 < n) sum[j + 1] += p.y;
-          if (j + 2 < n) sum[j + 2] += p.z;
-          if (j + 3 < n) sum[j + 3] += p.w;
-        }
-      }
+      auto stats_of = [&]() { head_stats(g, parts, cols, r + i0, stats); };
+      const float* rows = s + i0 * g.capacity;
+      const int j0 = (int)from * g.tile;
+      if (cols == 1) add_positions<1, 4>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
+      else if (cols == 2) add_positions<2, 3>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
+      else if (cols <= 4) add_positions<4, 2>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
+      else add_positions<8, 1>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
     }
   }
 }
@@ -297,8 +371,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t w, int 
 // Behind attend_kernel: the first jobs * of blocks join, the others add weights.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads, 4) finish_kernel(
-    const __grid_constant__ AttendArgs g, int jobs, bool by_warp, int of) {
-  static_assert(kJoinThreads / 32 == 1 << kLogPieces, "a warp per piece");
+    const __grid_constant__ AttendArgs g, int jobs, bool by_warp, int of, int64_t sum_warps) {
   __shared__ float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
   __shared__ int64_t s_sum[kJoinThreads / 16];
@@ -307,9 +380,9 @@ __global__ void __launch_bounds__(kJoinThreads, 4) finish_kernel(
     const int job = blockIdx.x / of;
     join<T>(g, job, by_warp, blockIdx.x - job * of, of, s_o, s_ml, s_sum);
   } else {
-    pdl_wait();
     const int warp = threadIdx.x >> 5;
-    add_weights(g, blockIdx.x - jobs * of, warp, kLogPieces, s_ml + warp * 16);
+    add_weights(g, (int64_t)(blockIdx.x - jobs * of) * (kJoinThreads / 32) + warp, sum_warps,
+                s_ml + warp * 16, s_sum);
   }
 }
 
@@ -395,10 +468,11 @@ void run(const Plan& p, cudaStream_t st) {
                                 std::max<int64_t>(1, 4 * kSMs / jobs));
     of = std::max(of, 1);
   }
-  // sums: a block for the share of each warp of attend_kernel
-  const int64_t grid = jobs * of + (g.w ? g.warps : 0);
+  // sums: what the SMs hold (4 blocks each) beside the joining blocks, two each at least
+  const int64_t sum_blocks = g.w ? std::max<int64_t>(2 * kSMs, 4 * kSMs - jobs * of) : 0;
+  const int64_t grid = jobs * of + sum_blocks;
   launch_pdl(finish_kernel<T>, dim3((unsigned)grid), dim3(kJoinThreads), 0, st, g, (int)jobs, by_warp,
-             of);
+             of, sum_blocks * (kJoinThreads / 32));
 }
 
 }  // namespace
