@@ -228,72 +228,28 @@ __device__ __forceinline__ void head_stats(const AttendArgs& g, const Parts& par
 }
 
 // Positions [j0, n) of one key head: sum[j] += the weights of `cols` heads, whose
-// scores are `stride` floats apart. A lane takes four positions in kRuns runs of
-// 128 and fetches kCols heads of each before it uses the first (all of this
-// waits on memory, little of it); the heads' statistics are looked up meanwhile.
-template <int kCols, int kRuns, typename Stats>
+// scores are `stride` floats apart; 32 consecutive positions a load, four loads
+// of a head at once.
 __device__ __forceinline__ void add_positions(const float* s, int64_t stride, int cols, float* sum,
-                                              int j0, int n, bool vec, const float2* stats,
-                                              Stats&& stats_of) {
-  const int lane = threadIdx.x & 31;
-  bool first = true;
-  for (int base = j0; base < n; base += 128 * kRuns) {
-    float4 p[kRuns], old[kRuns];
+                                              int j0, int n, const float2* stats) {
+  s += j0 + (threadIdx.x & 31);
+  sum += j0 + (threadIdx.x & 31);
+  int left = n - j0 - (int)(threadIdx.x & 31);  // positions from this lane's on
+  for (; __any_sync(0xffffffffu, left > 0); left -= 128, s += 128, sum += 128) {
+    float p[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* row = s;
+#pragma unroll 2
+    for (int c = 0; c < cols; ++c, row += stride) {
+      const float2 st = stats[c];
+      float x[4];
 #pragma unroll
-    for (int u = 0; u < kRuns; ++u) {
-      const int j = base + u * 128 + lane * 4;
-      p[u] = old[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (j + 4 <= n && vec) {
-        old[u] = *reinterpret_cast<const float4*>(sum + j);
-      } else if (j < n) {
-        old[u].x = sum[j];
-        if (j + 1 < n) old[u].y = sum[j + 1];
-        if (j + 2 < n) old[u].z = sum[j + 2];
-        if (j + 3 < n) old[u].w = sum[j + 3];
-      }
-    }
-    for (int c0 = 0; c0 < cols; c0 += kCols) {
-      float4 x[kRuns][kCols];
+      for (int u = 0; u < 4; ++u) x[u] = left > 32 * u ? row[32 * u] : -INFINITY;
 #pragma unroll
-      for (int u = 0; u < kRuns; ++u)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const int j = base + u * 128 + lane * 4;
-          x[u][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-          // (the rows are padded to a multiple of four positions)
-          if (j < n && c0 + c < cols)
-            x[u][c] = *reinterpret_cast<const float4*>(s + (c0 + c) * stride + j);
-        }
-      if (first) {
-        first = false;
-        stats_of();
-      }
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        if (c0 + c >= cols) break;
-        const float2 st = stats[c0 + c];
-#pragma unroll
-        for (int u = 0; u < kRuns; ++u) {
-          p[u].x += ex2(x[u][c].x - st.x) * st.y;
-          p[u].y += ex2(x[u][c].y - st.x) * st.y;
-          p[u].z += ex2(x[u][c].z - st.x) * st.y;
-          p[u].w += ex2(x[u][c].w - st.x) * st.y;
-        }
-      }
+      for (int u = 0; u < 4; ++u) p[u] += ex2(x[u] - st.x) * st.y;
     }
 #pragma unroll
-    for (int u = 0; u < kRuns; ++u) {
-      const int j = base + u * 128 + lane * 4;
-      if (j + 4 <= n && vec) {
-        *reinterpret_cast<float4*>(sum + j) = make_float4(old[u].x + p[u].x, old[u].y + p[u].y,
-                                                          old[u].z + p[u].z, old[u].w + p[u].w);
-      } else if (j < n) {
-        sum[j] = old[u].x + p[u].x;
-        if (j + 1 < n) sum[j + 1] = old[u].y + p[u].y;
-        if (j + 2 < n) sum[j + 2] = old[u].z + p[u].z;
-        if (j + 3 < n) sum[j + 3] = old[u].w + p[u].w;
-      }
-    }
+    for (int u = 0; u < 4; ++u)
+      if (left > 32 * u) sum[32 * u] += p[u];
   }
 }
 
@@ -323,7 +279,6 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t i, int6
   pdl_wait();
   if (t == t1) return;
   const int4 start = g.starts[w];
-  const bool vec = aligned16(g.w) && g.w_batch % 4 == 0 && g.w_head % 4 == 0;
   // the head block that holds tile t, its place there
   int b = start.x, head = start.y;
   int64_t from = start.z + (t - w0);
@@ -357,20 +312,15 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t i, int6
       const int64_t t0 = head0 + i0 / g.block * tiles;
       Parts parts{0, 1};
       if (g.part_ml && (t0 < w0 || t0 + tiles > w1)) parts = parts_of(t0, tiles, total, used);
-      auto stats_of = [&]() { head_stats(g, parts, cols, r + i0, stats); };
-      const float* rows = s + i0 * g.capacity;
-      const int j0 = (int)from * g.tile;
-      if (cols == 1) add_positions<1, 4>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
-      else if (cols == 2) add_positions<2, 3>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
-      else if (cols <= 4) add_positions<4, 2>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
-      else add_positions<8, 1>(rows, g.capacity, cols, sum, j0, n, vec, stats, stats_of);
+      head_stats(g, parts, cols, r + i0, stats);
+      add_positions(s + i0 * g.capacity, g.capacity, cols, sum, (int)from * g.tile, n, stats);
     }
   }
 }
 
 // Behind attend_kernel: the first jobs * of blocks join, the others add weights.
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads, 4) finish_kernel(
+__global__ void __launch_bounds__(kJoinThreads, 6) finish_kernel(
     const __grid_constant__ AttendArgs g, int jobs, bool by_warp, int of, int64_t sum_warps) {
   __shared__ float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
@@ -468,8 +418,8 @@ void run(const Plan& p, cudaStream_t st) {
                                 std::max<int64_t>(1, 4 * kSMs / jobs));
     of = std::max(of, 1);
   }
-  // sums: what the SMs hold (4 blocks each) beside the joining blocks, two each at least
-  const int64_t sum_blocks = g.w ? std::max<int64_t>(2 * kSMs, 4 * kSMs - jobs * of) : 0;
+  // sums: what the SMs hold
+  const int64_t sum_blocks = g.w ? 6 * kSMs : 0;
   const int64_t grid = jobs * of + sum_blocks;
   launch_pdl(finish_kernel<T>, dim3((unsigned)grid), dim3(kJoinThreads), 0, st, g, (int)jobs, by_warp,
              of, sum_blocks * (kJoinThreads / 32));
