@@ -16,53 +16,61 @@ namespace paged {
 
 enum DType : int { F32 = 1, F16 = 10, BF16 = 16 };  // ONNX TensorProto codes
 
-// Eight consecutive values of a row as they lie in memory (one 16-byte load of
-// a 16-bit type, two of fp32), to be widened when they are used.
+// Eight values of a row as they lie in memory, four from each of two places
+// (which may adjoin), to be widened when they are used.
 template <typename T>
 struct Raw8 {
-  static constexpr int kParts = sizeof(T) / 2;
-  uint4 part[kParts] = {};
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) part[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void store(T* p) const {
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) reinterpret_cast<uint4*>(p)[i] = part[i];
-  }
-  // The same of another lane of the warp.
-  __device__ __forceinline__ Raw8 from_lane(int lane) const {
-    Raw8 r;
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      r.part[i].x = __shfl_sync(0xffffffffu, part[i].x, lane);
-      r.part[i].y = __shfl_sync(0xffffffffu, part[i].y, lane);
-      r.part[i].z = __shfl_sync(0xffffffffu, part[i].z, lane);
-      r.part[i].w = __shfl_sync(0xffffffffu, part[i].w, lane);
-    }
-    return r;
+  using Four = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
+  Four part[2] = {};
+  __device__ __forceinline__ void load(const T* p, int second = 4) {
+    part[0] = *reinterpret_cast<const Four*>(p);
+    part[1] = *reinterpret_cast<const Four*>(p + second);
   }
   __device__ __forceinline__ void widen(float* x) const {
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const uint32_t w[4] = {part[i].x, part[i].y, part[i].z, part[i].w};
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (std::is_same_v<T, float>) {
+        x[4 * i] = __uint_as_float(part[i].x);
+        x[4 * i + 1] = __uint_as_float(part[i].y);
+        x[4 * i + 2] = __uint_as_float(part[i].z);
+        x[4 * i + 3] = __uint_as_float(part[i].w);
+      } else {
+        const uint32_t w[2] = {part[i].x, part[i].y};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (std::is_same_v<T, float>) {
-          x[4 * i + j] = __uint_as_float(w[j]);
-        } else {
+        for (int j = 0; j < 2; ++j) {
           float2 f;
           if constexpr (std::is_same_v<T, __half>)
             f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
           else
             f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-          x[2 * j] = f.x;
-          x[2 * j + 1] = f.y;
+          x[4 * i + 2 * j] = f.x;
+          x[4 * i + 2 * j + 1] = f.y;
         }
       }
     }
   }
 };
+
+// Four values rounded to T, to a place of 4 * sizeof(T) alignment.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* x) {
+  if constexpr (std::is_same_v<T, float>) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+}
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float* x) {

@@ -136,42 +136,46 @@ __device__ __forceinline__ Owner owner_of_token(const int32_t* cu, int64_t n, in
 // How a row's pairs lie in its lanes.
 enum Turn : int {
   kNone = 0,     // no rotation
-  kLanes = 1,    // (i, i + half), half a multiple of 8: the partner lane holds all eight
+  kHalves = 1,   // (i, i + half), half a multiple of 4: a lane holds four columns and their partners
   kWithin = 2,   // (2 i, 2 i + 1): in the lane itself
   kAcross = 3    // (i, i + half) at an odd offset: through shared memory
 };
-
-// Eight floats of a table row from `p`, two at a time 16 bytes where they are aligned.
-__device__ __forceinline__ void table8(const float* p, bool vector, float* x) {
-  if (vector) {
-    load8(p, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
-  }
-}
 
 // Rows a group of lanes fetches before it uses the first: 64 bytes a lane.
 template <typename T>
 constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
 
-// Rows [hb, h1) as far as they go; behind the last, the last once more (its
-// results are not stored). Lanes without columns keep zeros.
+// The eight columns of lane c: first .. first + 3 and first + second .. + 3.
+struct Columns {
+  int first, second;
+};
+template <int kTurn>
+__device__ __forceinline__ Columns columns_of(int c, int half) {
+  if (kTurn == kHalves && c * 4 < half) return {c * 4, half};
+  return {c * 8, 4};  // (behind the rotated columns too: half / 4 lanes hold 2 half columns)
+}
+
+// Rows [hb, h1) as far as they go. Lanes without columns keep zeros, and those
+// without a row what they had (its results are not stored).
 template <typename T, int G>
-__device__ __forceinline__ void fetch_rows(const T* src, int64_t src_head, int hb, int h1, int d,
+__device__ __forceinline__ void fetch_rows(const T* src, int64_t src_head, int hb, int h1,
+                                           bool column, const Columns& col,
                                            Raw8<T> (&raw)[kAhead<T>]) {
-  const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
+  const int sub = (threadIdx.x & 31) / G;
+  src += (hb + sub) * src_head + col.first;
 #pragma unroll
-  for (int u = 0; u < kAhead<T>; ++u)
-    if (c * 8 < d && hb < h1)
-      raw[u].load(src + min(hb + u * (32 / G) + sub, h1 - 1) * src_head + c * 8);
+  for (int u = 0; u < kAhead<T>; ++u) {
+    if (column && hb + u * (32 / G) + sub < h1) raw[u].load(src, col.second);
+    src += 32 / G * src_head;
+  }
 }
 
 // Norm and rotation of the heads [h0, h1) of the queries or the keys of one
 // token by one warp: G lanes share a row, 8 values each. With gamma, c and s folded,
 //   y_i = inv * (x_i * own_i + x_partner * other_i),
-// own_i = gamma_i c_i, other_i = -+ gamma_partner s_i (once per token), so that
-// a row costs one exchange of its raw values and three operations per value.
+// own_i = gamma_i c_i, other_i = -+ gamma_partner s_i (once per token). Lanes hold
+// the columns so that partners meet in one lane, and a row costs three
+// operations per value beside its mean.
 template <typename T, int G, int kTurn>
 __device__ __forceinline__ void rows_of(const T* src, int64_t src_head, T* dst, int64_t dst_head,
                                         int h0, int h1, const float* gamma,
@@ -181,10 +185,10 @@ __device__ __forceinline__ void rows_of(const T* src, int64_t src_head, T* dst, 
   const int lane = threadIdx.x & 31, c = lane % G, sub = lane / G;
   const bool column = c * 8 < d;
   const float inv_d = 1.0f / (float)d;
-  dst += (h0 + sub) * dst_head + c * 8;
-  const int64_t dst_step = kAtOnce * dst_head;
   const int half = rot.rotary_dim / 2;
-  const int partner = (c * 8 < half ? c + half / 8 : c - half / 8) & (G - 1);  // kLanes
+  const Columns col = columns_of<kTurn>(c, half);
+  dst += (h0 + sub) * dst_head + col.first;
+  const int64_t dst_step = kAtOnce * dst_head;
 
   float own[8], other[8];
   uint32_t in = 0;  // columns that are rotated
@@ -201,71 +205,78 @@ __device__ __forceinline__ void rows_of(const T* src, int64_t src_head, T* dst, 
       for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       inv = rsqrtf(sum * inv_d + rot.eps);
     }
-    if constexpr (kTurn == kWithin) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-    } else if constexpr (kTurn == kLanes) {
-      r.from_lane(lane - c + partner).widen(y);
-    } else if constexpr (kTurn == kAcross) {
+    if constexpr (kTurn == kAcross) {
       __syncwarp();
       store8(stage + lane * 8, x);
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int col = c * 8 + i;
-        y[i] = in >> i & 1 ? stage[(lane - c) * 8 + (col < half ? col + half : col - half)] : 0.f;
-      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= own[i];
-    if constexpr (kTurn == kLanes) {  // a lane's columns are rotated all or none
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (kTurn == kWithin) {
+        y[i] = x[i ^ 1];
+      } else if constexpr (kTurn == kHalves) {
+        y[i] = x[i ^ 4];
+      } else if constexpr (kTurn == kAcross) {
+        const int at = c * 8 + i;
+        y[i] = in >> i & 1 ? stage[(lane - c) * 8 + (at < half ? at + half : at - half)] : 0.f;
+      }
+    }
+    float z[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = x[i] * own[i];
+    if constexpr (kTurn == kHalves) {  // a lane's columns are rotated all or none
       if (in)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += y[i] * other[i];
+        for (int i = 0; i < 8; ++i) z[i] += y[i] * other[i];
     } else if constexpr (kTurn != kNone) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (in >> i & 1) x[i] += y[i] * other[i];
+        if (in >> i & 1) z[i] += y[i] * other[i];
     }
     if (gamma)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= inv;
-    if (live) store8(to, x);
+      for (int i = 0; i < 8; ++i) z[i] *= inv;
+    if (live) {
+      store4(to, z);
+      store4(to + col.second, z + 4);
+    }
   };
   for (int hb = h0; hb < h1; hb += kAtOnce * kAhead<T>) {
-    if (!fetched) fetch_rows<T, G>(src, src_head, hb, h1, d, raw);
+    if (!fetched) fetch_rows<T, G>(src, src_head, hb, h1, column, col, raw);
     fetched = false;
     if (!ready) {  // behind the first rows' loads
       ready = true;
 #pragma unroll
       for (int i = 0; i < 8; ++i) own[i] = 1.f, other[i] = 0.f;
-      if (gamma && column) load8(gamma + c * 8, own);
-      if (kTurn != kNone && column && c * 8 < 2 * half) {
+      if (gamma && column) {
+        const float4 a = *reinterpret_cast<const float4*>(gamma + col.first);
+        const float4 b = *reinterpret_cast<const float4*>(gamma + col.first + col.second);
+        own[0] = a.x; own[1] = a.y; own[2] = a.z; own[3] = a.w;
+        own[4] = b.x; own[5] = b.y; own[6] = b.z; own[7] = b.w;
+      }
+      if (kTurn != kNone && column && col.first < 2 * half) {
         const float* cs = rot.cos + pos * rot.table_stride;
         const float* sn = rot.sin + pos * rot.table_stride;
-        if constexpr (kTurn == kLanes) {
-          float co[8], si[8], g[8];
-          const int first = c * 8 < half ? c * 8 : c * 8 - half;
-          const bool vector = rot.table_stride % 4 == 0 && aligned16(rot.cos) && aligned16(rot.sin);
-          table8(cs + first, vector, co);
-          table8(sn + first, vector, si);
-          in = 0xff;
-          if (gamma) load8(gamma + partner * 8, g);
-          else
+        if constexpr (kTurn == kHalves) {
+          if (c * 4 < half) {
+            in = 0xff;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = 1.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) other[i] = (c * 8 < half ? -si[i] : si[i]) * g[i];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) own[i] *= co[i];
+            for (int i = 0; i < 4; ++i) {
+              const float co = cs[c * 4 + i], si = sn[c * 4 + i];
+              other[i] = -si * own[i + 4];
+              other[i + 4] = si * own[i];
+              own[i] *= co;
+              own[i + 4] *= co;
+            }
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int col = c * 8 + i;
-            const bool second = kTurn == kWithin ? i & 1 : col >= half;
-            const int pair = kTurn == kWithin ? col >> 1 : second ? col - half : col;
-            const int to = kTurn == kWithin ? col ^ 1 : second ? col - half : col + half;
-            if (col < 2 * half) {
+            const int at = c * 8 + i;
+            const bool second = kTurn == kWithin ? i & 1 : at >= half;
+            const int pair = kTurn == kWithin ? at >> 1 : second ? at - half : at;
+            const int to = kTurn == kWithin ? at ^ 1 : second ? at - half : at + half;
+            if (at < 2 * half) {
               in |= 1u << i;
               own[i] *= cs[pair];
               other[i] = (second ? sn[pair] : -sn[pair]) * (gamma ? gamma[to] : 1.f);
@@ -312,7 +323,8 @@ __global__ void __launch_bounds__(256, 3)
     const Heads& s = begin_kind ? r.k : r.q;
     const int before = begin_kind ? r.q.heads : 0;
     fetch_rows<T, G>(reinterpret_cast<const T*>(s.src) + t * s.src_token, s.src_head,
-                     first - before, min(last - before, s.heads), r.d, raw);
+                     first - before, min(last - before, s.heads), c * 8 < r.d,
+                     columns_of<kTurn>(c, r.rot.rotary_dim / 2), raw);
   }
   int64_t pos = t, b = t;
   int page = 0;
@@ -366,33 +378,29 @@ __global__ void __launch_bounds__(256, 3)
   if (c * 8 < r.d)
 #pragma unroll 4
     for (int h = max(first - before, 0) + sub; h < min(last - before, r.v.heads); h += 32 / G) {
-      Raw8<T> raw;
-      raw.load(src + h * r.v.src_head);
-      raw.store(dst + h * kv.v_head_stride);
+      const uint4* from = reinterpret_cast<const uint4*>(src + h * r.v.src_head);
+      uint4* to = reinterpret_cast<uint4*>(dst + h * kv.v_head_stride);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) to[i] = from[i];
     }
 }
-
-#ifndef SPREAD
-#define SPREAD 1
-#endif
-constexpr int kSpread = SPREAD;
 
 template <typename T, int G>
 void launch_rows_of(const RowArgs& r, cudaStream_t st) {
   const int heads = r.q.heads + r.k.heads + r.v.heads;
-  // Heads of a token per warp: what spreads the rows over four times the warps
-  // that the SMs hold (24 each), so that the last ones leave no SM idle for
-  // long and a decode step's few tokens do not wait for one another.
+  // Heads of a token per warp: what spreads the rows over the warps that the SMs
+  // hold (24 each), so that a decode step's few tokens do not wait for one
+  // another and what a token costs is paid once where there are many.
   const int unit = 32 / G;  // heads that a warp takes at once
-  const int64_t spread = (int64_t)148 * 24 * kSpread;
-  int per_warp = (int)((r.tokens * heads + spread - 1) / spread);
+  int per_warp = (int)((r.tokens * heads + 148 * 24 - 1) / (148 * 24));
   per_warp = std::min((per_warp + unit - 1) / unit * unit, (heads + unit - 1) / unit * unit);
   const int blocks = (heads + per_warp - 1) / per_warp;
+  per_warp = ((heads + blocks - 1) / blocks + unit - 1) / unit * unit;  // alike
   const int64_t warps = r.tokens * blocks;
   const int64_t grid = (warps + 7) / 8;
   IDEV_CHECK_ARG(grid <= INT32_MAX, "too many tokens in one call");
   auto* kernel = r.turn == kNone    ? rows_kernel<T, G, kNone>
-                 : r.turn == kLanes  ? rows_kernel<T, G, kLanes>
+                 : r.turn == kHalves ? rows_kernel<T, G, kHalves>
                  : r.turn == kWithin ? rows_kernel<T, G, kWithin>
                                      : rows_kernel<T, G, kAcross>;
   launch_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, st, r, per_warp, blocks, warps);
@@ -428,7 +436,7 @@ void set_rotary(RowArgs& r, const InfercHeadRotary* rot, const char* op) {
   r.rot = *rot;
   r.turn = rot->rotary_dim == 0       ? kNone
            : rot->interleaved         ? kWithin
-           : rot->rotary_dim % 16 == 0 ? kLanes
+           : rot->rotary_dim % 8 == 0  ? kHalves
                                        : kAcross;
 }
 
