@@ -358,9 +358,9 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
   g.block = block_of(g.group);
   g.blocks = (g.group + g.block - 1) / g.block;
   g.capacity = (kv.max_pages * kv.page_size + 3) / 4 * 4;
-  const Shape shape = kv.dtype == F32   ? shape_of<float>(kv.head_dim)
-                      : kv.dtype == F16 ? shape_of<__half>(kv.head_dim)
-                                        : shape_of<__nv_bfloat16>(kv.head_dim);
+  const Shape shape = kv.dtype == F32   ? shape_of<float>(kv.head_dim, g.group)
+                      : kv.dtype == F16 ? shape_of<__half>(kv.head_dim, g.group)
+                                        : shape_of<__nv_bfloat16>(kv.head_dim, g.group);
   g.tile = shape.tile;
   const int64_t tiles = (g.capacity + g.tile - 1) / g.tile;
   const int64_t most = kv.batch * kv.kv_heads * g.blocks * tiles;

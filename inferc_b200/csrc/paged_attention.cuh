@@ -217,6 +217,417 @@ struct Cursor {
   }
 };
 
+// Everything that one warp holds of a (sequence, head block) between tiles, on
+// tensor instructions: S^T = K Q^T, softmax, O^T += V^T P for kCols blocks of 8
+// query heads. `d` and the place of rows in a slot are as in Layout.
+template <typename T, int kDim, int kCols>
+struct TensorHeads {
+  using L = Layout<T, kDim>;
+  static constexpr bool kWide = L::kWide;
+  static constexpr int kSubs = L::kTile / kBox;
+  static constexpr int kKSteps = kWide ? kDim / 8 : kDim / 16;  // steps along head_dim
+  static constexpr int kMTiles = kDim / 16;                     // blocks of 16 columns of V
+  static constexpr int kPartFloats = kCols * 8 * kDim;
+  static constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
+  // fp32 queries are split once where their pieces fit the registers
+  static constexpr bool kSplitOnce = kWide && kDim * kCols <= 128;
+  uint32_t qf[kCols][kKSteps][kSplitOnce ? 4 : 2];
+  float o[kCols][kMTiles][4];
+  float m[kCols][2], l[kCols][2];
+  float sc[kSubs][kCols][4];  // of 16 positions gid and gid + 8, of 8 heads 2 tig and 2 tig + 1
+
+  __device__ __forceinline__ static int gid() { return (threadIdx.x & 31) >> 2; }
+  __device__ __forceinline__ static int tig() { return threadIdx.x & 3; }
+
+  __device__ __forceinline__ void begin(const T* q, int64_t q_head, int cols, int d) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int h = c * 8 + gid();
+      const T* row = q + (int64_t)h * q_head;
+#pragma unroll
+      for (int s = 0; s < kKSteps; ++s) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int col = kWide ? s * 8 + tig() + 4 * i : s * 16 + tig() * 2 + 8 * i;
+          const bool in = h < cols && col < d;
+          uint32_t x = 0;
+          if (in) x = *reinterpret_cast<const uint32_t*>(row + col);
+          if constexpr (kSplitOnce) split_tf32(__uint_as_float(x), qf[c][s][i], qf[c][s][2 + i]);
+          else qf[c][s][i] = x;
+        }
+      }
+      m[c][0] = m[c][1] = -INFINITY;
+      l[c][0] = l[c][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMTiles; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void scores(const unsigned char* slot, float scale) {
+    const int lane = threadIdx.x & 31;
+    // ldmatrix: row and 16-byte piece of this lane, swizzled; the step's bits of the piece are
+    // xored in
+    const uint32_t k_addr = smem_addr(slot) + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128 +
+                            (((lane >> 4) ^ (lane & 7)) << 4);
+    // two chains of products, so that one need not wait for the one before
+    float acc[kSubs][kCols][2][4] = {};
+#pragma unroll
+    for (int s = 0; s < kKSteps; ++s) {
+      uint32_t qs[kCols][4];
+      if constexpr (kWide) {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if constexpr (kSplitOnce) {
+              qs[c][i] = qf[c][s][i];
+              qs[c][2 + i] = qf[c][s][2 + i];
+            } else {
+              split_tf32(__uint_as_float(qf[c][s][i]), qs[c][i], qs[c][2 + i]);
+            }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u) {
+        uint32_t a[4];
+        ldmatrix4((k_addr ^ ((s & 3) << 5)) + (s >> 2) * L::kColumn + u * kBox * 128, a);
+        if constexpr (!kWide) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            mma16<T>(acc[u][c][s & 1], a, qf[c][s][0], qf[c][s][1]);
+        } else {
+          uint32_t big[4], small[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) cut_tf32(a[i], big[i], small[i]);
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            mma_tf32(acc[u][c][1], small, qs[c][0], qs[c][1]);
+            mma_tf32(acc[u][c][0], big, qs[c][0], qs[c][1]);
+            mma_tf32(acc[u][c][1], big, qs[c][2], qs[c][3]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[u][c][i] = (acc[u][c][0][i] + acc[u][c][1][i]) * scale;
+  }
+
+  // Rows without a bit in the mask are left out.
+  __device__ __forceinline__ void leave_out(uint32_t mask) {
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(mask >> (u * kBox + gid() + (i >> 1) * 8) & 1))
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) sc[u][c][i] = -INFINITY;
+  }
+
+  // The scores of `left` positions to `to` (row of the first head), `stride` apart.
+  __device__ __forceinline__ void write_scores(float* to0, int64_t stride, int cols, int left) {
+    to0 += tig() * 2 * stride + gid();
+    left -= gid();
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (c * 8 + tig() * 2 + i >= cols) continue;
+        float* to = to0 + (c * 8 + i) * stride;
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) {
+          if (left > u * kBox) to[u * kBox] = sc[u][c][i];
+          if (left > u * kBox + 8) to[u * kBox + 8] = sc[u][c][i + 2];
+        }
+      }
+  }
+
+  __device__ __forceinline__ void softmax() {
+    float top[kCols][2];
+    bool grew = false;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = fmaxf(sc[0][c][i], sc[0][c][i + 2]);
+#pragma unroll
+        for (int u = 1; u < kSubs; ++u) x = fmaxf(x, fmaxf(sc[u][c][i], sc[u][c][i + 2]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        top[c][i] = x - kLift;
+        grew |= top[c][i] > m[c][i];
+      }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        float keep[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float to = fmaxf(m[c][i], top[c][i]);
+          keep[i] = to == -INFINITY ? 1.f : ex2(m[c][i] - to);
+          m[c][i] = to;
+          l[c][i] *= keep[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kMTiles; ++i) {
+          o[c][i][0] *= keep[0];
+          o[c][i][1] *= keep[1];
+          o[c][i][2] *= keep[0];
+          o[c][i][3] *= keep[1];
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float base = m[c][i] == -INFINITY ? 0.f : m[c][i];
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) {
+          sc[u][c][i] = ex2(sc[u][c][i] - base);
+          sc[u][c][i + 2] = ex2(sc[u][c][i + 2] - base);
+          l[c][i] += sc[u][c][i] + sc[u][c][i + 2];
+        }
+      }
+  }
+
+  __device__ __forceinline__ void values(const unsigned char* slot) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (!kWide) {
+      const uint32_t v_addr = smem_addr(slot) + ((lane & 7) + (lane >> 4) * 8) * 128 +
+                              ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+      uint32_t hi[kSubs][kCols][2], lo[kSubs][kCols][2];
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            split_pair16<T>(sc[u][c][2 * i], sc[u][c][2 * i + 1], hi[u][c][i], lo[u][c][i]);
+            hi[u][c][i] = transpose8x8(hi[u][c][i]);
+            lo[u][c][i] = transpose8x8(lo[u][c][i]);
+          }
+#pragma unroll
+      for (int i = 0; i < kMTiles; ++i)
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) {
+          uint32_t a[4];
+          ldmatrix4_trans((v_addr ^ ((i & 3) << 5)) + (i >> 2) * L::kColumn + u * kBox * 128, a);
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, lo[u][c][0], lo[u][c][1]);
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, hi[u][c][0], hi[u][c][1]);
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // P of positions (2 tig, 2 tig + 1) of these 8, head gid, from the lanes that hold them
+          uint32_t big_p[kCols][2], small_p[kCols][2];
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int src = (tig() * 2 + i) * 4 + (gid() >> 1);
+              const float x = __shfl_sync(0xffffffffu, sc[u][c][2 * half], src);
+              const float y = __shfl_sync(0xffffffffu, sc[u][c][2 * half + 1], src);
+              split_tf32(gid() & 1 ? y : x, big_p[c][i], small_p[c][i]);
+            }
+          const unsigned char* r0 =
+              slot + (u * kBox + half * 8 + tig() * 2) * 128 + ((gid() ^ (tig() * 2)) << 4);
+          const unsigned char* r1 =
+              slot + (u * kBox + half * 8 + tig() * 2 + 1) * 128 + ((gid() ^ (tig() * 2 + 1)) << 4);
+#pragma unroll
+          for (int i = 0; i < kMTiles; i += 2) {
+            const uint4 x = *reinterpret_cast<const uint4*>(r0 + (i >> 1) * L::kColumn);
+            const uint4 y = *reinterpret_cast<const uint4*>(r1 + (i >> 1) * L::kColumn);
+            uint32_t big[2][4], small[2][4];
+            cut_tf32(x.x, big[0][0], small[0][0]);
+            cut_tf32(x.y, big[0][1], small[0][1]);
+            cut_tf32(y.x, big[0][2], small[0][2]);
+            cut_tf32(y.y, big[0][3], small[0][3]);
+            cut_tf32(x.z, big[1][0], small[1][0]);
+            cut_tf32(x.w, big[1][1], small[1][1]);
+            cut_tf32(y.z, big[1][2], small[1][2]);
+            cut_tf32(y.w, big[1][3], small[1][3]);
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) {
+                mma_tf32(o[c][i + v], small[v], big_p[c][0], big_p[c][1]);
+                mma_tf32(o[c][i + v], big[v], small_p[c][0], small_p[c][1]);
+                mma_tf32(o[c][i + v], big[v], big_p[c][0], big_p[c][1]);
+              }
+          }
+        }
+    }
+  }
+
+  // Passes (head, maximum, sum) once per head, then (head, column, value) of the
+  // lane's unnormalised output; the sums are the warp's.
+  template <typename Head, typename Value>
+  __device__ __forceinline__ void end(int cols, int d, Head&& head, Value&& value) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = l[c][i];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int h = c * 8 + tig() * 2 + i;
+        if (h >= cols) continue;
+        if (gid() == 0) head(h, m[c][i], x);
+        const float inv = x == 0.f ? 0.f : 1.f / x;  // 0: every page was bad
+#pragma unroll
+        for (int j = 0; j < kMTiles; ++j)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int col = kWide ? (j >> 1) * 32 + gid() * 4 + (j & 1) * 2 + half
+                                  : j * 16 + half * 8 + gid();
+            if (col < d) value(h, col, o[c][j][2 * half + i], inv);
+          }
+      }
+  }
+};
+
+// The same for one fp32 query head per key head, on the CUDA cores: the matrix
+// instruction would use one of its 8 columns, and three of them per product, plus
+// the splitting of K and V, are over twice the instructions (32 x 12 heads of 64,
+// 100 MB: XX us against 36 us). A lane takes a position of the tile (half of its
+// columns where the tile has 16 positions) for the scores, and kDim / 32 columns
+// for the values; P passes through shared memory. Two fp32 operations per
+// instruction (fma.rn.f32x2).
+template <int kDim>
+struct OneHead {
+  using L = Layout<float, kDim>;
+  static constexpr int kTile = L::kTile, kSplit = 32 / kTile;
+  static constexpr int kQuads = kDim / kSplit / 4;  // float4s of a row that a lane multiplies
+  static constexpr int kMine = kDim / 32;           // output columns of a lane: 2 or 4
+  static constexpr int kPartFloats = kDim;
+  unsigned long long q[kQuads][2], o[kMine / 2];
+  float m, l, s;
+
+  __device__ __forceinline__ static unsigned long long pack(float a, float b) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+  }
+  __device__ __forceinline__ static float2 unpack(unsigned long long v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+  __device__ __forceinline__ static unsigned long long fma2(unsigned long long a,
+                                                            unsigned long long b,
+                                                            unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+  }
+
+  __device__ __forceinline__ void begin(const float* row, int64_t, int, int d) {
+    const int first = (threadIdx.x & 31) / kTile * (kDim / kSplit);
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (first + 4 * i < d) x = *reinterpret_cast<const float4*>(row + first + 4 * i);
+      q[i][0] = pack(x.x, x.y);
+      q[i][1] = pack(x.z, x.w);
+    }
+#pragma unroll
+    for (int i = 0; i < kMine / 2; ++i) o[i] = 0;
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  __device__ __forceinline__ void scores(const unsigned char* slot, float scale) {
+    const int lane = threadIdx.x & 31, row = lane % kTile;
+    const int first = lane / kTile * kQuads;  // 16-byte piece of the row
+    unsigned long long a = 0, b = 0;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int piece = first + i;
+      const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(
+          slot + (piece >> 3) * L::kColumn + row * 128 + (((piece ^ row) & 7) << 4));
+      a = fma2(q[i][0], k.x, a);
+      b = fma2(q[i][1], k.y, b);
+    }
+    const float2 x = unpack(a), y = unpack(b);
+    s = (x.x + x.y) + (y.x + y.y);
+    if constexpr (kSplit == 2) s += __shfl_xor_sync(0xffffffffu, s, 16);
+    s *= scale;
+  }
+
+  __device__ __forceinline__ void leave_out(uint32_t mask) {
+    if (!(mask >> (threadIdx.x % kTile) & 1)) s = -INFINITY;
+  }
+
+  __device__ __forceinline__ void write_scores(float* to, int64_t, int, int left) {
+    const int lane = threadIdx.x & 31;
+    if (lane < kTile && lane < left) to[lane] = s;
+  }
+
+  __device__ __forceinline__ void softmax() {
+    const float top = fmaxf(m, warp_max(s));
+    if (top > m) {  // the same in every lane
+      const float keep = ex2(m - top);
+      m = top;
+      l *= keep;
+      const unsigned long long k2 = pack(keep, keep);
+#pragma unroll
+      for (int i = 0; i < kMine / 2; ++i) o[i] = fma2(o[i], k2, 0);
+    }
+    s = ex2(s - (m == -INFINITY ? 0.f : m));
+    if ((threadIdx.x & 31) < kTile) l += s;
+  }
+
+  __device__ __forceinline__ void values(const unsigned char* slot) {
+    __shared__ __align__(16) float2 s_p[kWarps][kTile];
+    const int lane = threadIdx.x & 31;
+    float2* p = s_p[threadIdx.x >> 5];
+    if (lane < kTile) p[lane] = make_float2(s, s);
+    __syncwarp();
+    const int piece = lane * kMine / 4, inside = lane * kMine % 4 * 4;
+    const unsigned char* column = slot + (piece >> 3) * L::kColumn + inside;
+#pragma unroll
+    for (int j = 0; j < kTile; j += 2) {
+      const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(p + j);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const unsigned char* at = column + (j + u) * 128 + (((piece ^ (j + u)) & 7) << 4);
+        const unsigned long long w = u ? pp.y : pp.x;
+        if constexpr (kMine == 4) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(at);
+          o[0] = fma2(w, v.x, o[0]);
+          o[kMine / 2 - 1] = fma2(w, v.y, o[kMine / 2 - 1]);
+        } else {
+          o[0] = fma2(w, *reinterpret_cast<const unsigned long long*>(at), o[0]);
+        }
+      }
+    }
+  }
+
+  template <typename Head, typename Value>
+  __device__ __forceinline__ void end(int, int d, Head&& head, Value&& value) {
+    const int lane = threadIdx.x & 31;
+    const float x = warp_sum(l), inv = x == 0.f ? 0.f : 1.f / x;  // 0: every page was bad
+    if (lane == 0) head(0, m, x);
+#pragma unroll
+    for (int i = 0; i < kMine / 2; ++i) {
+      const float2 v = unpack(o[i]);
+      const int col = lane * kMine + 2 * i;
+      if (col < d) value(0, col, v.x, inv);
+      if (col + 1 < d) value(0, col + 1, v.y, inv);
+    }
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void zero_heads(const AttendArgs& g, int64_t b, int h0, int h1) {
   const int pieces = g.a.kv.head_dim / 8;
@@ -281,12 +692,11 @@ __device__ __forceinline__ void join_whole(const AttendArgs& g, int b, int hk, i
   }
 }
 
-template <typename T, int kDim, int kCols, bool kTma>
+template <typename T, int kDim, typename Heads, bool kTma>
 __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     attend_kernel(const __grid_constant__ AttendArgs g, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map) {
   using L = Layout<T, kDim>;
-  constexpr bool kWide = L::kWide;
   constexpr int kElem = sizeof(T), kThreads = kWarps * 32, kTile = L::kTile;
   constexpr int kSubs = kTile / kBox;
   extern __shared__ unsigned char smem_raw[];
@@ -297,7 +707,6 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
   __shared__ float2 s_ml[kWarps * 16];  // g.whole: each warp's maxima and sums
   const InfercPagedKv& kv = g.a.kv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int gid = lane >> 2, tig = lane & 3;
   const int heads = (int)kv.kv_heads * g.blocks;
   const int batch = (int)kv.batch;
   const int d = kv.head_dim;
@@ -578,25 +987,12 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
 
   // g.whole: a warp's part, [head][head_dim], takes its ring's memory once all loads have arrived
   constexpr int kPart = L::kSlots * L::kSlot / 4;
-  static_assert(kPart >= kCols * 8 * kDim, "a part fits a ring");
+  static_assert(kPart >= Heads::kPartFloats, "a part fits a ring");
 
-  // ---- the state of one (sequence, head block)
-  constexpr int kKSteps = kWide ? kDim / 8 : kDim / 16;  // steps along head_dim
-  constexpr int kMTiles = kDim / 16;                     // blocks of 16 columns of V
-  constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
-  // fp32 queries are split once where their pieces fit the registers
-  constexpr bool kSplitOnce = kWide && kDim * kCols <= 128;
-  uint32_t qf[kCols][kKSteps][kSplitOnce ? 4 : 2];
-  float o[kCols][kMTiles][4];
-  float m[kCols][2], l[kCols][2];
+  Heads heads_of;  // the state of one (sequence, head block)
   bool begins = false;
   int q0 = 0, cols = 0;
-  // ldmatrix places: row and 16-byte piece of this lane, swizzled; the step's
-  // bits of the piece are xored in
-  const uint32_t k_place = ((lane & 7) + ((lane >> 3) & 1) * 8) * 128 +
-                           (((lane >> 4) ^ (lane & 7)) << 4);
-  const uint32_t v_place = ((lane & 7) + (lane >> 4) * 8) * 128 +
-                           ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  constexpr uint32_t kAll = kTile == 32 ? 0xffffffffu : (1u << (kTile & 31)) - 1;
 
   int t = 0;
 #pragma unroll 1
@@ -605,167 +1001,29 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       begins = use.tile == 0;
       q0 = use.hk * g.group + use.block * g.block;
       cols = min(g.block, (use.hk + 1) * g.group - q0);
-      const T* q = reinterpret_cast<const T*>(g.q) + use.b * g.q_batch + q0 * g.q_head;
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const int h = c * 8 + gid;
-        const T* row = q + (int64_t)h * g.q_head;
-#pragma unroll
-        for (int s = 0; s < kKSteps; ++s) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int col = kWide ? s * 8 + tig + 4 * i : s * 16 + tig * 2 + 8 * i;
-            const bool in = h < cols && col < d;
-            uint32_t x = 0;
-            if (in) x = *reinterpret_cast<const uint32_t*>(row + col);
-            if constexpr (kSplitOnce) split_tf32(__uint_as_float(x), qf[c][s][i], qf[c][s][2 + i]);
-            else qf[c][s][i] = x;
-          }
-        }
-        m[c][0] = m[c][1] = -INFINITY;
-        l[c][0] = l[c][1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kMTiles; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
-      }
+      heads_of.begin(reinterpret_cast<const T*>(g.q) + use.b * g.q_batch + q0 * g.q_head, g.q_head,
+                     cols, d);
     }
 
-    // ---- scores
     if (!wait()) break;
     const uint32_t mask = masks[slot_out];
-    float sc[kSubs][kCols][4];
-    {
-      const uint32_t k_addr = ring_addr + slot_out * L::kSlot + k_place;
-      // two chains of products, so that one need not wait for the one before
-      float acc[kSubs][kCols][2][4] = {};
-#pragma unroll
-      for (int s = 0; s < kKSteps; ++s) {
-        uint32_t qs[kCols][4];
-        if constexpr (kWide) {
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              if constexpr (kSplitOnce) {
-                qs[c][i] = qf[c][s][i];
-                qs[c][2 + i] = qf[c][s][2 + i];
-              } else {
-                split_tf32(__uint_as_float(qf[c][s][i]), qs[c][i], qs[c][2 + i]);
-              }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u) {
-          uint32_t a[4];
-          ldmatrix4((k_addr ^ ((s & 3) << 5)) + (s >> 2) * L::kColumn + u * kBox * 128, a);
-          if constexpr (!kWide) {
-#pragma unroll
-            for (int c = 0; c < kCols; ++c)
-              mma16<T>(acc[u][c][s & 1], a, qf[c][s][0], qf[c][s][1]);
-          } else {
-            uint32_t big[4], small[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) cut_tf32(a[i], big[i], small[i]);
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              mma_tf32(acc[u][c][1], small, qs[c][0], qs[c][1]);
-              mma_tf32(acc[u][c][0], big, qs[c][0], qs[c][1]);
-              mma_tf32(acc[u][c][1], big, qs[c][2], qs[c][3]);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sc[u][c][i] = (acc[u][c][0][i] + acc[u][c][1][i]) * g.scale;
-    }
+    heads_of.scores(ring + slot_out * L::kSlot, g.scale);
     __syncwarp();
     if constexpr (L::kSlots % 2 == 0) fill_k();
     else fill_v();
     released();
 
-    // ---- softmax: of 16 positions gid and gid + 8, of 8 heads 2 tig and 2 tig + 1
-    if (mask != (kTile == 32 ? 0xffffffffu : 0xffffu)) {
-#pragma unroll
-      for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(mask >> (u * kBox + gid + (i >> 1) * 8) & 1))
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) sc[u][c][i] = -INFINITY;
-    }
-    if (g.scores) {
-      const int left = use.len - use.tile * kTile - gid;  // positions from this lane's on
-      float* to0 = g.scores + (use.b * (int64_t)(kv.kv_heads * g.group) + q0 + tig * 2) *
-                                  g.capacity + use.tile * kTile + gid;
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (c * 8 + tig * 2 + i >= cols) continue;
-          float* to = to0 + (c * 8 + i) * g.capacity;
-#pragma unroll
-          for (int u = 0; u < kSubs; ++u) {
-            if (left > u * kBox) to[u * kBox] = sc[u][c][i];
-            if (left > u * kBox + 8) to[u * kBox + 8] = sc[u][c][i + 2];
-          }
-        }
-    }
-    float top[kCols][2];
-    bool grew = false;
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x = fmaxf(sc[0][c][i], sc[0][c][i + 2]);
-#pragma unroll
-        for (int u = 1; u < kSubs; ++u) x = fmaxf(x, fmaxf(sc[u][c][i], sc[u][c][i + 2]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        top[c][i] = x - kLift;
-        grew |= top[c][i] > m[c][i];
-      }
-    if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        float keep[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float to = fmaxf(m[c][i], top[c][i]);
-          keep[i] = to == -INFINITY ? 1.f : ex2(m[c][i] - to);
-          m[c][i] = to;
-          l[c][i] *= keep[i];
-        }
-#pragma unroll
-        for (int i = 0; i < kMTiles; ++i) {
-          o[c][i][0] *= keep[0];
-          o[c][i][1] *= keep[1];
-          o[c][i][2] *= keep[0];
-          o[c][i][3] *= keep[1];
-        }
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float base = m[c][i] == -INFINITY ? 0.f : m[c][i];
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u) {
-          sc[u][c][i] = ex2(sc[u][c][i] - base);
-          sc[u][c][i + 2] = ex2(sc[u][c][i + 2] - base);
-          l[c][i] += sc[u][c][i] + sc[u][c][i + 2];
-        }
-      }
+    if (mask != kAll) heads_of.leave_out(mask);
+    if (g.scores)
+      heads_of.write_scores(
+          g.scores + (use.b * (int64_t)(kv.kv_heads * g.group) + q0) * g.capacity +
+              use.tile * kTile,
+          g.capacity, cols, use.len - use.tile * kTile);
+    heads_of.softmax();
 
-    // ---- values
     if (!wait()) break;
     unsigned char* v_ptr = ring + slot_out * L::kSlot;
-    if (kTma && mask != (kTile == 32 ? 0xffffffffu : 0xffffu)) {  // rows that do not exist
+    if (kTma && mask != kAll) {  // rows that do not exist
 #pragma unroll
       for (int i = 0; i < L::kSlot / 512; ++i) {
         const int to = i * 512 + lane * 16;
@@ -775,80 +1033,13 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       tc::fence_proxy_async();  // before TMA writes here again
       __syncwarp();
     }
-    if constexpr (!kWide) {
-      const uint32_t v_addr = ring_addr + slot_out * L::kSlot + v_place;
-      uint32_t hi[kSubs][kCols][2], lo[kSubs][kCols][2];
-#pragma unroll
-      for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            split_pair16<T>(sc[u][c][2 * i], sc[u][c][2 * i + 1], hi[u][c][i], lo[u][c][i]);
-            hi[u][c][i] = transpose8x8(hi[u][c][i]);
-            lo[u][c][i] = transpose8x8(lo[u][c][i]);
-          }
-#pragma unroll
-      for (int i = 0; i < kMTiles; ++i)
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u) {
-          uint32_t a[4];
-          ldmatrix4_trans((v_addr ^ ((i & 3) << 5)) + (i >> 2) * L::kColumn + u * kBox * 128, a);
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, lo[u][c][0], lo[u][c][1]);
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, hi[u][c][0], hi[u][c][1]);
-        }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // P of positions (2 tig, 2 tig + 1) of these 8, head gid, from the lanes that hold them
-          uint32_t big_p[kCols][2], small_p[kCols][2];
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int src = (tig * 2 + i) * 4 + (gid >> 1);
-              const float x = __shfl_sync(0xffffffffu, sc[u][c][2 * half], src);
-              const float y = __shfl_sync(0xffffffffu, sc[u][c][2 * half + 1], src);
-              split_tf32(gid & 1 ? y : x, big_p[c][i], small_p[c][i]);
-            }
-          const unsigned char* r0 =
-              v_ptr + (u * kBox + half * 8 + tig * 2) * 128 + ((gid ^ (tig * 2)) << 4);
-          const unsigned char* r1 =
-              v_ptr + (u * kBox + half * 8 + tig * 2 + 1) * 128 + ((gid ^ (tig * 2 + 1)) << 4);
-#pragma unroll
-          for (int i = 0; i < kMTiles; i += 2) {
-            const uint4 x = *reinterpret_cast<const uint4*>(r0 + (i >> 1) * L::kColumn);
-            const uint4 y = *reinterpret_cast<const uint4*>(r1 + (i >> 1) * L::kColumn);
-            uint32_t big[2][4], small[2][4];
-            cut_tf32(x.x, big[0][0], small[0][0]);
-            cut_tf32(x.y, big[0][1], small[0][1]);
-            cut_tf32(y.x, big[0][2], small[0][2]);
-            cut_tf32(y.y, big[0][3], small[0][3]);
-            cut_tf32(x.z, big[1][0], small[1][0]);
-            cut_tf32(x.w, big[1][1], small[1][1]);
-            cut_tf32(y.z, big[1][2], small[1][2]);
-            cut_tf32(y.w, big[1][3], small[1][3]);
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-#pragma unroll
-              for (int c = 0; c < kCols; ++c) {
-                mma_tf32(o[c][i + v], small[v], big_p[c][0], big_p[c][1]);
-                mma_tf32(o[c][i + v], big[v], small_p[c][0], small_p[c][1]);
-                mma_tf32(o[c][i + v], big[v], big_p[c][0], big_p[c][1]);
-              }
-          }
-        }
-    }
+    heads_of.values(v_ptr);
     __syncwarp();
     if constexpr (L::kSlots % 2 == 0) fill_v();
     else fill_k();
     released();
 
-    // ---- the end of the sequence's head block, or of this warp's share
+    // the end of the sequence's head block, or of this warp's share
     const bool ends = use.tile + 1 == use.tiles;
     if (ends || t + 1 == count) {
       const bool whole = begins && ends && !g.whole;
@@ -858,47 +1049,25 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
         g.jobs[w] = make_int4(use.b, use.hk * g.blocks + use.block,
                               (int)(owner_of(last, total, used) - w) + 1, 0);
       }
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float x = l[c][i];
-          x += __shfl_xor_sync(0xffffffffu, x, 4);
-          x += __shfl_xor_sync(0xffffffffu, x, 8);
-          x += __shfl_xor_sync(0xffffffffu, x, 16);
-          const int h = c * 8 + tig * 2 + i;
-          const float inv = x == 0.f ? 0.f : 1.f / x;  // 0: every page was bad
-          if (h < cols) {
-            if (gid == 0) {
-              const float base = m[c][i] == -INFINITY ? 0.f : m[c][i];
-              if (g.whole) {
-                s_ml[warp * 16 + h] = make_float2(m[c][i], x);
-              } else if (!whole) {
-                g.part_ml[(part * g.block + h) * 2] = m[c][i];
-                g.part_ml[(part * g.block + h) * 2 + 1] = x;
-              } else if (g.stats) {
-                const int64_t r = use.b * (int64_t)(kv.kv_heads * g.group) + q0 + h;
-                g.stats[2 * r] = base;
-                g.stats[2 * r + 1] = inv;
-              }
+      T* out = reinterpret_cast<T*>(g.out) + use.b * g.o_batch + q0 * g.o_head;
+      float* po = g.whole ? reinterpret_cast<float*>(ring) : g.part_o + part * g.block * d;
+      heads_of.end(
+          cols, d,
+          [&](int h, float top, float sum) {
+            if (g.whole) {
+              s_ml[warp * 16 + h] = make_float2(top, sum);
+            } else if (!whole) {
+              reinterpret_cast<float2*>(g.part_ml)[part * g.block + h] = make_float2(top, sum);
+            } else if (g.stats) {
+              const int64_t r = use.b * (int64_t)(kv.kv_heads * g.group) + q0 + h;
+              reinterpret_cast<float2*>(g.stats)[r] =
+                  make_float2(top == -INFINITY ? 0.f : top, sum == 0.f ? 0.f : 1.f / sum);
             }
-            T* out = reinterpret_cast<T*>(g.out) + use.b * g.o_batch + (q0 + h) * g.o_head;
-            float* po = g.whole ? reinterpret_cast<float*>(ring) + h * d
-                                : g.part_o + (part * g.block + h) * d;
-#pragma unroll
-            for (int j = 0; j < kMTiles; ++j)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const int col = kWide ? (j >> 1) * 32 + gid * 4 + (j & 1) * 2 + half
-                                      : j * 16 + half * 8 + gid;
-                if (col < d) {
-                  if (whole) out[col] = T(o[c][j][2 * half + i] * inv);
-                  else po[col] = o[c][j][2 * half + i];
-                }
-              }
-          }
-        }
-      }
+          },
+          [&](int h, int col, float x, float inv) {
+            if (whole) out[h * g.o_head + col] = T(x * inv);
+            else po[h * d + col] = x;
+          });
     }
     use.next(g);
   }
@@ -960,15 +1129,24 @@ void launch_attend_dim(const AttendArgs& g, cudaStream_t st) {
   const unsigned grid = (unsigned)((g.warps + kWarps - 1) / kWarps);
   CUtensorMap k_map{}, v_map{};
   const bool tma = make_map<T>(g.a.kv, false, &k_map) && make_map<T>(g.a.kv, true, &v_map);
-  const bool one = g.block <= 8;
-  auto* kernel = tma ? (one ? attend_kernel<T, kDim, 1, true> : attend_kernel<T, kDim, 2, true>)
-                     : (one ? attend_kernel<T, kDim, 1, false> : attend_kernel<T, kDim, 2, false>);
+  // one head per key head in fp32, up to 8, or up to 16
+  const int kind = std::is_same_v<T, float> && kDim <= 128 && g.group == 1 ? 0 : g.block <= 8 ? 1 : 2;
+  using One = std::conditional_t<std::is_same_v<T, float> && (kDim == 64 || kDim == 128),
+                                 OneHead<kDim == 64 ? 64 : 128>, TensorHeads<T, kDim, 1>>;
+  using Eight = TensorHeads<T, kDim, 1>;
+  using Sixteen = TensorHeads<T, kDim, 2>;
+  auto* kernel = tma ? (kind == 0   ? attend_kernel<T, kDim, One, true>
+                        : kind == 1 ? attend_kernel<T, kDim, Eight, true>
+                                    : attend_kernel<T, kDim, Sixteen, true>)
+                     : (kind == 0   ? attend_kernel<T, kDim, One, false>
+                        : kind == 1 ? attend_kernel<T, kDim, Eight, false>
+                                    : attend_kernel<T, kDim, Sixteen, false>);
   // one request per kernel and device
   constexpr int kMost = 64;
-  static std::atomic<bool> ready[kMost][4];
+  static std::atomic<bool> ready[kMost][6];
   int dev = 0;
   IDEV_CUDA(cudaGetDevice(&dev));
-  std::atomic<bool>* known = dev < kMost ? &ready[dev][(tma ? 2 : 0) + (one ? 1 : 0)] : nullptr;
+  std::atomic<bool>* known = dev < kMost ? &ready[dev][(tma ? 3 : 0) + kind] : nullptr;
   if (!known || !known->load(std::memory_order_relaxed)) {
     IDEV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
     if (known) known->store(true, std::memory_order_relaxed);
@@ -976,11 +1154,17 @@ void launch_attend_dim(const AttendArgs& g, cudaStream_t st) {
   launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), L::kSmem, st, g, k_map, v_map);
 }
 
+// One fp32 head per key head runs on the CUDA cores, in rows of 64 or 128.
+template <typename T>
+constexpr bool one_head(int64_t group) {
+  return std::is_same_v<T, float> && group == 1;
+}
+
 template <typename T>
 void launch_attend_any(const AttendArgs& g, cudaStream_t st) {
   const int d = g.a.kv.head_dim;
   if (d <= 64) launch_attend_dim<T, 64>(g, st);
-  else if (d <= 96) launch_attend_dim<T, 96>(g, st);
+  else if (d <= 96 && !one_head<T>(g.group)) launch_attend_dim<T, 96>(g, st);
   else if (d <= 128) launch_attend_dim<T, 128>(g, st);
   else if (d <= 192) launch_attend_dim<T, 192>(g, st);
   else launch_attend_dim<T, 256>(g, st);
@@ -991,10 +1175,10 @@ struct Shape {
   int tile, blocks;
 };
 template <typename T>
-Shape shape_of(int d) {
+Shape shape_of(int d, int64_t group) {
   auto of = [](auto l) { return Shape{decltype(l)::kTile, decltype(l)::kBlocks}; };
   return d <= 64    ? of(Layout<T, 64>())
-         : d <= 96  ? of(Layout<T, 96>())
+         : d <= 96 && !one_head<T>(group) ? of(Layout<T, 96>())
          : d <= 128 ? of(Layout<T, 128>())
          : d <= 192 ? of(Layout<T, 192>())
                     : of(Layout<T, 256>());
