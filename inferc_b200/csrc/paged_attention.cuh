@@ -270,7 +270,7 @@ struct TensorHeads {
     const uint32_t k_addr = smem_addr(slot) + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128 +
                             (((lane >> 4) ^ (lane & 7)) << 4);
     // two chains of products, so that one need not wait for the one before
-    float acc[kSubs][kCols][2][4] = {};
+    float acc[kSubs][kCols][2][4] = {}, sum[kSubs][kCols][4] = {};
 #pragma unroll
     for (int s = 0; s < kKSteps; ++s) {
       uint32_t qs[kCols][4];
@@ -304,6 +304,7 @@ struct TensorHeads {
             mma_tf32(acc[u][c][1], small, qs[c][0], qs[c][1]);
             mma_tf32(acc[u][c][0], big, qs[c][0], qs[c][1]);
             mma_tf32(acc[u][c][1], big, qs[c][2], qs[c][3]);
+            if ((s & 3) == 3 || s + 1 == kKSteps) settle(sum[u][c], acc[u][c][0]);
           }
         }
       }
@@ -313,7 +314,19 @@ struct TensorHeads {
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[u][c][i] = (acc[u][c][0][i] + acc[u][c][1][i]) * scale;
+        for (int i = 0; i < 4; ++i)
+          sc[u][c][i] = ((kWide ? sum[u][c][i] : acc[u][c][0][i]) + acc[u][c][1][i]) * scale;
+  }
+
+  // The instruction adds to its accumulator by cutting, always towards zero: over many steps
+  // that would cost fp32 results a digit (2e-6 of an output of 1000 positions of 256 columns).
+  // So fp32 accumulators take four steps of the large products, then join a sum that is rounded.
+  __device__ __forceinline__ static void settle(float (&sum)[4], float (&acc)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum[i] += acc[i];
+      acc[i] = 0.f;
+    }
   }
 
   // Rows without a bit in the mask are left out.
@@ -423,48 +436,53 @@ struct TensorHeads {
           for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, hi[u][c][0], hi[u][c][1]);
         }
     } else {
+      constexpr int kEights = kSubs * 2;  // eight positions each
+      // P of positions (2 tig, 2 tig + 1) of each eight, head gid, from the lanes that hold them
+      uint32_t big_p[kEights][kCols][2], small_p[kEights][kCols][2];
 #pragma unroll
-      for (int u = 0; u < kSubs; ++u)
+      for (int e = 0; e < kEights; ++e)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // P of positions (2 tig, 2 tig + 1) of these 8, head gid, from the lanes that hold them
-          uint32_t big_p[kCols][2], small_p[kCols][2];
+        for (int c = 0; c < kCols; ++c)
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int src = (tig() * 2 + i) * 4 + (gid() >> 1);
-              const float x = __shfl_sync(0xffffffffu, sc[u][c][2 * half], src);
-              const float y = __shfl_sync(0xffffffffu, sc[u][c][2 * half + 1], src);
-              split_tf32(gid() & 1 ? y : x, big_p[c][i], small_p[c][i]);
-            }
-          const unsigned char* r0 =
-              slot + (u * kBox + half * 8 + tig() * 2) * 128 + ((gid() ^ (tig() * 2)) << 4);
-          const unsigned char* r1 =
-              slot + (u * kBox + half * 8 + tig() * 2 + 1) * 128 + ((gid() ^ (tig() * 2 + 1)) << 4);
-#pragma unroll
-          for (int i = 0; i < kMTiles; i += 2) {
-            const uint4 x = *reinterpret_cast<const uint4*>(r0 + (i >> 1) * L::kColumn);
-            const uint4 y = *reinterpret_cast<const uint4*>(r1 + (i >> 1) * L::kColumn);
-            uint32_t big[2][4], small[2][4];
-            cut_tf32(x.x, big[0][0], small[0][0]);
-            cut_tf32(x.y, big[0][1], small[0][1]);
-            cut_tf32(y.x, big[0][2], small[0][2]);
-            cut_tf32(y.y, big[0][3], small[0][3]);
-            cut_tf32(x.z, big[1][0], small[1][0]);
-            cut_tf32(x.w, big[1][1], small[1][1]);
-            cut_tf32(y.z, big[1][2], small[1][2]);
-            cut_tf32(y.w, big[1][3], small[1][3]);
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-#pragma unroll
-              for (int c = 0; c < kCols; ++c) {
-                mma_tf32(o[c][i + v], small[v], big_p[c][0], big_p[c][1]);
-                mma_tf32(o[c][i + v], big[v], small_p[c][0], small_p[c][1]);
-                mma_tf32(o[c][i + v], big[v], big_p[c][0], big_p[c][1]);
-              }
+          for (int i = 0; i < 2; ++i) {
+            const int src = (tig() * 2 + i) * 4 + (gid() >> 1);
+            const float x = __shfl_sync(0xffffffffu, sc[e >> 1][c][2 * (e & 1)], src);
+            const float y = __shfl_sync(0xffffffffu, sc[e >> 1][c][2 * (e & 1) + 1], src);
+            split_tf32(gid() & 1 ? y : x, big_p[e][c][i], small_p[e][c][i]);
           }
+      const unsigned char* r0 = slot + tig() * 2 * 128 + ((gid() ^ (tig() * 2)) << 4);
+      const unsigned char* r1 = slot + (tig() * 2 + 1) * 128 + ((gid() ^ (tig() * 2 + 1)) << 4);
+#pragma unroll
+      for (int i = 0; i < kMTiles; i += 2) {
+        float fresh[2][kCols][4] = {};
+#pragma unroll
+        for (int e = 0; e < kEights; ++e) {
+          const int at = (i >> 1) * L::kColumn + e * 8 * 128;
+          const uint4 x = *reinterpret_cast<const uint4*>(r0 + at);
+          const uint4 y = *reinterpret_cast<const uint4*>(r1 + at);
+          uint32_t big[2][4], small[2][4];
+          cut_tf32(x.x, big[0][0], small[0][0]);
+          cut_tf32(x.y, big[0][1], small[0][1]);
+          cut_tf32(y.x, big[0][2], small[0][2]);
+          cut_tf32(y.y, big[0][3], small[0][3]);
+          cut_tf32(x.z, big[1][0], small[1][0]);
+          cut_tf32(x.w, big[1][1], small[1][1]);
+          cut_tf32(y.z, big[1][2], small[1][2]);
+          cut_tf32(y.w, big[1][3], small[1][3]);
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              mma_tf32(fresh[v][c], small[v], big_p[e][c][0], big_p[e][c][1]);
+              mma_tf32(fresh[v][c], big[v], small_p[e][c][0], small_p[e][c][1]);
+              mma_tf32(fresh[v][c], big[v], big_p[e][c][0], big_p[e][c][1]);
+            }
         }
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) settle(o[c][i + v], fresh[v][c]);
+      }
     }
   }
 
