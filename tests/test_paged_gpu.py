@@ -10,7 +10,7 @@ result's type (finfo.eps / 2):
   products and sums in fp32: (d + 16) u relative to |a c| + |b s|;
 - attention: a score is a dot product of d terms accumulated in fp32 (one
   step, 2 u, per term where a matrix instruction truncates), with fp32
-  operands in two 11-bit pieces whose dropped part is 3 * 2^-22 of each
+  operands in two 11-bit pieces whose dropped part is at most 2^-20 of each
   product; then a scaling by two roundings and 2^x to 2^-21. So with
   S = scale * max_j sum_i |q_i k_ij| the weights are relatively off by at most
   e = 2 S ((d + 8) 2 u + 2^-20) + 2^-20, twice over because of the normaliser,
@@ -19,10 +19,17 @@ result's type (finfo.eps / 2):
   below 2^-38 vanish: n 2^-36 max|v| more.
 - a summed weight: e * p, and 2 u of the running sum per addition.
 """
+import os
+import random
+import subprocess
+import sys
+
 import pytest
 import torch
 
 from inferc_b200 import lib, ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -324,6 +331,103 @@ def test_attention(dtype, hk, group, d, page, token_major):
     got = check_attention(c, q, out=out[:, :h], repeat=True)
     assert got.data_ptr() == out.data_ptr() and (out[:, h] == 9).all()
     check_attention(c, q, weights=True, repeat=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hk,group,d,page,token_major", [
+    (1, 1, 64, 16, False), (3, 1, 96, 16, True), (2, 1, 128, 24, False), (2, 4, 128, 16, False),
+    (2, 8, 64, 48, True), (1, 16, 128, 32, False), (1, 17, 64, 16, False), (2, 3, 80, 24, True),
+    (1, 5, 256, 8, False), (1, 40, 96, 16, False), (2, 2, 8, 16, False), (1, 7, 192, 16, True),
+    (1, 12, 256, 16, False), (2, 1, 24, 16, False), (1, 9, 32, 3, False), (1, 1, 200, 16, False)])
+def test_attention_cut_among_warps(dtype, hk, group, d, page, token_major):
+    """The same lengths in a table wide enough that sequences are cut wherever
+    the warps' shares meet and joined by a second kernel."""
+    g = gen(hk * 1000 + group * 100 + d + page)
+    c = Cache(g, dtype, LENS + [1100], hk, d, page, wide=4000 // page, token_major=token_major)
+    q = randn(g, len(LENS) + 1, hk * group, d, dtype=dtype)
+    check_attention(c, q, repeat=True)
+    check_attention(c, q, weights=True, repeat=True)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_any_sizes(seed):
+    """Attention, append and eviction at sizes drawn from the whole range."""
+    r = random.Random(seed)
+    dtype = r.choice([F32, F16, BF16])
+    d, hk, group = 8 * r.randint(1, 32), r.randint(1, 6), r.choice([1, 1, 2, 3, 5, 8, 13, 20])
+    page = r.choice([1, 3, 8, 16, 16, 24, 32, 48, 64, 160])
+    lens = [r.choice([0, 1, r.randint(1, 40), r.randint(1, 900)]) for _ in range(r.randint(1, 9))]
+    wide = max(-(-max(lens) // page), 1) + r.choice([0, 0, 1, 2000 // page])
+    g = gen(seed)
+    c = Cache(g, dtype, lens, hk, d, page, wide=wide, token_major=r.random() < 0.5, poison=True,
+              spare=2)
+    q = randn(g, len(lens), hk * group, d, dtype=dtype)
+    check_attention(c, q, weights=r.random() < 0.5, repeat=True)
+    keep = r.randint(1, max(max(lens), 1) + 3)
+    w = torch.randint(0, 9, (len(lens), hk, c.kv.capacity), generator=g, device=DEV).float()
+    dst = None
+    if r.random() < 0.5:  # other pages
+        n = -(-min(keep, c.kv.capacity) // page)
+        extra = torch.zeros(len(lens) * n, *c.k.shape[1:], device=DEV, dtype=dtype)
+        c.k, c.v = torch.cat([c.k, extra]), torch.cat([c.v, extra])
+        dst = (torch.arange(len(lens) * n, device=DEV, dtype=torch.int32) + c.k.shape[0]
+               - len(lens) * n).view(len(lens), n)
+        c.kv = ops.PagedKV(c.k, c.v, c.table, c.lens)
+    check_evict(c, w, keep, r.randint(0, keep), dst, in_place_weights=r.random() < 0.5)
+
+
+def test_attention_without_pages_or_positions():
+    for batch in (2, 400):
+        k = torch.zeros(0, 1, 16, 64, device=DEV)
+        for width in (0, 3):
+            table = torch.full((batch, width), -1, dtype=torch.int32, device=DEV)
+            kv = ops.PagedKV(k, k, table, torch.zeros(batch, dtype=torch.int32, device=DEV))
+            out = torch.full((batch, 2, 64), 7.0, device=DEV)
+            ops.PagedDecodeAttention(torch.ones(batch, 2, 64, device=DEV), kv, out=out)
+            sync_ok()
+            assert (out == 0).all()
+
+
+def test_overlapping_calls_on_two_streams():
+    """Two batches of one pool, attended on two streams at once, many times."""
+    g = gen(21)
+    a = Cache(g, BF16, [900, 1500, 40], 4, 128, 16)
+    b = Cache(g, F32, [700, 333], 2, 64, 16)
+    qa, qb = randn(g, 3, 16, 128, dtype=BF16), randn(g, 2, 4, 64)
+    want_a, want_b = ops.PagedDecodeAttention(qa, a.kv), ops.PagedDecodeAttention(qb, b.kv)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(30):
+        for i, (q, c) in enumerate(((qa, a), (qb, b))):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.PagedDecodeAttention(q, c.kv))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want_a) for x in got[0])
+    assert all(torch.equal(x, want_b) for x in got[1])
+
+
+def test_first_calls_in_a_capture():
+    """In a process of its own: the operators' first calls are captured."""
+    code = (
+        "import torch\n"
+        "from inferc_b200 import ops\n"
+        "k = torch.randn(20, 2, 16, 64, device='cuda'); v = torch.randn_like(k)\n"
+        "t = torch.randperm(20, device='cuda')[:16].view(2, 8).int()\n"
+        "lens = torch.tensor([100, 7], dtype=torch.int32, device='cuda')\n"
+        "q = torch.randn(2, 4, 64, device='cuda'); w = torch.zeros(2, 2, 128, device='cuda')\n"
+        "kv = ops.PagedKV(k, v, t, lens)\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    x, _ = ops.QKNormRotary(q, q, torch.ones(64, device='cuda'))\n"
+        "    ops.PagedKVAppend(kv, q[:, :2], q[:, 2:])\n"
+        "    o = ops.PagedDecodeAttention(x, kv, weights=w)\n"
+        "    n, kept, _ = ops.PagedKVEvict(kv, w, 40, 4)\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "# four query heads' weights of each sequence add up to 4; the first loses some to eviction\n"
+        "s = w.sum((1, 2)).tolist()\n"
+        "assert n.tolist() == [40, 7] and abs(s[1] - 4) < 1e-4 and 0.5 < s[0] < 4, (n, s)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, timeout=300)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
