@@ -238,7 +238,7 @@ __device__ __forceinline__ void add_positions(const float* s, int64_t stride, in
   for (; __any_sync(0xffffffffu, left > 0); left -= 128, s += 128, sum += 128) {
     float p[4] = {0.f, 0.f, 0.f, 0.f};
     const float* row = s;
-#pragma unroll 2
+#pragma unroll 4
     for (int c = 0; c < cols; ++c, row += stride) {
       const float2 st = stats[c];
       float x[4];

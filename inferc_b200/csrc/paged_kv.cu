@@ -470,28 +470,30 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the block of `v` before this thread; *total: over all of it.
-__device__ __forceinline__ uint64_t block_exclusive(uint64_t v, uint64_t* warp_sums,
-                                                    uint64_t* total) {
+// Sum over the block of `v` before this thread; *total: over all of it. One
+// barrier: calls take turns between two rows of `sums`, so that a row is read by
+// all before it is written again.
+template <typename V>
+__device__ __forceinline__ V block_exclusive(V v, V (*sums)[kEvictWarps], int& turn, V* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t s = v;
+  V s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t n = __shfl_up_sync(0xffffffffu, s, o);
+    const V n = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += n;
   }
-  __syncthreads();  // warp_sums of the previous call are read
-  if (lane == 31) warp_sums[warp] = s;
+  if (lane == 31) sums[turn][warp] = s;
   __syncthreads();
-  uint64_t before = 0, all = 0;
+  V w = lane < kEvictWarps ? sums[turn][lane] : 0;
 #pragma unroll
-  for (int i = 0; i < kEvictWarps; ++i) {
-    const uint64_t x = warp_sums[i];
-    if (i < warp) before += x;
-    all += x;
+  for (int o = 1; o < kEvictWarps; o <<= 1) {
+    const V n = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += n;
   }
-  *total = all;
-  return before + s - v;
+  turn ^= 1;
+  *total = __shfl_sync(0xffffffffu, w, kEvictWarps - 1);
+  const V before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  return s - v + (warp ? before : 0);
 }
 
 // One cluster per (sequence, key head).
@@ -517,7 +519,8 @@ template <int kLanes, int kTurns, bool kInPlace>
 __global__ void __launch_bounds__(kEvictThreads, 2)
     evict_kernel(const __grid_constant__ EvictArgs e, int keys_held) {
   __shared__ __align__(16) uint32_t hist[3][kBins];
-  __shared__ uint64_t sums[kEvictWarps];
+  __shared__ uint32_t sums[2][kEvictWarps];
+  __shared__ uint64_t sums2[2][kEvictWarps];
   __shared__ uint64_t s_count;  // larger (high half) and equal weights in this block's slice
   __shared__ uint32_t s_bin, s_left, s_whole;
   extern __shared__ uint32_t keys[];
@@ -559,17 +562,18 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     if (kInPlace && !e.dst_table && wo == w) return;  // the whole cluster
   } else {
     const int limit = n - e.recent, need = e.keep - e.recent;
-    // slices are multiples of 4 so that a thread's four positions are in one
     const int slice = ((n + slices - 1) / slices + 3) & ~3;
     const int s0 = min(at_slice * slice, n), s1 = min(s0 + slice, n);
     const int c1 = min(s1, limit);  // candidates: [s0, c1)
     const bool held = slice <= keys_held;
     auto key_at = [&](int j) { return held ? keys[j - s0] : weight_key(w[j]); };
-    for (int i = tid; i < 3 * kBins; i += kEvictThreads) (&hist[0][0])[i] = 0;
+    for (int i = tid * 4; i < 3 * kBins; i += kEvictThreads * 4)
+      *reinterpret_cast<uint4*>(&hist[0][0] + i) = make_uint4(0, 0, 0, 0);
     if (held)
       for (int j = s0 + tid; j < c1; j += kEvictThreads) keys[j - s0] = weight_key(w[j]);
     __syncthreads();
     uint32_t prefix = 0, mask = 0, left = need;
+    int turn = 0;
     if (need > 0) {
       for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
@@ -582,17 +586,23 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
         // bins from the largest down, four a thread
         const int low = kBins - 4 - 4 * tid;
         uint4 c = make_uint4(0, 0, 0, 0);
-        if (alone)
+        if (alone) {
           c = *reinterpret_cast<const uint4*>(&hist[pass][low]);
-        else
-          for (int r = 0; r < blocks; ++r) {
-            const uint4 x = *reinterpret_cast<const uint4*>(
-                cluster.map_shared_rank(&hist[pass][low], r));
-            c.x += x.x; c.y += x.y; c.z += x.z; c.w += x.w;
+        } else {
+          uint4 x[kMoveCluster];  // all on their way before the first is used
+#pragma unroll
+          for (int r = 0; r < kMoveCluster; ++r) {
+            x[r] = make_uint4(0, 0, 0, 0);
+            if (r < blocks)
+              x[r] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&hist[pass][low], r));
           }
-        uint64_t total;
-        const uint32_t before =
-            (uint32_t)block_exclusive((uint64_t)c.x + c.y + c.z + c.w, sums, &total);
+#pragma unroll
+          for (int r = 0; r < kMoveCluster; ++r) {
+            c.x += x[r].x; c.y += x[r].y; c.z += x[r].z; c.w += x[r].w;
+          }
+        }
+        uint32_t all;
+        const uint32_t before = block_exclusive(c.x + c.y + c.z + c.w, sums, turn, &all);
         const uint32_t count[4] = {c.w, c.z, c.y, c.x};
         uint32_t run = before;
 #pragma unroll
@@ -612,41 +622,33 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
       }
     }
     // (k & mask) > prefix stays, and of those equal to it the first `left`
-    uint64_t total, done = 0;  // larger and equal ones before; done: in what is walked already
+    // A thread takes a run of consecutive positions (an odd number of them, so that the keys
+    // it reads lie in another bank than its neighbours'): counts what stays, adds up what
+    // stays before it, and walks the run again.
+    const int run = (max(c1 - s0, 0) + kEvictThreads - 1) / kEvictThreads | 1;
+    const int j0 = min(s0 + tid * run, c1), j1 = need > 0 ? min(j0 + run, c1) : j0;
+    uint64_t mine = 0;  // larger ones (high half) and equal ones
+    for (int j = j0; j < j1; ++j) {
+      const uint32_t k = key_at(j) & mask;
+      mine += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
+    }
+    uint64_t total, done = 0;
+    uint64_t at = block_exclusive(mine, sums2, turn, &total);
     if (!alone) {
-      uint64_t mine = 0;
-      if (need > 0)
-        for (int j = s0 + tid; j < c1; j += kEvictThreads) {
-          const uint32_t k = key_at(j) & mask;
-          mine += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
-        }
-      block_exclusive(mine, sums, &total);
       if (tid == 0) s_count = total;
       cluster.sync();
-      for (int r = 0; r < rank; ++r) done += *cluster.map_shared_rank(&s_count, r);
+      uint64_t x = lane < rank ? *cluster.map_shared_rank(&s_count, lane) : 0;
+#pragma unroll
+      for (int o = 1; o < kMoveCluster; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      done = __shfl_sync(0xffffffffu, x, 0);  // in the slices before this one
     }
-    for (int j0 = s0; j0 < c1; j0 += kEvictThreads * 4) {
-      const int j = j0 + tid * 4;
-      uint32_t stays = 0;  // bits 0..3 larger, 4..7 equal
-      uint64_t v = 0;
-      if (need > 0)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j + i < c1) {
-            const uint32_t k = key_at(j + i) & mask;
-            stays |= (uint32_t)(k > prefix) << i | (uint32_t)(k == prefix) << (4 + i);
-            v += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
-          }
-      uint64_t at = done + block_exclusive(v, sums, &total);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t larger = stays >> i & 1, equal = stays >> (4 + i) & 1;
-        const uint32_t eq_before = (uint32_t)at, gt_before = (uint32_t)(at >> 32);
-        const uint32_t to = gt_before + min(eq_before, left);
-        if ((larger || (equal && eq_before < left)) && to < (uint32_t)need) keep_row(to, j + i);
-        at += ((uint64_t)larger << 32) | equal;
-      }
-      done += total;
+    at += done;
+    for (int j = j0; j < j1; ++j) {
+      const uint32_t k = key_at(j) & mask;
+      const uint32_t eq_before = (uint32_t)at, gt_before = (uint32_t)(at >> 32);
+      const uint32_t to = gt_before + min(eq_before, left);
+      if ((k > prefix || (k == prefix && eq_before < left)) && to < (uint32_t)need) keep_row(to, j);
+      at += ((uint64_t)(k > prefix) << 32) | (uint64_t)(k == prefix);
     }
     for (int j = max(s0, limit) + tid; j < s1; j += kEvictThreads) keep_row(need + j - limit, j);
   }
