@@ -329,7 +329,7 @@ int inferc_dev_decode_attention(const float* q, const float* k_cache,
  * the type of the caches and of every query, key, value and output row that
  * meets them. head_dim: a multiple of 8, 8..256. Caches and rows are 16-byte
  * aligned with strides that are multiples of 16 bytes. page_size * max_pages
- * is at most 2^31 - 64. Sums, norms and softmax statistics are fp32; results are rounded to
+ * is at most 2^30, batch at most 2^20. Sums, norms and softmax statistics are fp32; results are rounded to
  * dtype once.
  *
  * A length, page id, token range or rotary position that points outside its
@@ -426,7 +426,7 @@ int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,
  * weight (weights as inferc_dev_paged_decode_attention keeps them; equal
  * weights: the lower position stays; a NaN counts as the largest). What stays
  * moves to positions 0 .. keep - 1 in its order, in keys, values and weights.
- * Other sequences stay whole. keep >= 1, 0 <= recent <= keep.
+ * Other sequences stay whole. 1 <= keep <= 2^30, 0 <= recent <= keep.
  * dst_table: page table of the result [batch, dst_max_pages], dst_max_pages *
  * page_size >= min(keep, max_pages * page_size). NULL: in place, in the
  * sequence's own pages. Otherwise the pages it names are not in page_table

@@ -14,6 +14,8 @@
 namespace inferc_dev {
 namespace paged {
 
+constexpr int64_t kMostPositions = 1 << 30;  // of a sequence
+
 enum DType : int { F32 = 1, F16 = 10, BF16 = 16 };  // ONNX TensorProto codes
 
 // Eight values of a row as they lie in memory, four from each of two places

@@ -393,11 +393,15 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
   return p;
 }
 
-void check(const InfercPagedKv* kv, int64_t q_heads) {
+void check(const InfercPagedKv* kv, int64_t q_heads, bool weights) {
   check_kv(kv, "PagedDecodeAttention");
   IDEV_CHECK_ARG(q_heads >= 1 && q_heads <= 65535 && q_heads % kv->kv_heads == 0,
                  "PagedDecodeAttention: q_heads must be a multiple of kv_heads");
-  IDEV_CHECK_ARG(kv->batch * q_heads <= INT32_MAX, "PagedDecodeAttention: too many heads in one call");
+  IDEV_CHECK_ARG(kv->batch * q_heads <= INT32_MAX,
+                 "PagedDecodeAttention: too many heads in one call");
+  // the scratch for weights: no more bytes than a device has, let alone than 64 bits count
+  IDEV_CHECK_ARG(!weights || kv->batch * q_heads * (kv->max_pages * kv->page_size >> 10) < 1 << 30,
+                 "PagedDecodeAttention: too many positions in one call to keep weights");
 }
 
 template <typename T>
@@ -438,7 +442,7 @@ int64_t inferc_dev_paged_decode_attention_workspace(const InfercPagedKv* kv, int
                                                     int with_weights) {
   int64_t bytes = -1;
   guard([&] {
-    check(kv, q_heads);
+    check(kv, q_heads, with_weights != 0);
     bytes = plan_of(*kv, q_heads, with_weights != 0, nullptr).bytes;
   });
   return bytes;
@@ -453,7 +457,7 @@ int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,
                                       int64_t workspace_bytes, void* stream) {
   return guard([&] {
     const char* op = "PagedDecodeAttention";
-    check(kv, q_heads);
+    check(kv, q_heads, weights != nullptr);
     if (kv->batch == 0) return;
     check_rows(op, "query", q, q_batch_stride, q_head_stride, kv->dtype);
     check_rows(op, "output", out, out_batch_stride, out_head_stride, kv->dtype);

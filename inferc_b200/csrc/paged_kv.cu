@@ -60,9 +60,10 @@ void check_kv(const InfercPagedKv* kv, const char* op) {
                      kv->kv_heads <= 65535 && kv->page_size >= 1 && kv->batch >= 0 &&
                      kv->batch <= (1 << 20) && kv->max_pages >= 0,
                  o + "bad cache shape");
-  IDEV_CHECK_ARG(kv->page_size <= INT32_MAX && kv->max_pages <= INT32_MAX &&
-                     kv->page_size * kv->max_pages <= INT32_MAX - 63,
-                 o + "page_size * max_pages must be at most 2^31 - 64");
+  // (positions are counted in 32 bits, with room for a grid's strides)
+  IDEV_CHECK_ARG(kv->page_size <= kMostPositions && kv->max_pages <= kMostPositions &&
+                     kv->page_size * kv->max_pages <= kMostPositions,
+                 o + "page_size * max_pages must be at most 2^30");
   IDEV_CHECK_ARG(kv->table_stride >= kv->max_pages, o + "page table rows overlap");
   if (kv->batch == 0) return;
   IDEV_CHECK_ARG(kv->lens != nullptr && (kv->max_pages == 0 || kv->page_table != nullptr),
@@ -392,7 +393,7 @@ void launch_rows_of(const RowArgs& r, cudaStream_t st) {
   // hold (24 each), so that a decode step's few tokens do not wait for one
   // another and what a token costs is paid once where there are many.
   const int unit = 32 / G;  // heads that a warp takes at once
-  int per_warp = (int)((r.tokens * heads + 148 * 24 - 1) / (148 * 24));
+  int per_warp = (int)std::min<int64_t>((r.tokens * heads + 148 * 24 - 1) / (148 * 24), heads);
   per_warp = std::min((per_warp + unit - 1) / unit * unit, (heads + unit - 1) / unit * unit);
   const int blocks = (heads + per_warp - 1) / per_warp;
   per_warp = ((heads + blocks - 1) / blocks + unit - 1) / unit * unit;  // alike
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
   // rows per warp and step of the move, and whether this block moves row r
   constexpr int kAtOnce = 32 / kLanes, kRows = kDeep / kTurns * kAtOnce;
   constexpr int kBlockRows = kEvictWarps * kRows;
-  const bool alone = kv.max_pages * kv.page_size <= kChooseAlone;
+  const bool alone = n <= kChooseAlone && n <= keys_held;  // the same for the whole cluster
   const int slices = alone ? 1 : blocks, at_slice = alone ? 0 : rank;
   auto sync = [&]() {
     if (alone) __syncthreads();
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     // it reads lie in another bank than its neighbours'): counts what stays, adds up what
     // stays before it, and walks the run again.
     const int run = (max(c1 - s0, 0) + kEvictThreads - 1) / kEvictThreads | 1;
-    const int j0 = min(s0 + tid * run, c1), j1 = need > 0 ? min(j0 + run, c1) : j0;
+    const int j0 = (int)min((int64_t)s0 + (int64_t)tid * run, (int64_t)c1), j1 = need > 0 ? min(j0 + run, c1) : j0;
     uint64_t mine = 0;  // larger ones (high half) and equal ones
     for (int j = j0; j < j1; ++j) {
       const uint32_t k = key_at(j) & mask;
@@ -861,10 +862,9 @@ int inferc_dev_paged_kv_evict(const InfercPagedKv* kv, const int32_t* dst_table,
   return guard([&] {
     const char* op = "PagedKVEvict";
     check_kv(kv, op);
-    IDEV_CHECK_ARG(keep >= 1 && keep <= INT32_MAX && recent >= 0 && recent <= keep,
-                   "PagedKVEvict: keep must be at least 1 and recent in [0, keep]");
+    IDEV_CHECK_ARG(keep >= 1 && keep <= kMostPositions && recent >= 0 && recent <= keep,
+                   "PagedKVEvict: keep must be in [1, 2^30] and recent in [0, keep]");
     const int64_t most = std::min<int64_t>(keep, kv->max_pages * kv->page_size);
-    IDEV_CHECK_ARG(most * 64 <= INT32_MAX, "PagedKVEvict: too many positions to keep");
     if (dst_table == kv->page_table) dst_table = nullptr;
     if (dst_table)
       IDEV_CHECK_ARG(dst_max_pages >= 0 && dst_max_pages <= INT32_MAX &&

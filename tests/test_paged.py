@@ -61,7 +61,8 @@ BAD_KV = [dict(head_dim=60), dict(head_dim=0), dict(head_dim=264), dict(dtype=2)
           dict(v=A + 8), dict(k_token_stride=62), dict(v_head_stride=1023), dict(k_page_stride=1),
           dict(kv_heads=0), dict(page_size=0), dict(batch=-1), dict(table_stride=7),
           dict(lens=None), dict(page_table=None), dict(num_pages=-1), dict(num_pages=1 << 31),
-          dict(page_size=1 << 16, max_pages=1 << 15, table_stride=1 << 15)]
+          dict(page_size=1 << 16, max_pages=1 << 15, table_stride=1 << 15),
+          dict(page_size=(1 << 30) + 16, max_pages=1), dict(batch=(1 << 20) + 1)]
 
 
 @pytest.mark.parametrize("over", BAD_KV, ids=lambda o: ",".join(map(str, o)))
@@ -81,6 +82,11 @@ def test_attention_refusals():
         assert attend(kv(), **over) == INVALID, over
     need = lib.load().inferc_dev_paged_decode_attention_workspace(ctypes.byref(kv()), 4, 1)
     assert need > 0
+    # weights of more positions than any device has room for (2^20 sequences of 2^30)
+    huge = kv(page_size=1 << 20, max_pages=1 << 10, table_stride=1 << 10, batch=1 << 20)
+    assert attend(huge, weights=A) == INVALID and "weights" in message()
+    assert lib.load().inferc_dev_paged_decode_attention_workspace(ctypes.byref(huge), 4, 1) == -1
+    assert lib.load().inferc_dev_paged_decode_attention_workspace(ctypes.byref(huge), 4, 0) > 0
     assert attend(kv(), weights=A, size=need - 1) == INVALID
     assert attend(kv(), weights=A, size=need, ws=None) == INVALID
     assert attend(kv(), weights=A, size=need, ws=A + 8) == INVALID
@@ -110,7 +116,7 @@ def test_norm_refusals():
 def test_evict_refusals():
     for over in (dict(keep=0), dict(recent=-1), dict(recent=33), dict(w=None), dict(kept=None),
                  dict(lens=None), dict(lens=A), dict(lens=A + 12), dict(lens=A - 12),
-                 dict(dst=A + 4, dst_pages=1), dict(keep=1 << 32)):
+                 dict(dst=A + 4, dst_pages=1), dict(keep=(1 << 30) + 1), dict(keep=1 << 32)):
         assert evict(kv(), **over) == INVALID, over
 
 
