@@ -417,8 +417,8 @@ void run(const Plan& p, cudaStream_t st) {
     const int64_t pairs = kv.batch * kv.kv_heads * g.blocks;
     by_warp = pairs > g.warps;
     jobs = by_warp ? g.warps : pairs;
-    // few jobs: several blocks each, of eight float4s of the result at least
-    of = (int)std::min<int64_t>(g.block * (kv.head_dim / 4) / 8,
+    // few jobs: several blocks each, of four float4s of the result at least
+    of = (int)std::min<int64_t>(g.block * (kv.head_dim / 4) / 4,
                                 std::max<int64_t>(1, 4 * kSMs / jobs));
     of = std::max(of, 1);
   }

@@ -407,6 +407,51 @@ def test_overlapping_calls_on_two_streams():
     assert all(torch.equal(x, want_b) for x in got[1])
 
 
+@pytest.mark.parametrize("dtype,hk,group,d,page", [(BF16, 4, 4, 128, 16), (F32, 12, 1, 64, 16),
+                                                   (F16, 2, 20, 96, 24)])
+def test_steps_without_waiting_equal_steps_with_waiting(dtype, hk, group, d, page):
+    """Each kernel starts while the one before it drains; what it reads must
+    still be that one's results: a run of steps queued at once, the lengths and
+    tables changing in between, gives the bits of the same run with a wait behind
+    every call."""
+    def steps(wait):
+        g = gen(33)
+        lens = [1, 700, 260, 999]
+        c = Cache(g, dtype, lens, hk, d, page, wide=-(-1100 // page), poison=False,
+                  spare=4 * -(-1100 // page))
+        need = torch.tensor([-(-n // page) for n in lens], device=DEV)
+        free = c.spare[: c.table.numel()].view_as(c.table)
+        c.table.copy_(torch.where(torch.arange(c.table.shape[1], device=DEV) < need[:, None],
+                                  c.table, free))
+        w = torch.zeros(4, hk, c.kv.capacity, device=DEV)
+        cos, sin = ops.RotaryTable(4096, d)
+        positions = c.lens.clone()
+        gamma = 1 + 0.1 * randn(g, d)
+        rows = [randn(g, 4, (group + 2) * hk, d, dtype=dtype) for _ in range(25)]
+        outs = []
+        torch.cuda.synchronize()
+        for i, r in enumerate(rows):
+            c.lens.add_(1)
+            q = ops.QKNormRotaryAppend(c.kv, r[:, : group * hk], r[:, group * hk: (group + 1) * hk],
+                                       r[:, (group + 1) * hk:], gamma, gamma, 1e-6, cos, sin,
+                                       positions)
+            wait()
+            outs.append(ops.PagedDecodeAttention(q, c.kv, weights=w))
+            wait()
+            positions.add_(1)
+            if i % 6 == 5:
+                new, kept, _ = ops.PagedKVEvict(c.kv, w, 250 + i, 9)
+                wait()
+                c.lens.copy_(new)
+                outs += [new, kept]
+        torch.cuda.synchronize()
+        return outs + [w, c.k, c.v]
+
+    for a, b in zip(steps(lambda: None), steps(torch.cuda.synchronize)):
+        assert torch.equal(a, b)
+    sync_ok()
+
+
 def test_first_calls_in_a_capture():
     """In a process of its own: the operators' first calls are captured."""
     code = (
