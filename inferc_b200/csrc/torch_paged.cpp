@@ -184,6 +184,8 @@ PyObject* make(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK(k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
                     v.device() == k.device(),
                 op, ": k_cache and v_cache must be alike, [pages, kv_heads, page, head_dim]");
+    TORCH_CHECK(k.size(1) >= 1 && k.size(2) >= 1, op,
+                ": caches must have a key head and a position per page at least");
     TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, op,
                 ": the caches' last dimension must be contiguous");
     TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt &&

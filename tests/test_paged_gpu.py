@@ -592,6 +592,14 @@ def test_attention_refusals():
         ops.PagedDecodeAttention(q, ops.PagedKV(c.k[..., :60], c.v[..., :60], c.table, c.lens))
 
 
+def test_caches_without_heads_or_positions_are_refused():
+    table, lens = int32([[0]]), int32([0])
+    for shape in ((2, 0, 16, 64), (2, 2, 0, 64)):
+        x = torch.zeros(shape, device=DEV)
+        with pytest.raises(RuntimeError, match="at least"):
+            ops.PagedKV(x, x.clone(), table, lens)
+
+
 # ---------------------------------------------------------------- eviction
 
 
