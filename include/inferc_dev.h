@@ -329,8 +329,9 @@ int inferc_dev_decode_attention(const float* q, const float* k_cache,
  * the type of the caches and of every query, key, value and output row that
  * meets them. head_dim: a multiple of 8, 8..256. Caches and rows are 16-byte
  * aligned with strides that are multiples of 16 bytes. page_size * max_pages
- * is at most 2^30, batch at most 2^20. Sums, norms and softmax statistics are fp32; results are rounded to
- * dtype once.
+ * is at most 2^30, batch at most 2^20. What a call writes (caches, outputs,
+ * weights) has strides under which no two rows share elements. Sums, norms and
+ * softmax statistics are fp32; results are rounded to dtype once.
  *
  * A length, page id, token range or rotary position that points outside its
  * buffer is never followed: the positions concerned are left out (attention; a

@@ -136,6 +136,13 @@ int* range_flag_ptr();
 void check_kv(const InfercPagedKv* kv, const char* op);
 void check_rows(const char* op, const char* what, const void* p, int64_t stride_a,
                 int64_t stride_b, int dtype);
+// Throws it when rows of `d` elements that a kernel writes, at i * a.stride +
+// j * b.stride + k * c.stride, may share elements.
+struct Steps {
+  int64_t count, stride;
+};
+void check_apart(const char* op, const char* what, int64_t d, Steps a, Steps b,
+                 Steps c = {1, 0});
 int elem_bytes(int dtype);
 
 }  // namespace paged

@@ -461,6 +461,11 @@ int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,
     if (kv->batch == 0) return;
     check_rows(op, "query", q, q_batch_stride, q_head_stride, kv->dtype);
     check_rows(op, "output", out, out_batch_stride, out_head_stride, kv->dtype);
+    check_apart(op, "output", kv->head_dim, {kv->batch, out_batch_stride},
+                {q_heads, out_head_stride});
+    if (weights)
+      check_apart(op, "weights", kv->max_pages * kv->page_size, {kv->batch, weights_batch_stride},
+                  {kv->kv_heads, weights_head_stride});
     Plan p = plan_of(*kv, q_heads, weights != nullptr, static_cast<char*>(workspace));
     IDEV_CHECK_ARG(workspace_bytes >= p.bytes && (p.bytes == 0 || (workspace && aligned16(workspace))),
                    "PagedDecodeAttention: the workspace is too small or not 16-byte aligned");

@@ -45,6 +45,30 @@ void check_rows(const char* op, const char* what, const void* p, int64_t stride_
                  std::string(op) + ": " + what + " must be 16-byte aligned, its strides too");
 }
 
+void check_apart(const char* op, const char* what, int64_t d, Steps a, Steps b, Steps c) {
+  Steps steps[3] = {a, b, c};
+  auto size = [](int64_t stride) { return stride < 0 ? -(__int128)stride : (__int128)stride; };
+  std::sort(steps, steps + 3, [&](const Steps& x, const Steps& y) {
+    return size(x.stride) < size(y.stride);
+  });
+  __int128 extent = d;  // of what the smaller steps reach
+  for (const Steps& s : steps) {
+    if (s.count == 0) return;
+    if (s.count == 1) continue;
+    IDEV_CHECK_ARG(size(s.stride) >= extent,
+                   std::string(op) + ": rows of the " + what + " overlap");
+    extent += size(s.stride) * (s.count - 1);
+  }
+}
+
+// The caches, where they are written.
+static void check_caches_apart(const char* op, const InfercPagedKv& kv) {
+  check_apart(op, "key cache", kv.head_dim, {kv.num_pages, kv.k_page_stride},
+              {kv.kv_heads, kv.k_head_stride}, {kv.page_size, kv.k_token_stride});
+  check_apart(op, "value cache", kv.head_dim, {kv.num_pages, kv.v_page_stride},
+              {kv.kv_heads, kv.v_head_stride}, {kv.page_size, kv.v_token_stride});
+}
+
 static void check_dtype_dim(const char* op, int dtype, int64_t head_dim) {
   IDEV_CHECK_ARG(dtype == F32 || dtype == F16 || dtype == BF16,
                  std::string(op) + ": dtype must be float, float16 or bfloat16");
@@ -800,10 +824,14 @@ int inferc_dev_qk_norm_rotary(const InfercHeadRotary* rot, int dtype, const void
     if (q_heads > 0) {
       check_rows(op, "query", q, q_token_stride, q_head_stride, dtype);
       check_rows(op, "query output", q_out, q_out_token_stride, q_out_head_stride, dtype);
+      check_apart(op, "query output", head_dim, {tokens, q_out_token_stride},
+                  {q_heads, q_out_head_stride});
     }
     if (kv_heads > 0) {
       check_rows(op, "key", k, k_token_stride, k_head_stride, dtype);
       check_rows(op, "key output", k_out, k_out_token_stride, k_out_head_stride, dtype);
+      check_apart(op, "key output", head_dim, {tokens, k_out_token_stride},
+                  {kv_heads, k_out_head_stride});
     }
     r.q = {q, q_out, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride,
            (int)q_heads};
@@ -840,7 +868,10 @@ int inferc_dev_paged_kv_append(const InfercPagedKv* kv, const InfercHeadRotary* 
     if (q_heads > 0) {
       check_rows(op, "query", q, q_token_stride, q_head_stride, kv->dtype);
       check_rows(op, "query output", q_out, q_out_token_stride, q_out_head_stride, kv->dtype);
+      check_apart(op, "query output", kv->head_dim, {tokens, q_out_token_stride},
+                  {q_heads, q_out_head_stride});
     }
+    check_caches_apart(op, *kv);
     r.a.kv = *kv;
     r.a.page = FastDiv((uint32_t)kv->page_size);
     r.a.flag = range_flag_ptr();
@@ -865,7 +896,10 @@ int inferc_dev_paged_kv_evict(const InfercPagedKv* kv, const int32_t* dst_table,
     IDEV_CHECK_ARG(keep >= 1 && keep <= kMostPositions && recent >= 0 && recent <= keep,
                    "PagedKVEvict: keep must be in [1, 2^30] and recent in [0, keep]");
     const int64_t most = std::min<int64_t>(keep, kv->max_pages * kv->page_size);
-    if (dst_table == kv->page_table) dst_table = nullptr;
+    if (dst_table == kv->page_table && (kv->batch <= 1 || dst_table_stride == kv->table_stride))
+      dst_table = nullptr;
+    IDEV_CHECK_ARG(!dst_table || dst_table != kv->page_table,
+                   "PagedKVEvict: dst_table starts as page_table does, but has another stride");
     if (dst_table)
       IDEV_CHECK_ARG(dst_max_pages >= 0 && dst_max_pages <= INT32_MAX &&
                          dst_table_stride >= dst_max_pages &&
@@ -877,6 +911,18 @@ int inferc_dev_paged_kv_evict(const InfercPagedKv* kv, const int32_t* dst_table,
     IDEV_CHECK_ARG(weights && lens_out && kept, "PagedKVEvict: null weights, lens_out or kept");
     IDEV_CHECK_ARG(lens_out + kv->batch <= kv->lens || kv->lens + kv->batch <= lens_out,
                    "PagedKVEvict: lens_out must not overlap lens");
+    check_caches_apart(op, *kv);
+    if (!weights_out) {
+      weights_out = weights;
+      weights_out_batch_stride = weights_batch_stride;
+      weights_out_head_stride = weights_head_stride;
+    }
+    check_apart(op, "weights", kv->max_pages * kv->page_size,
+                {kv->batch, weights_out_batch_stride}, {kv->kv_heads, weights_out_head_stride});
+    IDEV_CHECK_ARG(weights_out != weights || kv->batch * kv->kv_heads == 1 ||
+                       ((weights_out_batch_stride == weights_batch_stride || kv->batch == 1) &&
+                        (weights_out_head_stride == weights_head_stride || kv->kv_heads == 1)),
+                   "PagedKVEvict: weights_out starts as weights do, but has other strides");
     EvictArgs e{};
     e.a.kv = *kv;
     e.a.page = FastDiv((uint32_t)kv->page_size);
@@ -887,9 +933,9 @@ int inferc_dev_paged_kv_evict(const InfercPagedKv* kv, const int32_t* dst_table,
     e.w = weights;
     e.w_batch = weights_batch_stride;
     e.w_head = weights_head_stride;
-    e.w_out = weights_out ? weights_out : weights;
-    e.wo_batch = weights_out ? weights_out_batch_stride : weights_batch_stride;
-    e.wo_head = weights_out ? weights_out_head_stride : weights_head_stride;
+    e.w_out = weights_out;
+    e.wo_batch = weights_out_batch_stride;
+    e.wo_head = weights_out_head_stride;
     e.keep = (int)keep;
     e.recent = (int)recent;
     e.lens_out = lens_out;

@@ -120,6 +120,50 @@ def test_evict_refusals():
         assert evict(kv(), **over) == INVALID, over
 
 
+def test_written_rows_that_overlap_are_refused():
+    """Broadcast or interleaved outputs would get the values of several rows."""
+    L = lib.load()
+    c = kv()
+
+    def attend_to(batch=256, head=64, w=None, wb=256, wh=128, d=c):
+        return L.inferc_dev_paged_decode_attention(ctypes.byref(d), A, 256, 64, 4, 0.125, A, batch,
+                                                   head, w, wb, wh, None, 0, None)
+
+    for over in (dict(batch=0), dict(head=0), dict(head=60), dict(batch=252), dict(batch=64),
+                 dict(batch=-64), dict(w=A, wb=0), dict(w=A, wh=0), dict(w=A, wh=127),
+                 dict(w=A, wb=255)):
+        assert attend_to(**over) == INVALID and "overlap" in message(), over
+    # rows apart, head-major or with single rows: refused for the missing workspace alone
+    long = kv(max_pages=128, table_stride=128)
+    for over in (dict(batch=64, head=256, d=long), dict(w=A, wb=128, wh=512),
+                 dict(batch=-256, d=long), dict(batch=0, w=A, wb=0, d=kv(batch=1))):
+        assert attend_to(**over) == INVALID and "workspace" in message(), over
+    for over in (dict(k_page_stride=0), dict(v_head_stride=0), dict(k_token_stride=0),
+                 dict(v_page_stride=2048 - 64)):
+        for call in (append, evict):
+            assert call(kv(**over)) == INVALID and "overlap" in message(), (over, call)
+
+    def norm_to(q=128, k=128, kh=64):
+        return L.inferc_dev_qk_norm_rotary(ctypes.byref(rot()), 1, A, 128, 64, A, 128, 64, A, q, 64,
+                                           A, k, kh, 3, 2, 2, 64, None)
+
+    for over in (dict(q=0), dict(q=64), dict(k=124), dict(kh=0)):
+        assert norm_to(**over) == INVALID and "overlap" in message(), over
+    assert L.inferc_dev_paged_kv_append(
+        ctypes.byref(kv()), ctypes.byref(rot()), A, 256, 64, A, 128, 64, A, 128, 64, A, 0, 64, 4,
+        None, 4, None) == INVALID and "overlap" in message()
+
+    def evict_to(w_out=None, wb=256, wh=128, dst=None, dst_stride=8):
+        return L.inferc_dev_paged_kv_evict(ctypes.byref(kv()), dst, 8, dst_stride, A, 256, 128,
+                                           w_out, wb, wh, 32, 8, 2 * A, A, None)
+
+    for over in (dict(w_out=A + 64, wb=0), dict(w_out=A + 64, wh=64)):
+        assert evict_to(**over) == INVALID and "overlap" in message(), over
+    # the same place read and written in different orders
+    assert evict_to(w_out=A, wb=128, wh=512) == INVALID and "other strides" in message()
+    assert evict_to(dst=A, dst_stride=16) == INVALID and "another stride" in message()
+
+
 def test_empty_calls_do_nothing():
     none = kv(batch=0)
     assert attend(none) == 0 and evict(none) == 0 and append(none, tokens=0) == 0
