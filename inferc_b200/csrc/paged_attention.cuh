@@ -71,7 +71,6 @@ struct AttendArgs {
   int tile;         // positions per tile
   bool whole;       // one block of the grid reads one (sequence, key head), see attend_kernel
   int64_t warps;    // in the grid
-  int64_t* before;  // [batch + 1] tiles before each sequence
   int4* jobs;       // [warps] (sequence or -1, head block, parts) whose first part this warp left
   int4* starts;     // [warps] (sequence, head block, tile) where a warp's share begins
   float* part_ml;   // [2 warps, block, 2] maximum and sum of a part
@@ -799,14 +798,6 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       total += s_warp[i];
     }
     s_before[tid] = ahead + scan - mine;
-    if (blockIdx.x == 0 && g.before) {
-      int64_t at = ahead + scan - mine;
-      for (int b = run0; b < run1; ++b) {
-        g.before[b] = at;
-        at += (int64_t)((seq_len(g.a, b) + kTile - 1) / kTile) * heads;
-      }
-      if (tid == 0) g.before[batch] = total;
-    }
     // A sequence of length 0 gives zeros.
     for (int64_t b = blockIdx.x; b < batch; b += gridDim.x)
       if (seq_len(g.a, b) == 0)
