@@ -47,6 +47,13 @@ class PagedKV:
         _, self.kv_heads, self.page, self.head_dim = k_cache.shape
         self.capacity = self.max_pages * self.page
 
+    def __setattr__(self, name, value):
+        """Operators read the tensors given at first: another one (kv.lens = ...) would be
+        ignored. kv.lens += 1 works in place and is the same tensor."""
+        if name in self.__dict__ and self.__dict__[name] is not value:
+            raise RuntimeError(f"PagedKV: {name} is fixed; update it in place or make another view")
+        super().__setattr__(name, value)
+
 
 def RotaryTable(positions: int, rotary_dim: int, base: float = 10000.0, device="cuda"
                 ) -> tuple[torch.Tensor, torch.Tensor]:
@@ -110,8 +117,8 @@ def PagedKVEvict(kv: PagedKV, weights: torch.Tensor, keep: int, recent: int = 0,
     """Trims every sequence longer than `keep` to `keep` positions per key head:
     its last `recent`, and of the others those with the largest weight (ties: the
     lower position). They move to the front in their order, in keys, values and
-    weights. dst_table: int32 [batch, pages] of pages to put the result into
-    (None: the sequence's own, which no other sequence may share); weights_out:
+    weights. dst_table: int32 [batch, pages] of pages to put the result into,
+    none of them in kv.page_table (None: the sequence's own, which no other sequence may share); weights_out:
     like weights (None: in place). Returns (lens_out, kept, weights_out): the
     new lengths, a tensor apart from kv.lens; the old positions, int32 [batch,
     kv_heads, keep], -1 behind the last; and the weights."""

@@ -600,6 +600,15 @@ def test_caches_without_heads_or_positions_are_refused():
             ops.PagedKV(x, x.clone(), table, lens)
 
 
+def test_a_view_keeps_its_tensors():
+    c = Cache(gen(31), F32, [20, 3], 2, 64, 16)
+    for name in ("lens", "page_table", "k", "v"):
+        with pytest.raises(RuntimeError, match="fixed"):
+            setattr(c.kv, name, getattr(c.kv, name).clone())
+    c.kv.lens += 1
+    assert c.lens.tolist() == [21, 4] and c.kv.lens is c.lens
+
+
 # ---------------------------------------------------------------- eviction
 
 
