@@ -524,7 +524,7 @@ struct TensorHeads {
 // The same for one fp32 query head per key head, on the CUDA cores: the matrix
 // instruction would use one of its 8 columns, and three of them per product with
 // the splitting of K and V are over twice the instructions (32 x 12 heads of 64,
-// 100 MB and their running sums: 31 us against 36 us). A lane takes a position of the tile (half of its
+// 100 MB and their running sums: 31 us against 36 us, both with kTmaKeep). A lane takes a position of the tile (half of its
 // columns where the tile has 16 positions) for the scores, and kDim / 32 columns
 // for the values; P passes through shared memory. Two fp32 operations per
 // instruction (fma.rn.f32x2).
@@ -717,13 +717,21 @@ __device__ __forceinline__ void join_whole(const AttendArgs& g, int b, int hk, i
   }
 }
 
-template <typename T, int kDim, typename Heads, bool kTma>
+// How tiles are fetched: by cp.async, by TMA, or by TMA where the scores that the
+// kernel writes are read again by the kernel behind it, so that keys and values are to
+// leave L2 first (64 sequences, 50 MB of scores: 214 -> 209 us; fp32, 32 x 12 heads:
+// 31 -> 28 us). A kernel of its own: chosen at every load it took the calls
+// without scores 0.2 to 0.6 us.
+enum Fetch : int { kCopy, kTmaKeep, kTmaOnce };
+
+template <typename T, int kDim, typename Heads, int kFetch>
 __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     attend_kernel(const __grid_constant__ AttendArgs g, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map) {
   using L = Layout<T, kDim>;
   constexpr int kElem = sizeof(T), kThreads = kWarps * 32, kTile = L::kTile;
   constexpr int kSubs = kTile / kBox;
+  constexpr bool kTma = kFetch != kCopy;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -858,17 +866,31 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
   auto boxes = [&](const CUtensorMap* map) {
     const uint32_t bar = tc::smem_u32(&full[slot_in]);
     const uint32_t dst = ring_addr + slot_in * L::kSlot;
+    [[maybe_unused]] uint64_t policy = 0;
+    if constexpr (kFetch == kTmaOnce)
+      asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
 #pragma unroll
     for (int s = 0; s < kSubs; ++s)
       if (mask_in >> (s * kBox) & 1) {
 #pragma unroll
-        for (int i = 0; i < L::kColumns; ++i)
-          asm volatile(
-              "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-              " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + i * L::kColumn + s * kBox * 128),
-              "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(i * L::kElems), "r"(at[s]),
-              "r"(load.hk), "r"(page[s])
-              : "memory");
+        for (int i = 0; i < L::kColumns; ++i) {
+          if constexpr (kFetch == kTmaOnce)
+            asm volatile(
+                "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                ".L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(
+                    dst + i * L::kColumn + s * kBox * 128),
+                "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(i * L::kElems), "r"(at[s]),
+                "r"(load.hk), "r"(page[s]), "l"(policy)
+                : "memory");
+          else
+            asm volatile(
+                "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + i * L::kColumn +
+                                                             s * kBox * 128),
+                "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(i * L::kElems), "r"(at[s]),
+                "r"(load.hk), "r"(page[s])
+                : "memory");
+        }
       }
   };
   auto expect = [&]() {
@@ -1139,6 +1161,11 @@ bool make_map(const InfercPagedKv& kv, bool values, CUtensorMap* map) {
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename H>
+struct Named {
+  using type = H;
+};
+
 template <typename T, int kDim>
 void launch_attend_dim(const AttendArgs& g, cudaStream_t st) {
   using L = Layout<T, kDim>;
@@ -1152,18 +1179,22 @@ void launch_attend_dim(const AttendArgs& g, cudaStream_t st) {
                                  OneHead<kDim == 64 ? 64 : 128>, TensorHeads<T, kDim, 1>>;
   using Eight = TensorHeads<T, kDim, 1>;
   using Sixteen = TensorHeads<T, kDim, 2>;
-  auto* kernel = tma ? (kind == 0   ? attend_kernel<T, kDim, One, true>
-                        : kind == 1 ? attend_kernel<T, kDim, Eight, true>
-                                    : attend_kernel<T, kDim, Sixteen, true>)
-                     : (kind == 0   ? attend_kernel<T, kDim, One, false>
-                        : kind == 1 ? attend_kernel<T, kDim, Eight, false>
-                                    : attend_kernel<T, kDim, Sixteen, false>);
+  const Fetch fetch = !tma ? kCopy : g.scores ? kTmaOnce : kTmaKeep;
+  auto kernel_of = [&](auto heads) {
+    using Heads = typename decltype(heads)::type;
+    return fetch == kCopy      ? attend_kernel<T, kDim, Heads, kCopy>
+           : fetch == kTmaKeep ? attend_kernel<T, kDim, Heads, kTmaKeep>
+                               : attend_kernel<T, kDim, Heads, kTmaOnce>;
+  };
+  auto* kernel = kind == 0   ? kernel_of(Named<One>{})
+                 : kind == 1 ? kernel_of(Named<Eight>{})
+                             : kernel_of(Named<Sixteen>{});
   // one request per kernel and device
   constexpr int kMost = 64;
-  static std::atomic<bool> ready[kMost][6];
+  static std::atomic<bool> ready[kMost][9];
   int dev = 0;
   IDEV_CUDA(cudaGetDevice(&dev));
-  std::atomic<bool>* known = dev < kMost ? &ready[dev][(tma ? 3 : 0) + kind] : nullptr;
+  std::atomic<bool>* known = dev < kMost ? &ready[dev][3 * fetch + kind] : nullptr;
   if (!known || !known->load(std::memory_order_relaxed)) {
     IDEV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
     if (known) known->store(true, std::memory_order_relaxed);
