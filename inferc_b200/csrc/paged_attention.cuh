@@ -524,9 +524,9 @@ struct TensorHeads {
 // The same for one fp32 query head per key head, on the CUDA cores: the matrix
 // instruction would use one of its 8 columns, and three of them per product with
 // the splitting of K and V are over twice the instructions (32 x 12 heads of 64,
-// 100 MB and their running sums: 31 us against 36 us, both with kTmaKeep). A lane takes a position of the tile (half of its
-// columns where the tile has 16 positions) for the scores, and kDim / 32 columns
-// for the values; P passes through shared memory. Two fp32 operations per
+// 100 MB and their running sums: 31 us against 36 us, both with kTmaKeep). A lane
+// takes a position of the tile (half of its columns where the tile has 16
+// positions) for the scores, and kDim / 32 columns for the values; P passes through shared memory. Two fp32 operations per
 // instruction (fma.rn.f32x2).
 template <int kDim>
 struct OneHead {

@@ -657,7 +657,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     // it reads lie in another bank than its neighbours'): counts what stays, adds up what
     // stays before it, and walks the run again.
     const int run = (max(c1 - s0, 0) + kEvictThreads - 1) / kEvictThreads | 1;
-    const int j0 = (int)min((int64_t)s0 + (int64_t)tid * run, (int64_t)c1), j1 = need > 0 ? min(j0 + run, c1) : j0;
+    const int j0 = (int)min((int64_t)s0 + (int64_t)tid * run, (int64_t)c1);
+    const int j1 = need > 0 ? min(j0 + run, c1) : j0;
     uint64_t mine = 0;  // larger ones (high half) and equal ones
     for (int j = j0; j < j1; ++j) {
       const uint32_t k = key_at(j) & mask;
