@@ -326,8 +326,10 @@ struct TensorHeads {
   }
 
   // The instruction adds to its accumulator by cutting, always towards zero: over many steps
-  // that would cost fp32 results a digit (2e-6 of an output of 1000 positions of 256 columns).
-  // So fp32 accumulators take four steps of the large products, then join a sum that is rounded.
+  // that would cost fp32 results a digit (2e-6 of an output of 1000 positions of 256 columns) and
+  // bias 16-bit ones (262144 positions in one warp's share: 1.7e-3 too small, 3.5 half steps of
+  // fp16). So fp32 scores take four steps of the large products, and values those of one tile,
+  // then join a sum that is rounded.
   __device__ __forceinline__ static void settle(float (&sum)[4], float (&acc)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -432,16 +434,20 @@ struct TensorHeads {
             lo[u][c][i] = transpose8x8(lo[u][c][i]);
           }
 #pragma unroll
-      for (int i = 0; i < kMTiles; ++i)
+      for (int i = 0; i < kMTiles; ++i) {
+        float fresh[kCols][4] = {};
 #pragma unroll
         for (int u = 0; u < kSubs; ++u) {
           uint32_t a[4];
           ldmatrix4_trans((v_addr ^ ((i & 3) << 5)) + (i >> 2) * L::kColumn + u * kBox * 128, a);
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, lo[u][c][0], lo[u][c][1]);
+          for (int c = 0; c < kCols; ++c) mma16<T>(fresh[c], a, lo[u][c][0], lo[u][c][1]);
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) mma16<T>(o[c][i], a, hi[u][c][0], hi[u][c][1]);
+          for (int c = 0; c < kCols; ++c) mma16<T>(fresh[c], a, hi[u][c][0], hi[u][c][1]);
         }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) settle(o[c][i], fresh[c]);
+      }
     } else {
       constexpr int kEights = kSubs * 2;  // eight positions each
       // P of positions (2 tig, 2 tig + 1) of each eight, head gid, from the lanes that hold them
