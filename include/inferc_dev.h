@@ -403,7 +403,11 @@ int inferc_dev_paged_kv_append(const InfercPagedKv* kv, const InfercHeadRotary* 
 /* The paged, batched form of inferc_dev_decode_attention: one new token per
  * sequence, out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j over the
  * sequence's lens[b] positions; q_heads is a multiple of kv_heads, query head h
- * reads key head h / (q_heads / kv_heads). A sequence of length 0 gives zeros.
+ * reads key head h / (q_heads / kv_heads). A sequence of length 0, or a head
+ * without a score above -inf, gives zeros and adds nothing to weights.
+ * Infinities and NaN in rows that are read go by the same formula (a key whose
+ * score is -inf has weight 0, a value of inf gives inf); a weight below 2^-126
+ * of its head's largest counts as 0.
  * weights may be NULL; otherwise fp32 [batch, kv_heads, >= max_pages *
  * page_size] in the order of positions, to which each position's softmax
  * weight is added, summed over the query heads of its key head (in a fixed

@@ -48,6 +48,11 @@
 // pieces each, three products (big big, big small, small big), so that at most
 // 2^-20 of a product is lost (cut operands lose 3 * 2^-23, rounded ones 2^-22,
 // small * small is below 2^-21).
+//
+// Pieces of an infinity are an infinity and a NaN or a zero, whose products are
+// NaN where the definition has a weight of 0 or an infinite result. So a share
+// whose sums come out infinite or NaN is walked again in plain fp32 operations
+// (walk_again); the others pay one look at the sums per share.
 #pragma once
 
 #include <atomic>
@@ -236,6 +241,7 @@ struct TensorHeads {
   static constexpr int kMTiles = kDim / 16;                     // blocks of 16 columns of V
   static constexpr int kPartFloats = kCols * 8 * kDim;
   static constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
+  static constexpr bool kPieces = true;  // operands enter as sums of pieces
   // fp32 queries are split once where their pieces fit the registers
   static constexpr bool kSplitOnce = kWide && kDim * kCols <= 128;
   uint32_t qf[kCols][kKSteps][kSplitOnce ? 4 : 2];
@@ -247,6 +253,7 @@ struct TensorHeads {
   __device__ __forceinline__ static int tig() { return threadIdx.x & 3; }
 
   __device__ __forceinline__ void begin(const T* q, int64_t q_head, int cols, int d) {
+    bool odd = false;  // fp32: infinities and NaN, some of which split_tf32 makes zeros of
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       const int h = c * 8 + gid();
@@ -259,6 +266,7 @@ struct TensorHeads {
           const bool in = h < cols && col < d;
           uint32_t x = 0;
           if (in) x = *reinterpret_cast<const uint32_t*>(row + col);
+          if constexpr (kWide) odd |= (x & 0x7f800000u) == 0x7f800000u;
           if constexpr (kSplitOnce) split_tf32(__uint_as_float(x), qf[c][s][i], qf[c][s][2 + i]);
           else qf[c][s][i] = x;
         }
@@ -268,6 +276,25 @@ struct TensorHeads {
 #pragma unroll
       for (int i = 0; i < kMTiles; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
     }
+    if (kWide && __any_sync(0xffffffffu, odd))
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) l[c][0] = l[c][1] = NAN;
+  }
+
+  // Whether a sum of the warp's is infinite or NaN.
+  __device__ __forceinline__ bool odd() const {
+    float x[4] = {};  // NaN once anything infinite or NaN was multiplied by 0
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      x[0] = fmaf(l[c][0], 0.f, x[0]);
+      x[1] = fmaf(l[c][1], 0.f, x[1]);
+#pragma unroll
+      for (int i = 0; i < kMTiles; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(o[c][i][j], 0.f, x[j]);
+    }
+    const float any = (x[0] + x[1]) + (x[2] + x[3]);
+    return __any_sync(0xffffffffu, any != any);
   }
 
   __device__ __forceinline__ void scores(const unsigned char* slot, float scale) {
@@ -541,6 +568,7 @@ struct OneHead {
   static constexpr int kQuads = kDim / kSplit / 4;  // float4s of a row that a lane multiplies
   static constexpr int kMine = kDim / 32;           // output columns of a lane: 2 or 4
   static constexpr int kPartFloats = kDim;
+  static constexpr bool kPieces = false;
   unsigned long long q[kQuads][2], o[kMine / 2];
   float m, l, s;
 
@@ -723,6 +751,117 @@ __device__ __forceinline__ void join_whole(const AttendArgs& g, int b, int hk, i
   }
 }
 
+// Positions [j0, j1) of query heads q0 .. q0 + cols - 1 of a sequence once more, in
+// plain fp32 operations and from global memory, and what the warp's share leaves of
+// them; for operands with infinities or NaN, so simple: a head at a time, a lane for a
+// position's score and for every 32nd column of the values.
+template <typename T>
+__device__ __forceinline__ void walk_heads(const AttendArgs& g, int b, int hk, int q0, int cols,
+                                           int j0, int j1, bool whole, int64_t part, float2* ml,
+                                           float* po) {
+  const InfercPagedKv& kv = g.a.kv;
+  const int lane = threadIdx.x & 31, d = kv.head_dim;
+  constexpr int kMine = 256 / 32;
+  for (int h = 0; h < cols; ++h) {
+    const T* q = reinterpret_cast<const T*>(g.q) + b * g.q_batch + (q0 + h) * g.q_head;
+    const int64_t row = b * (kv.kv_heads * g.group) + q0 + h;
+    float m = -INFINITY, l = 0.f, o[kMine] = {};
+    for (int first = j0; first < j1; first += 32) {
+      const int j = first + lane;
+      int64_t off_v = -1;
+      float s = -INFINITY;
+      if (j < j1) {
+        const uint32_t index = g.a.page.div(j), slot = j - index * g.a.page.d;
+        const int id = page_of(g.a, kv.page_table + b * kv.table_stride, index);
+        if (id >= 0) {
+          const T* k = reinterpret_cast<const T*>(kv.k) + id * kv.k_page_stride +
+                       slot * kv.k_token_stride + hk * kv.k_head_stride;
+          off_v = id * kv.v_page_stride + slot * kv.v_token_stride + hk * kv.v_head_stride;
+          float sum = 0.f;
+          for (int c = 0; c < d; c += 8) {
+            float x[8], y[8];
+            load8(q + c, x);
+            load8(k + c, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], y[i], sum);
+          }
+          s = sum * g.scale;
+        }
+        if (g.scores) g.scores[row * g.capacity + j] = s;
+      }
+      const float top = fmaxf(m, warp_max(s)), to = top == -INFINITY ? 0.f : top;
+      const float keep = ex2(m - to), p = ex2(s - to);
+      m = top;
+      l = l * keep + p;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) o[i] *= keep;
+      if (__any_sync(0xffffffffu, p != p)) {  // the head's sum is NaN, and all of its results
+        l = NAN;
+        break;
+      }
+      for (int r = 0; r < 32; ++r) {
+        const int64_t off = __shfl_sync(0xffffffffu, off_v, r);
+        const float w = __shfl_sync(0xffffffffu, p, r);
+        if (off < 0) continue;
+        const T* v = reinterpret_cast<const T*>(kv.v) + off;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          if (lane + 32 * i < d) o[i] = fmaf(w, static_cast<float>(v[lane + 32 * i]), o[i]);
+      }
+    }
+    const float sum = warp_sum(l), inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (lane == 0) {
+      if (g.whole) {
+        ml[h] = make_float2(m, sum);
+      } else if (!whole) {
+        reinterpret_cast<float2*>(g.part_ml)[part * g.block + h] = make_float2(m, sum);
+      } else if (g.stats) {
+        reinterpret_cast<float2*>(g.stats)[row] = make_float2(m == -INFINITY ? 0.f : m, inv);
+      }
+    }
+    T* out = reinterpret_cast<T*>(g.out) + b * g.o_batch + (q0 + h) * g.o_head;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int col = lane + 32 * i;
+      if (col >= d) continue;
+      if (whole) out[col] = T(o[i] * inv);
+      else po[h * d + col] = o[i];
+    }
+  }
+}
+
+// The head blocks of a warp's share, `count` tiles from (sequence, head block, tile) =
+// `first` on, that have a bit in `bits` (number them through, modulo 64). Behind the
+// kernel's loop and a function of its own, so that it takes none of the loop's
+// registers (called within it, 16 x 32/4 heads of 256 took 46 us instead of 40).
+template <typename T, int kTile>
+__device__ __noinline__ void walk_again(const AttendArgs& g, int3 first, int count, int64_t w,
+                                        unsigned long long bits, float2* ml, float* ring) {
+  const InfercPagedKv& kv = g.a.kv;
+  __syncwarp();  // what is written over is other lanes'
+  Cursor<kTile> at;
+  at.open(g, first.x);
+  at.hk = first.y / g.blocks;
+  at.block = first.y - at.hk * g.blocks;
+  at.tile = first.z;
+  while (count > 0 && at.b < (int)kv.batch) {
+    const int n = min(count, at.tiles - at.tile);
+    const bool begins = at.tile == 0, ends = at.tile + n == at.tiles;
+    const int head = at.hk * g.blocks + at.block;
+    if (bits >> ((at.b * (int64_t)(kv.kv_heads * g.blocks) + head) & 63) & 1) {
+      const int q0 = at.hk * g.group + at.block * g.block;
+      const int64_t part = 2 * w + (begins ? 1 : 0);
+      walk_heads<T>(g, at.b, at.hk, q0, min(g.block, (at.hk + 1) * g.group - q0),
+                    at.tile * kTile, min(at.len, (at.tile + n) * kTile),
+                    begins && ends && !g.whole, part, ml,
+                    g.whole ? ring : g.part_o + part * g.block * kv.head_dim);
+    }
+    count -= n;
+    at.tile = at.tiles - 1;
+    at.next(g);
+  }
+}
+
 // How tiles are fetched: by cp.async, by TMA, or by TMA where the scores that the
 // kernel writes are read again by the kernel behind it, so that keys and values are to
 // leave L2 first (64 sequences, 50 MB of scores: 214 -> 209 us; fp32, 32 x 12 heads:
@@ -744,6 +883,8 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
   __shared__ int64_t s_before[kThreads];
   __shared__ int64_t s_warp[kWarps];
   __shared__ float2 s_ml[kWarps * 16];  // g.whole: each warp's maxima and sums
+  __shared__ int3 s_first[kWarps];      // where a warp's share begins,
+  __shared__ unsigned long long s_odd[kWarps];  // its head blocks to be walked again
   const InfercPagedKv& kv = g.a.kv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int heads = (int)kv.kv_heads * g.blocks;
@@ -844,6 +985,10 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
   }
   Cursor<kTile> use = load;
   const int whole_len = load.len;
+  if (Heads::kPieces && lane == 0) {
+    s_first[warp] = make_int3(load.b, load.hk * g.blocks + load.block, load.tile);
+    s_odd[warp] = 0;
+  }
 
   // ---- loads: one slot at a time, the keys of a tile, then its values.
   // Kept from a tile's keys to its values:
@@ -1113,10 +1258,19 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
             if (whole) out[h * g.o_head + col] = T(x * inv);
             else po[h * d + col] = x;
           });
+      if constexpr (Heads::kPieces)
+        if (heads_of.odd() && lane == 0)
+          s_odd[warp] |= 1ull << ((use.b * (int64_t)heads + use.hk * g.blocks + use.block) & 63);
     }
     use.next(g);
   }
   if (kTma && t < count) give_up();  // a wait ran out, or the lengths changed under the kernel
+  if constexpr (Heads::kPieces) {
+    __syncwarp();
+    if (s_odd[warp])
+      walk_again<T, kTile>(g, s_first[warp], t, w, s_odd[warp], s_ml + warp * 16,
+                           reinterpret_cast<float*>(ring));
+  }
   if (!g.whole) return;
   if (count == 0 && lane < 16) s_ml[warp * 16 + lane] = make_float2(-INFINITY, 0.f);
   __syncthreads();
