@@ -1148,11 +1148,11 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
 
   int slot_out = 0;
   uint32_t phase = 0;
-  // Waits for the slot's rows; false after the time limit.
+  // Waits for the slot's rows; false, in every lane, after the time limit.
   auto wait = [&]() {
     bool done = true;
     if constexpr (kTma) {
-      done = tc::mbar_try(&full[slot_out], phase) || tc::mbar_wait(&full[slot_out], phase);
+      done = tc::warp_wait(&full[slot_out], phase);
     } else {
       asm volatile("cp.async.wait_group %0;" ::"n"(L::kSlots - 1) : "memory");
       __syncwarp();

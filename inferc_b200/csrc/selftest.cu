@@ -17,14 +17,30 @@ namespace {
 
 __device__ int g_selftest_error;
 
+// One thread waits for an arrival that never comes; then a warp waits for one
+// that comes after half of its lanes have run out of time (60 ms later at least)
+// and before the others have: the warp has to give up as one.
 __global__ void selftest_mbar_kernel(unsigned long long limit_ns) {
-  __shared__ __align__(8) uint64_t bar;
+  constexpr unsigned long long kLate = 60ull * 1000 * 1000, kLong = 1000ull * 1000 * 1000;
+  __shared__ __align__(8) uint64_t never, late;
   if (threadIdx.x == 0) {
-    tc::mbar_init(&bar, 1);
+    tc::mbar_init(&never, 1);
+    tc::mbar_init(&late, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  if (threadIdx.x == 0 && !tc::mbar_wait(&bar, 0, limit_ns)) atomicExch(&g_selftest_error, 1);
+  if (threadIdx.x < 32) {
+    bool ran_out = true;
+    if (threadIdx.x == 0) ran_out = !tc::mbar_wait(&never, 0, limit_ns);
+    __syncwarp();
+    const bool done = tc::warp_wait(&late, 0, threadIdx.x < 16 ? limit_ns : limit_ns + kLong);
+    const bool none = __ballot_sync(0xffffffffu, done) == 0;
+    if (threadIdx.x == 0 && ran_out && none) atomicExch(&g_selftest_error, 1);
+  } else if (threadIdx.x == 32) {
+    const unsigned long long t0 = tc::gclock_ns();
+    while (tc::gclock_ns() - t0 < 2 * limit_ns + kLate) __nanosleep(10000);
+    tc::mbar_arrive(&late);
+  }
   __syncthreads();
 }
 
@@ -72,7 +88,7 @@ extern "C" int inferc_dev_selftest_wait_timeout(int which, int64_t limit_us, voi
     cudaStream_t st = as_stream(stream);
     const unsigned long long ns = (unsigned long long)limit_us * 1000ull;
     if (which == 0) {
-      selftest_mbar_kernel<<<1, 32, 0, st>>>(ns);
+      selftest_mbar_kernel<<<1, 64, 0, st>>>(ns);
       IDEV_LAUNCHED();
     } else {
       void* counter = nullptr;

@@ -70,6 +70,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   }
 }
 
+// The same by a whole warp, with the same answer in every lane: lanes read the
+// clock for themselves, so a phase that completes about the limit would let some
+// go on, to instructions of the whole warp, and others give up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
+                                          unsigned long long limit_ns = kWaitLimitNs) {
+  return __all_sync(0xffffffffu, mbar_try(bar, parity) || mbar_wait(bar, parity, limit_ns));
+}
+
 // Abort path of a TMA producer thread: waits (bounded) on the full barriers
 // of the last min(issued, stages) ring generations it issued, so that no
 // copy into this CTA's shared memory is still in flight when the CTA leaves.
