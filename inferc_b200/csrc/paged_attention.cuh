@@ -1165,11 +1165,11 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       phase ^= 1;
     }
   };
-  // Gives up: no copy into this block's memory may be in flight when it leaves.
-  auto give_up = [&]() {
+  // Gives up behind `taken` slots: no copy into this block's memory may be in flight when it
+  // leaves.
+  auto give_up = [&](int taken) {
     if (lane == 0) atomicExch(g.a.flag + 1, 1);
-    const int fills = min(2 * tiles_in + (fetched ? 1 : 0), (int)L::kSlots);
-    for (int i = 0; i < fills; ++i) {
+    for (int i = fills_in_flight(tiles_in, fetched, taken); i > 0; --i) {
       tc::mbar_wait(&full[slot_out], phase);
       released();
     }
@@ -1184,7 +1184,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
   int q0 = 0, cols = 0;
   constexpr uint32_t kAll = kTile == 32 ? 0xffffffffu : (1u << (kTile & 31)) - 1;
 
-  int t = 0;
+  int t = 0, keys_taken = 0;  // of a tile whose values did not come
 #pragma unroll 1
   for (; t < count && use.b < batch; ++t) {
     if (t == 0 || use.tile == 0) {
@@ -1211,7 +1211,10 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
           g.capacity, cols, use.len - use.tile * kTile);
     heads_of.softmax();
 
-    if (!wait()) break;
+    if (!wait()) {
+      keys_taken = 1;
+      break;
+    }
     unsigned char* v_ptr = ring + slot_out * L::kSlot;
     if (kTma && mask != kAll) {  // rows that do not exist
 #pragma unroll
@@ -1264,7 +1267,7 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
     }
     use.next(g);
   }
-  if (kTma && t < count) give_up();  // a wait ran out, or the lengths changed under the kernel
+  if (kTma && t < count) give_up(2 * t + keys_taken);  // a wait ran out, or the lengths changed under the kernel
   if constexpr (Heads::kPieces) {
     __syncwarp();
     if (s_odd[warp])

@@ -57,5 +57,11 @@ PAGED_HD int64_t owner_of(int64_t t, int64_t total, int64_t warps) {
   return divide((t + 1) * warps - 1, total);
 }
 
+// Slots of a warp's ring that were filled, for the keys and values of `tiles` tiles and
+// the keys of one more (`keys`), and not taken yet: the ones a warp that gives up waits for.
+PAGED_HD int fills_in_flight(int tiles, bool keys, int taken) {
+  return 2 * tiles + (keys ? 1 : 0) - taken;
+}
+
 }  // namespace paged
 }  // namespace inferc_dev
