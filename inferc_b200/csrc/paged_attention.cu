@@ -14,25 +14,6 @@ constexpr int kSMs = 148;  // B200; elsewhere the grid runs in waves
 constexpr int kWholeTiles = 16;
 constexpr int kJoinThreads = 128;
 
-// The parts of one (sequence, head block): warp `first`'s second slot, then
-// the first slots of the warps behind it.
-struct Parts {
-  int64_t first;
-  int count;
-  __device__ __forceinline__ int64_t slot(int i) const {
-    return i == 0 ? 2 * first + 1 : 2 * (first + i);
-  }
-};
-
-// Where a (sequence, head block)'s parts are.
-__device__ __forceinline__ Parts parts_of(int64_t t0, int64_t tiles, int64_t total,
-                                          int64_t used) {
-  Parts p;
-  p.first = owner_of(t0, total, used);
-  p.count = (int)(owner_of(t0 + tiles - 1, total, used) - p.first) + 1;
-  return p;
-}
-
 // Tiles of one head block: of all sequences, and (*ahead) of those before b. By
 // the whole block; the lengths may be read while attend_kernel still runs.
 __device__ __forceinline__ int64_t all_tiles(const AttendArgs& g, int64_t b, int64_t* ahead_out,
@@ -86,8 +67,7 @@ __device__ __forceinline__ void join(const AttendArgs& g, int job, bool by_warp,
     if (left.x < 0) return;
     b = left.x;
     head = left.y;
-    parts.first = job;
-    parts.count = left.z;
+    parts = parts_within(job, left.z, g.warps);
   } else {
     b = job / heads;
     head = job - (int)b * heads;
@@ -279,6 +259,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs& g, int64_t i, int6
   pdl_wait();
   if (t == t1) return;
   const int4 start = g.starts[w];
+  if (start.x >= (int)kv.batch) return;  // that warp found no tile: the lengths changed
   // the head block that holds tile t, its place there
   int b = start.x, head = start.y;
   int64_t from = start.z + (t - w0);

@@ -976,7 +976,10 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       left -= (int64_t)load.tiles * heads;
       load.open(g, load.b + 1);
     }
-    if (load.b >= batch) return;  // only if the lengths change under the kernel
+    if (load.b >= batch) {  // only if the lengths change under the kernel
+      if (g.starts && lane == 0) g.starts[w] = make_int4(batch, 0, 0, 0);
+      return;
+    }
     const int head = (int)divide(left, load.tiles);
     load.hk = head / g.blocks;
     load.block = head - load.hk * g.blocks;

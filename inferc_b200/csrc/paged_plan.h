@@ -57,6 +57,30 @@ PAGED_HD int64_t owner_of(int64_t t, int64_t total, int64_t warps) {
   return divide((t + 1) * warps - 1, total);
 }
 
+// The parts of one (sequence, head block): warp `first`'s second slot, then
+// the first slots of the warps behind it.
+struct Parts {
+  int64_t first;
+  int count;
+  PAGED_HD int64_t slot(int i) const { return i == 0 ? 2 * first + 1 : 2 * (first + i); }
+};
+
+// `count` parts from warp `first` on. Of the `warps` there are, whatever the numbers:
+// lengths that change while they are read must not name a slot that is none.
+PAGED_HD Parts parts_within(int64_t first, int64_t count, int64_t warps) {
+  if (first > warps - 1) first = warps - 1;
+  if (first < 0) first = 0;
+  if (count > warps - first) count = warps - first;
+  return {first, count > 1 ? (int)count : 1};
+}
+
+// Those of tiles t0 .. t0 + tiles - 1 of `total`, which `used` warps share.
+PAGED_HD Parts parts_of(int64_t t0, int64_t tiles, int64_t total, int64_t used) {
+  if (total < 1) return {0, 1};
+  const int64_t first = owner_of(t0, total, used);
+  return parts_within(first, owner_of(t0 + tiles - 1, total, used) - first + 1, used);
+}
+
 // Slots of a warp's ring that were filled, for the keys and values of `tiles` tiles and
 // the keys of one more (`keys`), and not taken yet: the ones a warp that gives up waits for.
 PAGED_HD int fills_in_flight(int tiles, bool keys, int taken) {
