@@ -330,8 +330,9 @@ int inferc_dev_decode_attention(const float* q, const float* k_cache,
  * meets them. head_dim: a multiple of 8, 8..256. Caches and rows are 16-byte
  * aligned with strides that are multiples of 16 bytes. page_size * max_pages
  * is at most 2^30, batch at most 2^20. What a call writes (caches, outputs,
- * weights) has strides under which no two rows share elements. Sums, norms and
- * softmax statistics are fp32; results are rounded to dtype once.
+ * weights) has strides under which no two rows share elements, and apart from
+ * the in-place forms named below nothing that the call reads lies in it. Sums,
+ * norms and softmax statistics are fp32; results are rounded to dtype once.
  *
  * A length, page id, token range or rotary position that points outside its
  * buffer is never followed: the positions concerned are left out (attention; a
@@ -436,7 +437,7 @@ int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,
  * page_size >= min(keep, max_pages * page_size). NULL: in place, in the
  * sequence's own pages. Otherwise the pages it names are not in page_table
  * (needed when sequences share pages). weights_out: like weights, or NULL for
- * in place; of row (b, h), positions 0 .. lens[b] - 1 are written, those from
+ * in place, sharing no element with weights otherwise; of row (b, h), positions 0 .. lens[b] - 1 are written, those from
  * keep on with 0. lens_out [batch] receives min(lens[b], keep) and may not be
  * lens itself. kept [batch, kv_heads, keep] receives the old positions, -1
  * behind the last. */

@@ -930,6 +930,13 @@ int inferc_dev_paged_kv_evict(const InfercPagedKv* kv, const int32_t* dst_table,
                        ((weights_out_batch_stride == weights_batch_stride || kv->batch == 1) &&
                         (weights_out_head_stride == weights_head_stride || kv->kv_heads == 1)),
                    "PagedKVEvict: weights_out starts as weights do, but has other strides");
+    const Rows2 read{reinterpret_cast<intptr_t>(weights) / 4, kv->max_pages * kv->page_size,
+                     {{kv->batch, weights_batch_stride}, {kv->kv_heads, weights_head_stride}}};
+    const Rows2 written{reinterpret_cast<intptr_t>(weights_out) / 4, read.length,
+                        {{kv->batch, weights_out_batch_stride},
+                         {kv->kv_heads, weights_out_head_stride}}};
+    IDEV_CHECK_ARG(weights_out == weights || !rows_meet(read, written),
+                   "PagedKVEvict: weights_out must be weights or share nothing with them");
     EvictArgs e{};
     e.a.kv = *kv;
     e.a.page = FastDiv((uint32_t)kv->page_size);

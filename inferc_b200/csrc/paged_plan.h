@@ -81,6 +81,60 @@ PAGED_HD Parts parts_of(int64_t t0, int64_t tiles, int64_t total, int64_t used) 
   return parts_within(first, owner_of(t0 + tiles - 1, total, used) - first + 1, used);
 }
 
+// Rows of `length` elements at base + i * step[0].stride + j * step[1].stride.
+struct Step {
+  int64_t count, stride;
+};
+struct Rows2 {
+  int64_t base, length;
+  Step step[2];
+};
+
+// Whether two sets of rows share an element; b's own rows do not. A look at the extents
+// decides where those are apart; else each of a's rows is looked up among b's.
+inline bool rows_meet(Rows2 a, Rows2 b) {
+  auto extent = [](Rows2& r) {
+    int64_t n = r.length;
+    for (Step& s : r.step) {
+      if (s.count <= 0) return (int64_t)0;
+      if (s.count == 1) s.stride = 0;
+      if (s.stride < 0) {  // the same rows, from the other end
+        r.base += s.stride * (s.count - 1);
+        s.stride = -s.stride;
+      }
+      n += s.stride * (s.count - 1);
+    }
+    return r.length > 0 ? n : 0;
+  };
+  const int64_t n = extent(a), m = extent(b);
+  if (n == 0 || m == 0 || a.base + n <= b.base || b.base + m <= a.base) return false;
+  const bool first = b.step[0].stride >= b.step[1].stride;
+  const Step outer = b.step[first ? 0 : 1], inner = b.step[first ? 1 : 0];
+  const int64_t block = b.length + inner.stride * (inner.count - 1);
+  // indexes m of rows [m * stride, m * stride + size) that [x, x + a.length) meets
+  struct Range {
+    int64_t from, to;
+  };
+  auto meets = [&](int64_t x, Step s, int64_t size) {
+    if (s.count == 1) return Range{0, x < size && x + a.length > 0 ? 1 : 0};
+    auto floor_div = [](int64_t n, int64_t d) { return n >= 0 ? n / d : -((-n + d - 1) / d); };
+    int64_t from = floor_div(x - size, s.stride) + 1, to = floor_div(x + a.length - 1, s.stride) + 1;
+    if (from < 0) from = 0;
+    if (to > s.count) to = s.count;
+    return Range{from, to};
+  };
+  for (int64_t i = 0; i < a.step[0].count; ++i)
+    for (int64_t j = 0; j < a.step[1].count; ++j) {
+      const int64_t x = a.base + i * a.step[0].stride + j * a.step[1].stride - b.base;
+      const Range blocks = meets(x, outer, block);
+      for (int64_t k = blocks.from; k < blocks.to; ++k) {
+        const Range rows = meets(x - k * outer.stride, inner, b.length);
+        if (rows.from < rows.to) return true;
+      }
+    }
+  return false;
+}
+
 // Slots of a warp's ring that were filled, for the keys and values of `tiles` tiles and
 // the keys of one more (`keys`), and not taken yet: the ones a warp that gives up waits for.
 PAGED_HD int fills_in_flight(int tiles, bool keys, int taken) {

@@ -119,7 +119,7 @@ def PagedKVEvict(kv: PagedKV, weights: torch.Tensor, keep: int, recent: int = 0,
     lower position). They move to the front in their order, in keys, values and
     weights. dst_table: int32 [batch, pages] of pages to put the result into,
     none of them in kv.page_table (None: the sequence's own, which no other sequence may share); weights_out:
-    like weights (None: in place). Returns (lens_out, kept, weights_out): the
+    like weights, apart from them (None: in place). Returns (lens_out, kept, weights_out): the
     new lengths, a tensor apart from kv.lens; the old positions, int32 [batch,
     kv_heads, keep], -1 behind the last; and the weights."""
     return _x().evict(kv._h, weights, keep, recent, dst_table, weights_out, lens_out, kept)
