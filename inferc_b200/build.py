@@ -5,7 +5,8 @@ torch binding of the paged-cache operators (csrc/torch_paged.cpp) against it.
 
 Objects go to inferc_b200/_build/, the shared library to
 inferc_b200/libinferc_b200.so and the binding to inferc_b200/_paged.so; all are
-git-ignored build products.
+git-ignored build products. Without torch the binding is left out; the library
+needs nvcc alone.
 """
 from __future__ import annotations
 
@@ -52,12 +53,18 @@ def _compile(src: str, force: bool, verbose_ptxas: bool) -> str:
 
 
 def _build_binding(force: bool) -> None:
+    """The torch binding; without torch the library stands alone, as its C ABI does."""
     src = os.path.join(CSRC, "torch_paged.cpp")
     if not (force or _stale(BINDING, [src, LIB] + _deps())):
         return
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        print(f"torch is not installed: {os.path.basename(BINDING)} (the paged-cache operators of "
+              "inferc_b200.ops) is not built", file=sys.stderr)
+        return
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api",
                                                        "include"),

@@ -23,7 +23,11 @@ def _x():
     if _binding is None:
         from . import lib
         lib.load()  # one instance of the library, and its message when it is missing
-        from . import _paged
+        try:
+            from . import _paged
+        except ImportError as e:
+            raise ImportError("inferc_b200/_paged.so is missing or does not load: build it with "
+                              "`python -m inferc_b200.build`, torch installed") from e
         _binding = _paged
     return _binding
 
