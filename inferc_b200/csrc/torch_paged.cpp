@@ -21,9 +21,11 @@ namespace {
 
 constexpr const char* kHandle = "inferc_b200.PagedKV";
 
-// A cache descriptor as PagedKV made it, with what the checks compare to.
+// A cache descriptor as PagedKV made it, with what the checks compare to. It keeps its
+// tensors alive.
 struct Handle {
   InfercPagedKv kv;
+  at::Tensor k, v, table, lens;
   at::ScalarType type;
   int dev;
   int64_t capacity;
@@ -86,6 +88,15 @@ int64_t integer(PyObject* o) {
 Handle& handle(PyObject* o) {
   auto* h = static_cast<Handle*>(PyCapsule_GetPointer(o, kHandle));
   if (!h) throw std::runtime_error("");
+  // x.data = y, x.set_(y), a resize: the tensor is the same, its old memory may be another's
+  auto same = [](const at::Tensor& t, const void* p, const char* what) {
+    TORCH_CHECK(t.const_data_ptr() == p, "PagedKV: the memory of ", what,
+                " was replaced; make another view");
+  };
+  same(h->k, h->kv.k, "k_cache");
+  same(h->v, h->kv.v, "v_cache");
+  same(h->table, h->kv.page_table, "page_table");
+  same(h->lens, h->kv.lens, "lens");
   return *h;
 }
 
@@ -197,6 +208,10 @@ PyObject* make(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto h = std::make_unique<Handle>();
     h->type = k.scalar_type();
     h->dev = k.get_device();
+    h->k = k;
+    h->v = v;
+    h->table = table;
+    h->lens = lens;
     InfercPagedKv& kv = h->kv;
     kv = InfercPagedKv{};
     kv.k = k.data_ptr();

@@ -41,7 +41,8 @@ class PagedKV:
     positions each sequence holds, tokens being appended by the current step
     included. The tensors are read when an operator runs, so they are updated
     in place between steps (lens.add_(1), new table entries) and must outlive
-    the work queued on them."""
+    the work queued on them. Giving one of them other memory (lens.data = ...,
+    set_, resize_) ends the view: operators on it raise."""
 
     def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                  lens: torch.Tensor):
