@@ -387,7 +387,8 @@ int inferc_dev_qk_norm_rotary(const InfercHeadRotary* rot, int dtype, const void
 /* The paged form of inferc_dev_kv_append: writes `tokens` new key and value
  * rows into the cache. Sequence b's new tokens are rows cu_tokens[b] ..
  * cu_tokens[b+1] - 1 (cu_tokens: DEVICE [batch + 1], not decreasing, from 0;
- * NULL: one token per sequence, tokens == batch) and become its last
+ * NULL: one token per sequence, tokens == batch; boundaries that name rows
+ * outside 0 .. tokens - 1 are reported, the rows there are written) and become its last
  * positions, lens[b] counting them already. Rows behind the last sequence are
  * left alone, q's among them. rot may be NULL (plain append); with it keys are
  * normed and rotated on the way, and so are the queries of the same rows when

@@ -370,6 +370,8 @@ __global__ void __launch_bounds__(256, 3)
       b = o.b;
       begin = o.begin;
       count = o.count;
+      // tokens that belong to a sequence and are not among the rows
+      if (w == 0 && lane == 0 && (r.cu[0] != 0 || r.cu[kv.batch] > r.tokens)) *r.a.flag = 1;
     }
     const int64_t len = kv.lens[b], at = len - count + (t - begin);
     if (at < 0 || at >= len || len > kv.max_pages * kv.page_size) {
