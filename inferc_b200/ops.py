@@ -34,11 +34,22 @@ __all__ = ["FusedMatMulAddGELU", "FusedQKVProjection", "FusedAttention", "LayerN
            "MatMul", "Gelu", "GeluTanh", "Softmax", "Gemv", "Int4GemvRowScale",
            "Int4GemvBatched", "Argmax", "PagedKV", "PagedKVAppend", "QKNormRotary",
            "QKNormRotaryAppend", "PagedDecodeAttention", "PagedKVEvict", "RotaryTable",
-           "InfercError"]
+           "Synchronize", "InfercError"]
 
 
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def Synchronize(stream: torch.cuda.Stream | None = None) -> None:
+    """Waits for the stream (None: the current one) and raises InfercError for what the kernels
+    of its device found since the last call and could not report when they were queued: an
+    index outside its buffer (code 5, those rows were skipped), an activation that does not fit
+    fp16 (5), or a wait that ran out (4, results invalid)."""
+    if stream is None:
+        stream = torch.cuda.current_stream()
+    with torch.cuda.device(stream.device):
+        _lib.check(_lib.load().inferc_dev_stream_synchronize(stream.cuda_stream))
 
 
 def _f32(name: str, *ts: torch.Tensor) -> None:

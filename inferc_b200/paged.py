@@ -5,8 +5,8 @@ inferc_b200.ops.
 The reference keeps one dense cache per request, grown by Concat
 (src/kernels/movement.cc:142-189, src/cli/main.cpp:831-836); these are the
 batched forms a server needs. Checks raise RuntimeError as the other ops do;
-an index found out of range on the device is reported by
-inferc_dev_stream_synchronize (INFERC_ERR_RANGE) and never followed.
+an index found out of range on the device is never followed, and the next
+ops.Synchronize (inferc_dev_stream_synchronize) raises for it.
 """
 from __future__ import annotations
 
