@@ -417,7 +417,9 @@ int inferc_dev_paged_kv_append(const InfercPagedKv* kv, const InfercHeadRotary* 
  * inferc_dev_paged_decode_attention_workspace() bytes, 16-byte aligned, which
  * no other call in flight may use; calls (or captured graphs) that may overlap
  * need one each. That size depends on the sizes in kv, q_heads and on whether
- * weights are kept, not on lens; it is -1 for sizes the call would refuse. */
+ * weights are kept, not on lens: with weights 4 bytes for each query head of a
+ * sequence and each position that the table's width allows, so a table is as
+ * wide as the longest sequence needs. It is -1 for sizes the call would refuse. */
 int64_t inferc_dev_paged_decode_attention_workspace(const InfercPagedKv* kv, int64_t q_heads,
                                                     int with_weights);
 int inferc_dev_paged_decode_attention(const InfercPagedKv* kv, const void* q,

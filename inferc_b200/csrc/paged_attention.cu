@@ -348,7 +348,7 @@ Plan plan_of(const InfercPagedKv& kv, int64_t q_heads, bool weights, char* ws) {
   g.warps = std::max<int64_t>(1, std::min<int64_t>((int64_t)kSMs * shape.blocks * kWarps, most));
   // Short sequences of few heads: a block each (see attend_kernel). At most one wave of blocks,
   // whose warps take four tiles each at most; one request of 160 positions and 12 fp32 heads:
-  // 5.0 us against 9.4 us. (Longer ones would gain where all lengths are alike: 32 x 8 bf16
+  // 5.1 us against 6.9 us. (Longer ones would gain where all lengths are alike: 32 x 8 bf16
   // key heads of 2000 positions 45.7 against 52.4 us; one long sequence among short ones, or few
   // of them, loses: 1 x 8 of 1000 15.6 against 9.3 us.)
   const int64_t pairs = kv.batch * kv.kv_heads;

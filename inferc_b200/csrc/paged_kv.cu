@@ -480,7 +480,7 @@ constexpr int kMoveCluster = 8;  // blocks at most that share a (sequence, key h
 struct EvictArgs {
   Args a;
   const int32_t* dst_table;  // nullptr: in place
-  int64_t dst_stride, dst_pages;
+  int64_t dst_stride;
   float* w;
   int64_t w_batch, w_head;
   float* w_out;
@@ -945,7 +945,6 @@ int inferc_dev_paged_kv_evict(const InfercPagedKv* kv, const int32_t* dst_table,
     e.a.flag = range_flag_ptr();
     e.dst_table = dst_table;
     e.dst_stride = dst_table_stride;
-    e.dst_pages = dst_max_pages;
     e.w = weights;
     e.w_batch = weights_batch_stride;
     e.w_head = weights_head_stride;
