@@ -110,9 +110,10 @@ int read_and_clear_paged() {
   if (dev < paged::kMostDevices && !paged::g_known[dev].load()) return 0;
   int v[2] = {0, 0};
   IDEV_CUDA(cudaMemcpyFromSymbol(v, paged::g_flags, sizeof v));
-  if (v[0] | v[1]) {
-    const int z[2] = {0, 0};
-    IDEV_CUDA(cudaMemcpyToSymbol(paged::g_flags, z, sizeof z));
+  // only what was seen: the other may be raised meanwhile, by work on another stream
+  for (int i = 0; i < 2; ++i) {
+    const int z = 0;
+    if (v[i]) IDEV_CUDA(cudaMemcpyToSymbol(paged::g_flags, &z, sizeof z, i * sizeof z));
   }
   return v[0] | v[1] << 1;
 }
