@@ -14,8 +14,8 @@
 // 16 rows of queries would.
 //
 // What bounds it: every byte of K and V is read once and used for 2 flops per
-// query head, so HBM: 0.93 of the measured copy rate for 1.07 GB in 64 sequences
-// (175 us), 0.83 for one sequence of 131k positions and 8 key heads (98 us), and
+// query head, so HBM: 0.92 of the measured copy rate for 1.07 GB in 64 sequences
+// (177 us), 0.86 for one sequence of 131k positions and 8 key heads (95 us), and
 // latency below some 20 MB. mma.sync is enough (at 8 heads, 0.1 PFLOP/s of it at
 // full bandwidth); tcgen05 tiles would need 64 rows and a trip through tensor
 // memory for each 16 positions.
