@@ -130,3 +130,39 @@ def test_largest_numbers():
         c.k[..., 1:] = 0.0
         c.v[..., 2] = 1e36
         check(c, q)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_short_sequences_in_one_share(dtype):
+    """Some seventy (sequence, key head)s in every warp's share, infinities in a few of them."""
+    g = gen(8)
+    batch, hk, group, d, page = 20000, 4, 2, 16, 16
+    k, v = (randn(g, batch, hk, page, d, dtype=dtype) for _ in range(2))
+    q = randn(g, batch, hk * group, d, dtype=dtype)
+    lens = torch.randint(0, page + 1, (batch,), generator=g, device=DEV, dtype=torch.int32)
+    for x, count in ((k, 300), (v, 300)):
+        at = torch.randint(0, x.numel(), (count,), generator=g, device=DEV)
+        x.view(-1)[at] = torch.where(torch.rand(count, generator=g, device=DEV) < 0.5, 1.0,
+                                     -1.0).to(dtype) * float("inf")
+    table = torch.arange(batch, device=DEV, dtype=torch.int32)[:, None].contiguous()
+    w = torch.zeros(batch, hk, page, device=DEV)
+    out = ops.PagedDecodeAttention(q, ops.PagedKV(k, v, table, lens), weights=w)
+    sync_ok()
+    held = torch.arange(page, device=DEV) < lens[:, None]
+    kk, vv = k.double(), v.double()
+    x = (q.double().view(batch, hk, group, 1, d) * kk[:, :, None]).sum(-1) * d ** -0.5
+    x = torch.where(held[:, None, None], x, -torch.inf)
+    p = torch.where((x == -torch.inf).all(-1, keepdim=True), 0.0, torch.softmax(x, -1))
+    vv = torch.where(held[:, None, :, None], vv, 0.0)
+    want = (p[..., None] * vv[:, :, None]).sum(3).view(batch, hk * group, d)
+    got = out.double()
+    odd = ~want.isfinite()
+    assert 200 < int(odd.any(-1).sum()) < 5000
+    assert torch.equal(got[odd].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0),
+                       want[odd].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
+    # scores below 40, 16 positions: fp32 steps of 80 (d + 8) u, one rounding to the type
+    tol = half_step(dtype) * want[~odd].abs() * (1 + 2.0 ** -7) + 2.0 ** -11 * 2.0 ** -4
+    assert ((got - want)[~odd].abs() <= tol).all()
+    sums = torch.where(held[:, None], p.sum(2), 0.0)  # only positions that are held get any
+    assert torch.equal(w.isnan(), sums.isnan())
+    assert ((w - sums)[~sums.isnan()].abs() <= 2.0 ** -15 * group).all()
