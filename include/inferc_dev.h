@@ -406,7 +406,8 @@ int inferc_dev_paged_kv_append(const InfercPagedKv* kv, const InfercHeadRotary* 
  * sequence, out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j over the
  * sequence's lens[b] positions; q_heads is a multiple of kv_heads, query head h
  * reads key head h / (q_heads / kv_heads). A sequence of length 0, or a head
- * without a score above -inf, gives zeros and adds nothing to weights.
+ * without a score above -inf, gives zeros and adds nothing to weights. out may
+ * be q, with its strides.
  * Infinities and NaN in rows that are read go by the same formula (a key whose
  * score is -inf has weight 0, a value of inf gives inf); a weight below 2^-126
  * of its head's largest counts as 0.

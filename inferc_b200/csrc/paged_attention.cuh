@@ -1247,7 +1247,12 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
       }
       T* out = reinterpret_cast<T*>(g.out) + use.b * g.o_batch + q0 * g.o_head;
       float* po = g.whole ? reinterpret_cast<float*>(ring) : g.part_o + part * g.block * d;
-      heads_of.end(
+      bool odd = false;
+      if constexpr (Heads::kPieces) odd = heads_of.odd();
+      if (odd) {  // leaves nothing yet: the queries are read again, and out may be where they are
+        if (lane == 0)
+          s_odd[warp] |= 1ull << ((use.b * (int64_t)heads + use.hk * g.blocks + use.block) & 63);
+      } else heads_of.end(
           cols, d,
           [&](int h, float top, float sum) {
             if (g.whole) {
@@ -1264,13 +1269,11 @@ __global__ void __launch_bounds__(kWarps * 32, Layout<T, kDim>::kBlocks)
             if (whole) out[h * g.o_head + col] = T(x * inv);
             else po[h * d + col] = x;
           });
-      if constexpr (Heads::kPieces)
-        if (heads_of.odd() && lane == 0)
-          s_odd[warp] |= 1ull << ((use.b * (int64_t)heads + use.hk * g.blocks + use.block) & 63);
     }
     use.next(g);
   }
-  if (kTma && t < count) give_up(2 * t + keys_taken);  // a wait ran out, or the lengths changed under the kernel
+  // a wait ran out, or the lengths changed under the kernel
+  if (kTma && t < count) give_up(2 * t + keys_taken);
   if constexpr (Heads::kPieces) {
     __syncwarp();
     if (s_odd[warp])
