@@ -6,7 +6,8 @@
 // host then reports INFERC_ERR_TIMEOUT from inferc_dev_stream_synchronize and
 // the context stays usable. This file runs those wait loops on something that
 // is never signalled (an mbarrier nothing arrives at, an arrival counter no
-// CTA increments) with a caller-chosen short limit, so a test can watch the
+// CTA increments; for a warp's wait an arrival that comes too late for half of
+// its lanes) with a caller-chosen short limit, so a test can watch the
 // whole path: the wait gives up, the flag is set, the host reads and clears
 // it, and later launches work. Nothing here traps, faults or spins without a
 // bound.
